@@ -6,6 +6,7 @@ reaches a kernel without the library raises: there is no CPU fallback anywhere i
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from pathlib import Path
@@ -16,7 +17,7 @@ LIB_PATH = Path(__file__).with_name("libbpt_b200.so")
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_WORKSPACE, ERR_CUDA = range(6)
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-KV_FP8, KV_INT8 = 1, 2
+KV_FP8, KV_INT8, KV_F16, KV_BF16 = 1, 2, 3, 4
 FLAG_PDL = 1
 FLAG_KV_READY = 2
 
@@ -35,6 +36,8 @@ SIGNATURES: dict[str, list] = {
     "bpt_rms_norm_residual": [P, P, P, P, P, I64, I64, F32, I32, P],
     "bpt_qk_norm_rope_kv_write": [P, I64, I64, I64, I64, I64, P, P, P, P, F32, P, P, P, P, P, F32, F32, I64, I64, I32,
                                   P],
+    "bpt_rope_kv_append": [P, P, P, I32, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, P, P, P, I64, I32, P, P,
+                           F32, P, P, P, P, P, I32, F32, F32, P, P, I64, I64, I32, P],
     "bpt_rms_norm_int8": [P, I32, I64, P, I32, P, P, P, P, I64, I64, F32, I32, P],
     "bpt_w4a16_quantize": [P, I32, I64, I64, I64, P, P, P, P],
     "bpt_paged_decode_partials": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, P, I64, I64, I64, I64, I64, I64,
@@ -44,13 +47,17 @@ SIGNATURES: dict[str, list] = {
                          F32, P, I32, P, I64, I32, P],
     "bpt_paged_attend_noalloc": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, P, I64, I64, I64, I64, I64, I64,
                                  I64, I64, F32, P, I32, I32, P],
+    "bpt_paged_read_workspace_bytes": [I64, I64, I64, I64],
+    "bpt_paged_read": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, I64, P, P, P, F32, I64, I64, I64, I64, I64,
+                       I64, I64, I64, I64, F32, P, I32, P, P, P, I64, I32, P],
     "bpt_merge_partials": [P, P, I64, I64, I64, I64, P, I32, P],
     "bpt_kivi_decode_partials": [P, I32, I64, I64, I32, I32, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64,
                                  I64, I64, F32, P, P, P],
     "bpt_paged_kv_write": [P, P, I32, I64, I64, I64, I64, I64, I64, I64, P, P, P, P, I32, F32, F32, P, P, I64, I64, P],
     "bpt_kivi_quantize": [P, P, I32, I64, I64, I64, I64, I32, I64, P, P, P, P, P, P, I64, I64, I64, P],
 }
-RESTYPES = {"bpt_last_error": ctypes.c_char_p, "bpt_paged_attend_workspace_bytes": ctypes.c_int64}
+RESTYPES = {"bpt_last_error": ctypes.c_char_p, "bpt_paged_attend_workspace_bytes": ctypes.c_int64,
+            "bpt_paged_read_workspace_bytes": ctypes.c_int64}
 
 
 class KernelLibraryMissing(RuntimeError):
@@ -109,6 +116,22 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     if device is None:
         raise ValueError("no tensor given")
     return device
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one (kernels launch on the current device's streams only)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def as_int32(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous int32 copy of an integer tensor (itself where it is one already), out-of-range values saturated."""
+    if t.dtype == torch.int32:
+        return t.contiguous()
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise ValueError(f"expected whole numbers, got {t.dtype}")
+    return t.clamp(-(2**31), 2**31 - 1).to(torch.int32).contiguous() if t.dtype == torch.int64 else t.to(torch.int32).contiguous()
 
 
 def device_error() -> int:

@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from bpt_b200 import _lib
-from bpt_b200._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
+from bpt_b200._lib import as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
 
 
 @dataclass
@@ -57,10 +57,11 @@ class QuantKV:
 
 @dataclass
 class PagedQuantKV:
-    """One layer's paged, quantized KV cache.
+    """One layer's paged KV cache, quantized or 16-bit.
 
     kind         "fp8": E4M3 bytes (uint8), k_scale / v_scale are per-tensor floats
                  "int8": int8 codes, k_scale / v_scale are fp16 [num_blocks, block_size, Hkv] (one per token, head)
+                 "bf16", "f16": the keys and values themselves (bfloat16 / float16); the scales are unused
     k_pool/v_pool [num_blocks, block_size, Hkv, D]
     block_table  int32 [B, n_blocks]: physical block of each sequence's logical block j (tokens j*bs .. j*bs+bs-1)
     """
@@ -92,7 +93,7 @@ class PagedQuantKV:
 
     def bytes_per_token(self) -> float:
         """Bytes one token occupies across this layer's KV heads, scales included."""
-        per = 2 * self.kv_heads * self.head_dim
+        per = 2 * self.kv_heads * self.head_dim * (2 if self.kind in ("bf16", "f16") else 1)
         return float(per + (2 * self.kv_heads * 2 if self.kind == "int8" else 0))
 
 
@@ -136,6 +137,101 @@ def _lengths(lengths: torch.Tensor) -> torch.Tensor:
     return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else lengths.to(torch.int32).contiguous()
 
 
+# kind -> (the library's code, the pools' dtypes)
+_FORMATS = {"fp8": (_lib.KV_FP8, (torch.uint8, torch.float8_e4m3fn)), "int8": (_lib.KV_INT8, (torch.int8, torch.uint8)),
+            "f16": (_lib.KV_F16, (torch.float16,)), "bf16": (_lib.KV_BF16, (torch.bfloat16,))}
+
+
+def pool_format(kv: PagedQuantKV):
+    """(format code, k scale, v scale, k scale pool, v scale pool, blocks, block size, KV heads, head dim) of a paged cache of
+    any kind, checked."""
+    if kv.kind not in _FORMATS:
+        raise ValueError(f"kind must be one of {', '.join(map(repr, _FORMATS))}, got {kv.kind!r}")
+    code, dtypes = _FORMATS[kv.kind]
+    k, v = kv.k_pool, kv.v_pool
+    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError(f"pools must be contiguous [num_blocks, block_size, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype not in dtypes or v.dtype not in dtypes:
+        raise ValueError(f"{kv.kind!r} pools must be {dtypes[0]}, got {k.dtype} and {v.dtype}")
+    nb, bs, hkv, d = k.shape
+    if kv.block_size != bs:
+        raise ValueError(f"block_size is {kv.block_size}, the pools' blocks hold {bs}")
+    if kv.kind == "int8":
+        for s in (kv.k_scale, kv.v_scale):
+            if not (isinstance(s, torch.Tensor) and s.dtype == torch.float16 and tuple(s.shape) == (nb, bs, hkv)
+                    and s.is_contiguous() and s.device == k.device):
+                raise ValueError("int8 pools need fp16 k_scale / v_scale of shape [num_blocks, block_size, Hkv]")
+        return code, 1.0, 1.0, kv.k_scale, kv.v_scale, nb, bs, hkv, d
+    if kv.kind == "fp8":
+        return code, float(kv.k_scale), float(kv.v_scale), None, None, nb, bs, hkv, d
+    return code, 1.0, 1.0, None, None, nb, bs, hkv, d
+
+
+def paged_read_split(batch: int, heads: int, keys: int, sms: int = 148) -> int:
+    """Keys per CTA of the any-format decode read, whose CTA covers one KV head (eight query heads) of one sequence: about
+    six CTAs per SM at the longest length, at least 128 keys (two groups of 16 for each of its four warps)."""
+    split = -(-batch * heads * keys // (6 * sms))
+    return max(128, -(-split // 64) * 64)
+
+
+def _row_tensor(name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype) -> torch.Tensor | None:
+    """An optional per-row argument, in the dtype the kernels take."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    return as_int32(t) if dtype == torch.int32 else t.to(dtype).contiguous()
+
+
+def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_slopes, key_starts, out=None,
+                workspace=None, partials=False, flags=0):
+    """`attend` (or, with partials, `decode_attention`) over a paged cache of any kind with any of the score options."""
+    device = require_cuda(q, lengths, kv.k_pool, kv.v_pool, kv.block_table, alibi_slopes, key_starts, out, workspace)
+    code, ks, vs, kss, vss, nb, bs, hkv, d = pool_format(kv)
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % hkv:
+        raise ValueError(f"pool shape {tuple(kv.k_pool.shape)} does not match q {tuple(q.shape)}")
+    b, hq, _ = q.shape
+    table = kv.block_table
+    if table.dim() != 2 or table.shape[0] != b or table.dtype != torch.int32 or table.stride(1) != 1:
+        raise ValueError(f"the block table must be int32 [{b}, blocks], got {table.dtype} {tuple(table.shape)}")
+    if tuple(lengths.shape) != (b,):
+        raise ValueError(f"lengths must be [{b}], got {tuple(lengths.shape)}")
+    if window < 0 or softcap < 0:
+        raise ValueError(f"window and softcap must not be negative, got {window} and {softcap}")
+    with on_device(device):
+        q, lengths = _q_view(q), as_int32(lengths)
+        slopes = _row_tensor("alibi_slopes", alibi_slopes, (hq,), torch.float32)
+        starts = _row_tensor("key_starts", key_starts, (b,), torch.int32)
+        tokens = kv.tokens if tokens is None else tokens
+        keys = max(tokens, 1) if partials or not window else max(1, min(tokens, window + 15))  # a window starts anywhere
+        if split is None:
+            split = paged_read_split(b, hkv * -(-hq // hkv // 8), keys, _sms(device))
+        if split % 16 or split <= 0:
+            raise ValueError(f"split {split} must be a multiple of 16")
+        n_splits = -(-keys // split)
+        part_out = part_lse = None
+        need = 0
+        if partials:
+            part_out = torch.empty((b, hq, n_splits, d), dtype=torch.float32, device=device)
+            part_lse = torch.empty((b, hq, n_splits), dtype=torch.float32, device=device)
+        else:
+            if out is None:
+                out = torch.empty((b, hq, d), dtype=torch.float32, device=device)
+            elif tuple(out.shape) != (b, hq, d) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{b}, {hq}, {d}] tensor")
+            if n_splits > 1 and workspace is None:
+                workspace = _zeroed_workspace(int(lib().bpt_paged_read_workspace_bytes(b, hq, d, n_splits)), device)
+            need = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        st = lib().bpt_paged_read(
+            ptr(q), dtype_code(q.dtype), q.stride(0), q.stride(1), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs, ptr(kss),
+            ptr(vss), ptr(table), table.stride(0) if b > 1 else table.shape[1], table.shape[1], ptr(lengths), ptr(starts),
+            ptr(slopes), float(softcap), int(window), b, hq, hkv, d, bs, nb, split, n_splits, float(scale), ptr(out),
+            dtype_code(out.dtype) if out is not None else 0, ptr(part_out), ptr(part_lse), ptr(workspace), need, flags,
+            stream_of(device))
+    check(st, "decode_attention (paged)" if partials else "attend (paged)")
+    return (part_out, part_lse) if partials else out
+
+
 def _paged_args(q: torch.Tensor, kv: PagedQuantKV):
     if kv.kind not in ("fp8", "int8"):
         raise ValueError(f"kind must be 'fp8' or 'int8', got {kv.kind!r}")
@@ -168,14 +264,22 @@ def decode_attention(
     tokens: int | None = None,
     split: int | None = None,
     num_warps: int = 1,
+    softcap: float = 0.0,
+    window: int = 0,
+    alibi_slopes: torch.Tensor | None = None,
+    key_starts: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Partial attentions of one query per head over a quantized cache, one per split of `split` tokens.
 
     q [B, Hq, D] (fp32, fp16 or bf16); lengths [B] int32. `tokens` bounds the launch when the caller knows the
     longest length (no host sync on lengths.max()). Returns (out [B, Hq, S, D], lse [B, Hq, S]) in fp32; a split
-    past a row's end has out 0 and lse -inf, so `merge_partials` ignores it.
+    past a row's end has out 0 and lse -inf, so `merge_partials` ignores it. `softcap`, `window`, `alibi_slopes` and
+    `key_starts` (paged caches only): see `attend`.
     """
     del num_warps
+    if _any_format(kv, softcap, window, alibi_slopes, key_starts):
+        return _paged_read(q, kv, lengths, scale, tokens=tokens, split=split, softcap=softcap, window=window,
+                           alibi_slopes=alibi_slopes, key_starts=key_starts, partials=True)
     device = require_cuda(q, lengths, kv.k_codes if not isinstance(kv, PagedQuantKV) else kv.k_pool)
     q = _q_view(q)
     lengths = _lengths(lengths)
@@ -257,6 +361,28 @@ def attend_workspace(batch: int, q_heads: int, head_dim: int, n_splits: int, dev
     return ws
 
 
+def _zeroed_workspace(need: int, device: torch.device) -> torch.Tensor:
+    """A workspace whose tickets are zero. While a CUDA graph is captured it is the graph's own (zeroed by every replay), so
+    that two graphs never share one; otherwise the device's and stream's cached one (`attend_workspace`)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(need, dtype=torch.uint8, device=device)
+    key = (device.index or 0, stream_of(device))
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.numel() < need:
+        ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+    return ws
+
+
+def _any_format(kv, softcap, window, alibi_slopes, key_starts) -> bool:
+    """Whether a call takes the any-format read: 16-bit pages, or a score option over pages of any kind."""
+    options = bool(softcap) or bool(window) or alibi_slopes is not None or key_starts is not None
+    if not isinstance(kv, PagedQuantKV):
+        if options:
+            raise ValueError("softcap, window, alibi_slopes and key_starts need a paged cache")
+        return False
+    return options or kv.kind in ("bf16", "f16")
+
+
 def attend(
     q: torch.Tensor,
     kv: QuantKV | PagedQuantKV,
@@ -265,15 +391,28 @@ def attend(
     *,
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
+    softcap: float = 0.0,
+    window: int = 0,
+    alibi_slopes: torch.Tensor | None = None,
+    key_starts: torch.Tensor | None = None,
     **launch,
 ) -> torch.Tensor:
-    """Decode attention over a quantized cache: [B, Hq, D] (fp32 unless `out` says otherwise).
+    """Decode attention over a cache: [B, Hq, D] (fp32 unless `out` says otherwise).
 
     Paged caches run one fused launch: the splits of a sequence are merged by the last of its CTAs to finish.
     KIVI caches run the split kernel, then the merge kernel. `pdl=True` launches with programmatic dependent
     launch; `kv_ready=True` adds the promise that the lengths, block table and pools are not written by the
     kernel this call follows, so the persistent kernel starts copying pages before it waits on that kernel.
+
+    Paged caches of any kind take, and 16-bit pages ("bf16", "f16") always run, the any-format kernel with: `softcap` c > 0
+    (scores c * tanh(score / c)), `window` w > 0 (only the last w keys are seen), `alibi_slopes` fp32 [Hq] (a score falls
+    by slope * distance) and `key_starts` int32 [B] (the first key each sequence sees). A sequence that sees no key
+    gives zeros.
     """
+    if _any_format(kv, softcap, window, alibi_slopes, key_starts):
+        return _paged_read(q, kv, lengths, scale, tokens=launch.get("tokens"), split=launch.get("split"), softcap=softcap,
+                           window=window, alibi_slopes=alibi_slopes, key_starts=key_starts, out=out, workspace=workspace,
+                           flags=_lib.FLAG_PDL if launch.get("pdl") else 0)
     if not isinstance(kv, PagedQuantKV):  # the merge writes straight into `out` when one is given
         if launch.get("split") is None:
             launch = dict(launch, split=kivi_attend_split(q.shape[0], kv.k_codes.shape[1],

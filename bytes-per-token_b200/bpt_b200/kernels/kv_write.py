@@ -14,8 +14,8 @@ from __future__ import annotations
 import torch
 
 from bpt_b200 import _lib
-from bpt_b200._lib import check, dtype_code, lib, ptr, require_cuda, stream_of
-from bpt_b200.kernels.kv_attention import PagedQuantKV, QuantKV
+from bpt_b200._lib import FLAG_PDL, as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
+from bpt_b200.kernels.kv_attention import PagedQuantKV, QuantKV, pool_format
 
 
 def quantize_kv_paged(k: torch.Tensor, v: torch.Tensor, kv: PagedQuantKV, write_blocks: torch.Tensor,
@@ -44,6 +44,76 @@ def quantize_kv_paged(k: torch.Tensor, v: torch.Tensor, kv: PagedQuantKV, write_
         ptr(k), ptr(v), dtype_code(k.dtype), k.stride(0), k.stride(1), k.stride(2), b, hkv, q, d, ptr(wb), ptr(wo),
         ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs, ptr(kss), ptr(vss), bs, nb, stream_of(device))
     check(st, "quantize_kv_paged")
+
+
+def rope_table(positions: int, rotary_dim: int, theta: float = 1e6, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos, sin [positions, rotary_dim / 2] in fp32 for angles p * theta^(-2i / rotary_dim) (engine/rope.py:12-28), from
+    angles in 64 bits: in 32, position 100,000 is off by up to 0.004 radians."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even, got {rotary_dim}")
+    inv = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
+    return angle.cos().float(), angle.sin().float()
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [T, H, D], or a copy of it whose rows start on 16 bytes."""
+    unit = 16 // x.element_size()
+    if x.stride(2) == 1 and x.stride(0) % unit == 0 and x.stride(1) % unit == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: PagedQuantKV, positions: torch.Tensor,
+                   cos: torch.Tensor, sin: torch.Tensor, write_blocks: torch.Tensor, write_offsets: torch.Tensor, *,
+                   q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                   interleaved: bool = False, q_out: torch.Tensor | None = None, pdl: bool = False) -> torch.Tensor:
+    """Rotate T new tokens' q [T, Hq, D] and k [T, Hkv, D] and store k, v [T, Hkv, D] in the pools; returns the rotated q.
+
+    positions, write_blocks, write_offsets: [T] whole numbers: each token's row of cos / sin (fp32 [positions, R / 2]; the
+    first R dims rotate, the rest pass) and the slot that receives its key and value; slots of one call must be distinct. A
+    token with write_blocks -1 is padding: nothing of it is read, stored or written to q_out. q, k and v may be views of one
+    projection's output (any token and head strides). `q_norm` / `k_norm` [D]: RMSNorm weights applied per head before
+    the rotation. `interleaved`: dims 2i and 2i + 1 rotate together instead of i and i + R / 2. Rows are rounded once, from
+    fp32, to q_out's type (q's) and to the cache's format.
+    """
+    device = require_cuda(q, k, v, kv.k_pool, kv.v_pool, positions, cos, sin, write_blocks, write_offsets, q_norm, k_norm,
+                          q_out)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"q must be [T, Hq, D], k and v [T, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    code, ks, vs, kss, vss, nb, bs, pool_heads, pool_dim = pool_format(kv)
+    if (hkv, d) != (pool_heads, pool_dim):
+        raise ValueError(f"k has {hkv} heads of {d}, the pool {pool_heads} of {pool_dim}")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError("cos and sin must be float32 [positions, rotary / 2]")
+    for w in (q_norm, k_norm):
+        if w is not None and (tuple(w.shape) != (d,) or w.dtype != q.dtype):
+            raise ValueError(f"norm weights must be [{d}] in {q.dtype}")
+    for x in (positions, write_blocks, write_offsets):
+        if x.numel() != t:
+            raise ValueError(f"positions, write_blocks and write_offsets must hold {t} entries")
+    if q_out is None:
+        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
+    elif tuple(q_out.shape) != (t, hq, d) or q_out.dtype != q.dtype or not q_out.is_contiguous():
+        raise ValueError(f"q_out must be a contiguous [{t}, {hq}, {d}] tensor of {q.dtype}")
+    with on_device(device):
+        q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+        cos, sin = cos.contiguous(), sin.contiguous()
+        q_norm = q_norm if q_norm is None else q_norm.contiguous()
+        k_norm = k_norm if k_norm is None else k_norm.contiguous()
+        pos, wb, wo = as_int32(positions), as_int32(write_blocks), as_int32(write_offsets)
+        st = lib().bpt_rope_kv_append(
+            ptr(q), ptr(k), ptr(v), dtype_code(q.dtype), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+            v.stride(1), t, hq, hkv, d, 2 * cos.shape[1], ptr(pos), ptr(cos), ptr(sin), cos.shape[0], int(interleaved),
+            ptr(q_norm), ptr(k_norm), float(eps), ptr(q_out), ptr(wb), ptr(wo), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs,
+            ptr(kss), ptr(vss), bs, nb, FLAG_PDL if pdl else 0, stream_of(device))
+    check(st, "rope_kv_append")
+    return q_out
 
 
 def empty_quant_kv(batch: int, kv_heads: int, tokens: int, head_dim: int, bits: int, group: int, device,

@@ -46,6 +46,7 @@ enum DeviceError : int {
   kDevErrTimeout = 1,      // an mbarrier wait gave up
   kDevErrBlockIndex = 2,   // a block-table entry outside [0, num_blocks)
   kDevErrSlotIndex = 3,    // a write slot outside the block
+  kDevErrPosition = 4,     // a position outside the cos / sin table
 };
 
 __device__ __forceinline__ void record_error(int code) { atomicCAS(&g_device_error, 0, code); }

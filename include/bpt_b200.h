@@ -43,6 +43,8 @@ extern "C" {
 /* KV cache formats */
 #define BPT_KV_FP8 1  /* E4M3 bytes, one fp32 scale per tensor (K and V each)            */
 #define BPT_KV_INT8 2 /* symmetric int8 codes, one fp16 scale per (token, KV head)      */
+#define BPT_KV_F16 3  /* fp16 values (bpt_rope_kv_append, bpt_paged_read, bpt_paged_prefill) */
+#define BPT_KV_BF16 4 /* bf16 values (the same)                                         */
 
 /* launch flags */
 #define BPT_FLAG_PDL 1 /* launch with programmatic dependent launch (prologue overlaps the previous kernel) */
@@ -62,7 +64,8 @@ extern "C" {
 int bpt_abi_version(void);
 const char* bpt_last_error(void);
 /* Synchronizes the device, returns the first device-side error code recorded since the last call and clears
- * it (0 = none, 1 = a bounded wait ran out, 2 = a block-table entry out of range, 3 = a slot out of range). */
+ * it (0 = none, 1 = a bounded wait ran out, 2 = a block-table entry out of range, 3 = a slot out of range,
+ * 4 = a position outside the cos / sin table). */
 int bpt_device_error(void);
 
 /* ---- W4A16: INT4 group-wise weight-only linear ---------------------------------------------------------------
@@ -152,6 +155,28 @@ int bpt_paged_attend(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_s
                      int64_t split, int64_t n_splits, float sm_scale, void* out, int out_dtype, void* workspace,
                      int64_t workspace_bytes, int flags, void* stream);
 
+/* Decode attention over a paged cache of any format (BPT_KV_*), with the masks and score changes of current models. Query b
+ * sits at position p = lengths[b] - 1 and sees the keys j with max(0, key_starts[b], p - window + 1) <= j <= p:
+ *   s_j = softcap tanh(sm_scale q.k_j / softcap) - alibi_slopes[head] (p - j)
+ * softcap 0: no cap; window 0: no window; key_starts (int32 [B]) and alibi_slopes (fp32 [Hq]) may be NULL. No visible key
+ * gives 0. block_table int32 [B, bt_width], row stride bt_stride; a length beyond the table's pages is cut to them and
+ * recorded (device error 2), keys of a block out of range are left out and recorded.
+ * With out_partial NULL: the merged attention out [B, Hq, D] in out_dtype; a sequence takes up to n_splits CTAs of `split`
+ * keys per KV head (the last takes the rest, whatever its length), joined by the last to finish. n_splits > 1 needs
+ * `workspace`: bpt_paged_read_workspace_bytes(...) bytes, ZEROED before its first use, tickets left at zero by every call;
+ * calls that may overlap need workspaces of their own. Otherwise out_partial f32 [B, Hq, n_splits, D] and lse_partial f32
+ * [B, Hq, n_splits] receive the parts (keys [i split, (i + 1) split); out 0, lse -inf where none is visible).
+ * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024, split a multiple of 16.
+ * Replaces: as bpt_paged_attend, for the reference's unquantized pages too (engine/kv_cache.py:98-169). */
+int64_t bpt_paged_read_workspace_bytes(int64_t B, int64_t Hq, int64_t D, int64_t n_splits);
+int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, const void* k_pool,
+                   const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales, const void* v_scales,
+                   const int32_t* block_table, int64_t bt_stride, int64_t bt_width, const int32_t* lengths,
+                   const int32_t* key_starts, const float* alibi_slopes, float softcap, int64_t window, int64_t B,
+                   int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size, int64_t num_blocks, int64_t split,
+                   int64_t n_splits, float sm_scale, void* out, int out_dtype, float* out_partial, float* lse_partial,
+                   void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
 /* bpt_paged_attend without a workspace argument, for callers that cannot allocate device memory: serving
  * engines that hand all free HBM to their paged KV pool at start-up (so a later cudaMalloc fails or fragments
  * the pool), runtimes whose memory policy forbids device allocation after initialization, and foreign-language
@@ -238,6 +263,26 @@ int bpt_qk_norm_rope_kv_write(const void* qkv, int64_t ld, int64_t B, int64_t Hq
                               void* q_out, const int32_t* write_blocks, const int32_t* write_offsets, void* k_pool,
                               void* v_pool, float k_scale, float v_scale, int64_t block_size, int64_t num_blocks,
                               int flags, void* stream);
+
+/* T new tokens' q [T, Hq, D], k and v [T, Hkv, D] (dtype; strides in elements for token and head, unit stride over D):
+ * an optional RMSNorm per head of q (q_norm [D] in dtype, NULL for none) and of k (k_norm), rotation of the first `rotary`
+ * dims of q and k by the angles of their positions, q -> q_out [T, Hq, D] (dtype, contiguous), k and v -> slot
+ * write_offsets[t] of block write_blocks[t] of the pools [num_blocks, block_size, Hkv, D] in the cache format `kind`.
+ *   cos, sin     fp32 [table_rows, rotary / 2]: row p holds the angles of position p (positions int32 [T])
+ *   interleaved  0: dim i rotates with dim i + rotary / 2; otherwise dim 2i with dim 2i + 1
+ * fp32 arithmetic, one rounding to q_out's or the cache's format (BPT_KV_FP8 and BPT_KV_INT8 as bpt_paged_kv_write, from
+ * the fp32 rotation). A token whose write_blocks entry is -1 is padding: nothing of it is read or written. A position
+ * outside the table (device error 4) skips the token; a block or offset out of range (2, 3) stores no k and v. Slots of
+ * one call must be distinct. D in {64, 128, 256}, rotary a multiple of 16 from 16 to D; rows of q, k, v start
+ * on 16 bytes. Replaces: rope.apply (engine/rope.py:31-43), q_norm / k_norm (engine/model.py:63-70) and the cache write
+ * (engine/kv_cache.py:150-161) for any number of tokens and any of the cache's formats. */
+int bpt_rope_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_t, int64_t q_stride_h,
+                       int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, int64_t T,
+                       int64_t Hq, int64_t Hkv, int64_t D, int64_t rotary, const int32_t* positions, const float* cos,
+                       const float* sin, int64_t table_rows, int interleaved, const void* q_norm, const void* k_norm,
+                       float eps, void* q_out, const int32_t* write_blocks, const int32_t* write_offsets, void* k_pool,
+                       void* v_pool, int kind, float k_scale, float v_scale, void* k_scales, void* v_scales,
+                       int64_t block_size, int64_t num_blocks, int flags, void* stream);
 
 /* RMSNorm fused with per-token symmetric INT8 quantization (the activation quantizer before a W8A8 linear):
  * for every row of x [rows, d] (x_dtype, row stride x_row_stride elements, unit inner stride) and weight [d]
