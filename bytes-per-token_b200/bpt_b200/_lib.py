@@ -50,6 +50,9 @@ SIGNATURES: dict[str, list] = {
     "bpt_paged_read_workspace_bytes": [I64, I64, I64, I64],
     "bpt_paged_read": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, I64, P, P, P, F32, I64, I64, I64, I64, I64,
                        I64, I64, I64, I64, F32, P, I32, P, P, P, I64, I32, P],
+    "bpt_paged_prefill_workspace_bytes": [I64, I64, I64, I64, I64, I64],
+    "bpt_paged_prefill": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, I64, P, P, P, P, P, P, F32, I64, I64, I64, I64,
+                          I64, I64, I64, I64, I64, F32, P, P, I64, I32, P],
     "bpt_merge_partials": [P, P, I64, I64, I64, I64, P, I32, P],
     "bpt_kivi_decode_partials": [P, I32, I64, I64, I32, I32, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64,
                                  I64, I64, F32, P, P, P],
@@ -57,7 +60,7 @@ SIGNATURES: dict[str, list] = {
     "bpt_kivi_quantize": [P, P, I32, I64, I64, I64, I64, I32, I64, P, P, P, P, P, P, I64, I64, I64, P],
 }
 RESTYPES = {"bpt_last_error": ctypes.c_char_p, "bpt_paged_attend_workspace_bytes": ctypes.c_int64,
-            "bpt_paged_read_workspace_bytes": ctypes.c_int64}
+            "bpt_paged_read_workspace_bytes": ctypes.c_int64, "bpt_paged_prefill_workspace_bytes": ctypes.c_int64}
 
 
 class KernelLibraryMissing(RuntimeError):

@@ -1,0 +1,418 @@
+// Prefill attention over a paged cache of any format: the new tokens of a ragged batch attend over their sequences' pages, with
+// score caps, distance bias, sliding windows, documents (a first visible key per token) and a shared prefix.
+//
+//   s_j = cap tanh(scale q.k_j / cap) - slope |p - j|,  out = sum_j softmax(s)_j v_j  over  lo <= j < hi,
+//   lo = max(0, start, p - window + 1), hi = min(length, max(p + 1, prefix));  no visible key gives 0.
+//
+// One pass over the keys with the running maximum and sum. The query heads of a KV head are packed with their tokens into
+// rows (row = token * rep + head), so every key and value brought in serves all of them; a row carries its own interval
+// [lo, hi), and a tile of rows visits only the keys between its smallest lo and largest hi.
+//
+// This kernel multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. A CTA that
+// has few companions takes a part of its keys only; the parts of a tile are joined by the last of its CTAs to finish.
+#include "paged_prefill.cuh"
+
+namespace bpt {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 16 * kWarps;
+constexpr int kKeys = 64;
+
+template <int KIND, int D>
+struct PrefillShape {
+  static constexpr int RB = D * kElemBytes<KIND>;
+  static constexpr int kScaleBytes = KIND == BPT_KV_INT8 ? kKeys * 4 : 0;  // 16 K then 16 V scales (fp16) per 16 keys
+  static constexpr int kStage = 2 * kKeys * RB + kScaleBytes + 16;          // keys, values, scales, a flag per 16 keys
+  static constexpr int kQ = kWarps * (D / 16) * 32 * 16;                    // the q fragments
+  static constexpr int kStages = 2;
+  static constexpr int kSmem = kStages * kStage + kQ;
+};
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillArgs a) {
+  using S = PrefillShape<KIND, D>;
+  constexpr int RB = S::RB;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int s_range[2][kWarps];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int hk = blockIdx.y, sp = blockIdx.z;
+  pdl_launch_dependents();
+  pdl_wait();
+  const TileAt at = find_tile(a, kRows, int(blockIdx.x));
+  if (at.b < 0) return;
+  const int b = at.b;
+  const int len = sequence_length(a, b, tid == 0 && hk == 0 && sp == 0);
+
+  // this lane's rows g and g + 8 of its warp's 16
+  RowAt row[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) row[i] = row_at(a, at, at.row0 + warp * 16 + g + 8 * i, hk, len);
+  {  // the keys that the CTA's rows, and that all rows of this warp, see
+    int lo = INT_MAX, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (row[i].hi > row[i].lo) {
+        lo = min(lo, row[i].lo);
+        hi = max(hi, row[i].hi);
+      }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      s_range[0][warp] = lo;
+      s_range[1][warp] = hi;
+    }
+  }
+  const int all_lo = __reduce_max_sync(0xffffffffu, max(row[0].lo, row[1].lo));
+  const int all_hi = __reduce_min_sync(0xffffffffu, min(row[0].hi, row[1].hi));
+  __syncthreads();
+  int lo = s_range[0][0], hi = s_range[1][0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) {
+    lo = min(lo, s_range[0][w]);
+    hi = max(hi, s_range[1][w]);
+  }
+  const int base = lo == INT_MAX ? 0 : lo & ~15;
+  const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
+  if (sp >= max(parts, 1)) return;
+  const int from = base + sp * a.split;  // of the part; keys below lo are masked by the rows
+  const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
+  const int steps = (to - from + kKeys - 1) / kKeys;
+
+  const uint32_t smem_u = smem_u32(smem);
+  auto stage = [&](int st) { return smem_u + st * S::kStage; };
+  auto scales_of = [&](int st, int w) {
+    return reinterpret_cast<uint16_t*>(smem + st * S::kStage + 2 * kKeys * RB) + 32 * w;
+  };
+  auto flag_of = [&](int st) { return reinterpret_cast<uint32_t*>(smem + st * S::kStage + 2 * kKeys * RB + S::kScaleBytes); };
+  // warp w brings keys 16 w .. 16 w + 15 of a step
+  GroupLoader<KIND, D> loader(a.src, b, hk, from + 16 * warp, kKeys, steps, max(from, lo), to, lane);
+  auto request = [&](int i, int st) {
+    if (i < steps)
+      loader.request(i, stage(st) + warp * 16 * RB, stage(st) + (kKeys + warp * 16) * RB, flag_of(st) + warp);
+    cp_async_commit();
+  };
+  request(0, 0);
+
+  // q as A fragments in shared memory, [k-step][lane]: scaled by a power of two into [-1, 1] for f16 products of bf16
+  // queries (exact, but for parts 2^-24 below the row's largest), as it is otherwise
+  uint4* qs = reinterpret_cast<uint4*>(smem + S::kStages * S::kStage) + warp * (D / 16) * 32;
+  float unit[2];
+  {
+    float amax[2] = {0.f, 0.f};
+    if (KIND != BPT_KV_BF16 && a.q_dtype == BPT_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (row[i].q >= 0)
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              amax[i] = fmaxf(amax[i], fabsf(load_16(a.q, a.q_dtype, row[i].q + q_dim<KIND>(j, t, e))));
+        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1));
+        amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 2));
+      }
+    }
+    const float2 u0 = unit_range(amax[0]), u1 = unit_range(amax[1]);
+    unit[0] = u0.y;
+    unit[1] = u1.y;
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t f[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = 0.f, y = 0.f;
+          if (row[i].q >= 0) {
+            x = load_16(a.q, a.q_dtype, row[i].q + q_dim<KIND>(j, t, 2 * e)) * (i ? u1.x : u0.x);
+            y = load_16(a.q, a.q_dtype, row[i].q + q_dim<KIND>(j, t, 2 * e + 1)) * (i ? u1.x : u0.x);
+          }
+          f[2 * e + i] = pack2<KIND>(x, y);
+        }
+      qs[j * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+    }
+    __syncwarp();
+  }
+  const bool cap = a.softcap > 0.f;
+  const float cap_out = a.softcap * kLog2e;
+  float mul[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float raw = a.sm_scale * unit[i] * a.src.k_scale;
+    mul[i] = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
+  }
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+
+  for (int i = 0; i < steps; ++i) {
+    const int st = i & 1, key0 = from + i * kKeys;
+    if constexpr (KIND == BPT_KV_INT8) loader.place(scales_of(st, warp));
+    __syncthreads();  // everyone is done with the stage refilled next
+    request(i + 1, st ^ 1);
+    cp_async_wait<1>();
+    __syncthreads();  // this step's keys and values have landed
+    float s[kKeys / 8][4];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int n = 0; n < kKeys / 16; ++n) {
+      scores16<KIND, D>(stage(st) + n * 16 * RB, lane, [&](int j) {
+        const uint4 u = qs[j * 32 + lane];
+        return MmaRows{{u.x, u.y, u.z, u.w}};
+      }, s[2 * n], s[2 * n + 1]);
+    }
+    const bool masked = key0 < all_lo || key0 + kKeys > all_hi;
+    const uint4 bad = *reinterpret_cast<const uint4*>(flag_of(st));
+    const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i2 = e >> 1, key = key0 + 8 * n + 2 * t + (e & 1);
+        float x = s[n][e];
+        if constexpr (KIND == BPT_KV_INT8) x *= __half2float(reinterpret_cast<const __half*>(scales_of(st, n >> 1))[8 * (n & 1) + 2 * t + (e & 1)]);
+        x *= mul[i2];
+        if (cap) x = capped(x, cap_out);
+        if (a.slopes) x = fmaf(row[i2].slope, fabsf(float(key - row[i2].pos)), x);
+        if (masked && (key < row[i2].lo || key >= row[i2].hi)) x = -INFINITY;
+        if (any_bad) {
+          const uint32_t w = n >> 1 == 0 ? bad.x : n >> 1 == 1 ? bad.y : n >> 1 == 2 ? bad.z : bad.w;
+          if (w >> (n & 1) & 1u) x = -INFINITY;
+        }
+        s[n][e] = x;
+        top[i2] = fmaxf(top[i2], x);
+      }
+    }
+    float off[2];
+#pragma unroll
+    for (int i2 = 0; i2 < 2; ++i2) {
+      top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 1));
+      top[i2] = fmaxf(top[i2], __shfl_xor_sync(0xffffffffu, top[i2], 2));
+      const float to_m = fmaxf(m[i2], top[i2]);
+      off[i2] = to_m == -INFINITY ? 0.f : to_m;
+      const float shrink = exp2_approx(m[i2] - off[i2]);
+      m[i2] = to_m;
+      l[i2] *= shrink;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][2 * i2] *= shrink;
+        o[n][2 * i2 + 1] *= shrink;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kKeys / 16; ++n) {
+      // The probabilities enter the product rounded to 16 bits (as any operand of these matrix instructions); the sum that
+      // divides them is taken before the rounding, in fp32.
+      uint32_t p[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+          float x = exp2_approx(s[2 * n + k][2 * i2] - off[i2]), y = exp2_approx(s[2 * n + k][2 * i2 + 1] - off[i2]);
+          l[i2] += x + y;
+          if constexpr (KIND == BPT_KV_INT8) {
+            const __half* vs = reinterpret_cast<const __half*>(scales_of(st, n)) + 16 + 8 * k + 2 * t;
+            x *= __half2float(vs[0]);
+            y *= __half2float(vs[1]);
+          }
+          p[2 * k + i2] = pack2<KIND>(x, y);
+        }
+      values16<KIND, D>(stage(st) + (kKeys + n * 16) * RB, lane, p, o);
+    }
+  }
+  cp_async_wait<0>();
+  float inv[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    inv[i] = l[i] == 0.f ? 0.f : a.src.v_scale / l[i];
+  }
+  if (parts <= 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (row[i].out < 0) continue;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        const float x = o[n][2 * i] * inv[i], y = o[n][2 * i + 1] * inv[i];
+        const int64_t dst = row[i].out + v_dim<KIND, D>(n, t, 0);
+        if constexpr (kIs16<KIND>) {
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + dst) = pack2<KIND>(x, y);
+        } else {
+          store_16(a.out, a.q_dtype, dst, x);
+          store_16(a.out, a.q_dtype, row[i].out + v_dim<KIND, D>(n, t, 1), y);
+        }
+      }
+    }
+    return;
+  }
+  // a part: [rows][D] and the rows' log2-sum-exp2 of tile (blockIdx.x, hk), part sp
+  const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
+  float* part = a.part_out + (tile * a.n_splits + sp) * (kRows * D);
+  float* part_lse = a.part_lse + (tile * a.n_splits + sp) * kRows;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = warp * 16 + g + 8 * i;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      part[r * D + v_dim<KIND, D>(n, t, 0)] = o[n][2 * i] * inv[i];
+      part[r * D + v_dim<KIND, D>(n, t, 1)] = o[n][2 * i + 1] * inv[i];
+    }
+    if (t == 0) part_lse[r] = l[i] == 0.f ? -INFINITY : (m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i]);
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) s_last = atomicAdd(&a.tickets[tile], 1u) == unsigned(parts - 1);
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  join_parts<D>(a, at, hk, tile, parts, kRows, warp, kWarps, lane);
+  if (tid == 0) a.tickets[tile] = 0u;
+}
+
+template <int KIND, int D>
+int launch_prefill(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
+  using S = PrefillShape<KIND, D>;
+  const int st = set_max_smem(reinterpret_cast<const void*>(paged_prefill_kernel<KIND, D>), S::kSmem);
+  if (st) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<KIND, D>, a);
+  if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
+  return BPT_OK;
+}
+
+template <int KIND>
+int prefill_dim(const PrefillArgs& a, int64_t D, int64_t tiles, int flags, cudaStream_t stream) {
+  if (D == 64) return launch_prefill<KIND, 64>(a, tiles, flags, stream);
+  if (D == 128) return launch_prefill<KIND, 128>(a, tiles, flags, stream);
+  return launch_prefill<KIND, 256>(a, tiles, flags, stream);
+}
+
+// How a call is cut: rows per tile, the most tiles that the rows can make, keys per part and parts.
+struct Plan {
+  int rows;
+  int64_t tiles;
+  int64_t split, n_splits;
+};
+
+Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t tokens) {
+  Plan p;
+  p.rows = kRows;
+  p.tiles = T * (Hq / Hkv) / p.rows + B;
+  // Fewer CTAs than two per SM: each tile's keys in parts of at least 512 until there are.
+  const int64_t ctas = p.tiles * Hkv, want = 2 * int64_t(num_sms());
+  p.n_splits = ctas >= want ? 1 : std::min((want + ctas - 1) / ctas, (tokens + 511) / 512);
+  p.n_splits = std::max<int64_t>(p.n_splits, 1);
+  p.split = ((tokens + p.n_splits - 1) / p.n_splits + kKeys - 1) / kKeys * kKeys;
+  p.split = std::max<int64_t>(p.split, kKeys);
+  return p;
+}
+
+constexpr int64_t kTickets = 65536;  // of a workspace that other merging kernels use too
+constexpr int64_t kTicketBytes = kTickets * 4;
+
+int64_t lse_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * p.n_splits * p.rows * 4 + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace bpt
+
+using namespace bpt;
+
+extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
+  if (T < 1 || B < 1 || Hkv < 1 || Hq < Hkv || tokens < 1) return 0;
+  const Plan p = plan_prefill(T, B, Hq, Hkv, tokens);
+  return p.n_splits > 1 ? kTicketBytes + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
+}
+
+extern "C" int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
+                                 const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
+                                 const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
+                                 const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions,
+                                 const int32_t* key_starts, const int32_t* prefix_lens, const float* alibi_slopes,
+                                 float softcap, int64_t window, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                 int64_t block_size, int64_t num_blocks, int64_t tokens, float sm_scale, void* out,
+                                 void* workspace, int64_t workspace_bytes, int flags, void* stream) {
+  const char* who = "paged prefill";
+  BPT_REQUIRE(T >= 0 && T < (1ll << 30) && B >= 0 && B < (1 << 20), BPT_ERR_INVALID, "%s: T=%lld B=%lld", who, (long long)T,
+              (long long)B);
+  if (T == 0 || B == 0) return BPT_OK;
+  BPT_REQUIRE(q && cu_seqlens && lengths && out, BPT_ERR_INVALID, "%s: null pointer argument", who);
+  PrefillArgs a;
+  const int bad = paged_source(a.src, who, k_pool, v_pool, kind, k_scale, v_scale, k_scales, v_scales, block_table, bt_stride,
+                               bt_width, Hkv, D, block_size, num_blocks);
+  if (bad) return bad;
+  BPT_REQUIRE(q_dtype == BPT_DTYPE_F16 || q_dtype == BPT_DTYPE_BF16, BPT_ERR_INVALID, "%s: q dtype %d (f16 or bf16)", who,
+              q_dtype);
+  BPT_REQUIRE((kind != BPT_KV_F16 || q_dtype == BPT_DTYPE_F16) && (kind != BPT_KV_BF16 || q_dtype == BPT_DTYPE_BF16),
+              BPT_ERR_UNSUPPORTED, "%s: 16-bit pages take queries of their own type", who);
+  BPT_REQUIRE(Hq >= 1 && Hq % Hkv == 0 && Hq < (1 << 15), BPT_ERR_INVALID, "%s: Hq=%lld is not a multiple of Hkv=%lld", who,
+              (long long)Hq, (long long)Hkv);
+  BPT_REQUIRE(T * (Hq / Hkv) < (1ll << 31) - 1024, BPT_ERR_INVALID, "%s: too many rows", who);
+  BPT_REQUIRE(tokens >= 1 && tokens < (1ll << 30), BPT_ERR_INVALID, "%s: tokens=%lld", who, (long long)tokens);
+  BPT_REQUIRE(window >= 0, BPT_ERR_INVALID, "%s: window=%lld", who, (long long)window);
+  BPT_REQUIRE(softcap >= 0.f && softcap < INFINITY, BPT_ERR_INVALID, "%s: softcap must be finite and not negative", who);
+  BPT_REQUIRE(q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && aligned16(q) && aligned16(out), BPT_ERR_ALIGNMENT,
+              "%s: rows must start on 16 bytes", who);
+  a.q = q;
+  a.q_dtype = q_dtype;
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.cu = cu_seqlens;
+  a.lengths = lengths;
+  a.positions = positions;
+  a.key_starts = key_starts;
+  a.prefix_lens = prefix_lens;
+  a.slopes = alibi_slopes;
+  a.softcap = softcap;
+  a.sm_scale = sm_scale;
+  a.window = window < (1 << 30) ? int(window) : 0;
+  a.T = int(T);
+  a.B = int(B);
+  a.Hq = int(Hq);
+  a.D = int(D);
+  a.rep = int(Hq / Hkv);
+  a.out = out;
+  const Plan p = plan_prefill(T, B, Hq, Hkv, tokens);
+  a.split = int(p.split);
+  a.n_splits = int(p.n_splits);
+  BPT_REQUIRE(p.tiles < (1ll << 31) && Hkv < 65536 && p.n_splits < 65536, BPT_ERR_INVALID, "%s: too many rows", who);
+  a.tickets = nullptr;
+  a.part_lse = nullptr;
+  a.part_out = nullptr;
+  if (p.n_splits > 1) {
+    const int64_t need = bpt_paged_prefill_workspace_bytes(T, B, Hq, Hkv, D, tokens);
+    BPT_REQUIRE(workspace, BPT_ERR_WORKSPACE, "%s: no workspace", who);
+    BPT_REQUIRE(aligned16(workspace), BPT_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", who);
+    BPT_REQUIRE(workspace_bytes >= need, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
+                (long long)workspace_bytes, (long long)need);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.tickets = reinterpret_cast<unsigned int*>(ws);
+    a.part_lse = reinterpret_cast<float*>(ws + kTicketBytes);
+    a.part_out = reinterpret_cast<float*>(ws + kTicketBytes + lse_bytes(p, Hkv));
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (kind) {
+    case BPT_KV_FP8: return prefill_dim<BPT_KV_FP8>(a, D, p.tiles, flags, s);
+    case BPT_KV_INT8: return prefill_dim<BPT_KV_INT8>(a, D, p.tiles, flags, s);
+    case BPT_KV_F16: return prefill_dim<BPT_KV_F16>(a, D, p.tiles, flags, s);
+    default: return prefill_dim<BPT_KV_BF16>(a, D, p.tiles, flags, s);
+  }
+}

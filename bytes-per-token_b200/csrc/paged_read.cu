@@ -70,7 +70,7 @@ struct ReadShape {
 template <int KIND, int D>
 __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) {
   using S = ReadShape<KIND, D>;
-  constexpr int RB = S::RB, NST = S::kStages, CPR = RB / 16;
+  constexpr int RB = S::RB, NST = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
     const int key0 = first + 16 * (warp + kWarps * i);
     const uint32_t tile_u = ring_u + st * S::kStage;
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    scores16<KIND, D>(tile_u, lane, [&](int j) -> const uint32_t(&)[4] { return qf[j]; }, s0, s1);
+    scores16<KIND, D>(tile_u, lane, [&](int j) { return MmaRows{{qf[j][0], qf[j][1], qf[j][2], qf[j][3]}}; }, s0, s1);
     float s[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};  // keys 2t, 2t + 1, 2t + 8, 2t + 9
     float vs[4] = {1.f, 1.f, 1.f, 1.f};
     if constexpr (KIND == BPT_KV_INT8) {
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
     for (int e = 0; e < 4; ++e) {
       const int key = key0 + 2 * t + (e & 1) + (e >> 1) * 8;
       s[e] *= mul;
-      if (cap) s[e] = cap_out - __fdividef(2.f * cap_out, exp2_approx(s[e]) + 1.f);
+      if (cap) s[e] = capped(s[e], cap_out);
       s[e] = fmaf(slope, float(key - pos), s[e]);
       if (key < from || key >= to) s[e] = -INFINITY;
     }

@@ -49,6 +49,10 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return c ^ ((((r >> 1) & 3) << 1) ^ ((r & 1) << 2));
 }
 
+struct MmaRows {  // an A fragment: 16 rows of a k-step
+  uint32_t v[4];
+};
+
 template <int KIND>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (KIND == BPT_KV_BF16) {
@@ -139,8 +143,9 @@ __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, fl
     for (int j = 0; j < D / 16; ++j) {
       uint32_t b[4];
       ldmatrix4(b, base + swizzled<KIND, D>(row, 2 * j + c) * 16);
-      mma_16816<KIND>(s0, q(j), b[0], b[1]);
-      mma_16816<KIND>(s1, q(j), b[2], b[3]);
+      const MmaRows qj = q(j);
+      mma_16816<KIND>(s0, qj.v, b[0], b[1]);
+      mma_16816<KIND>(s1, qj.v, b[2], b[3]);
     }
   } else {
     const int g = lane >> 2, t = lane & 3;
@@ -151,8 +156,9 @@ __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, fl
       const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mma_16816<KIND>(s0, q(4 * j4 + i), codes_to_f16<KIND>(xs[i] & 0xFFFFu), codes_to_f16<KIND>(xs[i] >> 16));
-        mma_16816<KIND>(s1, q(4 * j4 + i), codes_to_f16<KIND>(ys[i] & 0xFFFFu), codes_to_f16<KIND>(ys[i] >> 16));
+        const MmaRows qj = q(4 * j4 + i);
+        mma_16816<KIND>(s0, qj.v, codes_to_f16<KIND>(xs[i] & 0xFFFFu), codes_to_f16<KIND>(xs[i] >> 16));
+        mma_16816<KIND>(s1, qj.v, codes_to_f16<KIND>(ys[i] & 0xFFFFu), codes_to_f16<KIND>(ys[i] >> 16));
       }
     }
   }
@@ -293,11 +299,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// A raw product as a score in base 2: cap tanh(x / cap) (cap > 0) or x, times log2 e. tanh y = 1 - 2 / (e^2y + 1): its
-// absolute error is a few 2^-24, so the score's is a few 2^-24 of the cap. `cap_in` = 2 log2 e / cap, `cap_out` = cap log2 e.
-__device__ __forceinline__ float capped(float x, float cap_in, float cap_out) {
-  const float e = exp2_approx(x * cap_in);
-  return cap_out - __fdividef(2.f * cap_out, e + 1.f);
+// cap tanh(x / cap) as a base-2 score, from y = 2 log2(e) x / cap; `cap_out` = cap log2 e. tanh = 1 - 2 / (2^y + 1): its
+// absolute error is a few 2^-24, so the score's is a few 2^-24 of the cap.
+__device__ __forceinline__ float capped(float y, float cap_out) {
+  return cap_out - __fdividef(2.f * cap_out, exp2_approx(y) + 1.f);
 }
 
 // The power of two that brings |x| <= amax to at most 1, as (factor, its inverse): keeps any q inside f16's range.

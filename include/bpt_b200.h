@@ -44,7 +44,7 @@ extern "C" {
 #define BPT_KV_FP8 1  /* E4M3 bytes, one fp32 scale per tensor (K and V each)            */
 #define BPT_KV_INT8 2 /* symmetric int8 codes, one fp16 scale per (token, KV head)      */
 #define BPT_KV_F16 3  /* fp16 values (bpt_rope_kv_append, bpt_paged_read, bpt_paged_prefill) */
-#define BPT_KV_BF16 4 /* bf16 values (the same)                                         */
+#define BPT_KV_BF16 4 /* bf16 values (the same)                                             */
 
 /* launch flags */
 #define BPT_FLAG_PDL 1 /* launch with programmatic dependent launch (prologue overlaps the previous kernel) */
@@ -176,6 +176,29 @@ int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_str
                    int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size, int64_t num_blocks, int64_t split,
                    int64_t n_splits, float sm_scale, void* out, int out_dtype, float* out_partial, float* lse_partial,
                    void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
+/* Prefill attention over a paged cache of any format: q [T, Hq, D] (f16 or bf16; the pages' own type where they are 16-bit)
+ * holds the new tokens of B sequences, sequence b's in rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]; rows of
+ * none are not touched in out). Their keys and values are in the cache already, lengths[b] (int32 [B]) counting them. A
+ * token sits at position p = positions[row] (int32 [T]), or, with positions NULL, the sequence's new tokens are its last
+ * ones; it sees the keys j with max(0, key_starts[row], p - window + 1) <= j < min(lengths[b], max(p + 1, prefix_lens[b])):
+ *   s_j = softcap tanh(sm_scale q.k_j / softcap) - alibi_slopes[head] |p - j|
+ * key_starts (int32 [T]: documents packed in one sequence), prefix_lens (int32 [B]: a prefix that all of its tokens see
+ * whole) and alibi_slopes (fp32 [Hq]) may be NULL; softcap 0: no cap; window 0: no window. No visible key gives 0. out
+ * [T, Hq, D] contiguous, in q's type. `tokens` bounds the longest length (it sizes the launch, not the result).
+ * A value that is NaN or infinite spreads to every query whose tile reads its key, visible to it or not.
+ * `workspace`: bpt_paged_prefill_workspace_bytes(...) bytes (0: none needed), as for bpt_paged_read.
+ * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024; rows of q start on 16 bytes.
+ * Replaces: the prefill read of PagedKVCache + Attention.forward (engine/kv_cache.py:158-169, engine/attention.py:12-31). */
+int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens);
+int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
+                      const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
+                      const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
+                      const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions,
+                      const int32_t* key_starts, const int32_t* prefix_lens, const float* alibi_slopes, float softcap,
+                      int64_t window, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size,
+                      int64_t num_blocks, int64_t tokens, float sm_scale, void* out, void* workspace,
+                      int64_t workspace_bytes, int flags, void* stream);
 
 /* bpt_paged_attend without a workspace argument, for callers that cannot allocate device memory: serving
  * engines that hand all free HBM to their paged KV pool at start-up (so a later cudaMalloc fails or fragments
