@@ -50,7 +50,7 @@ SIGNATURES: dict[str, list] = {
     "bpt_paged_read_workspace_bytes": [I64, I64, I64, I64],
     "bpt_paged_read": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, I64, P, P, P, F32, I64, I64, I64, I64, I64,
                        I64, I64, I64, I64, F32, P, I32, P, P, P, I64, I32, P],
-    "bpt_paged_prefill_workspace_bytes": [I64, I64, I64, I64, I64, I64],
+    "bpt_paged_prefill_workspace_bytes": [I64, I64, I64, I64, I64, I32, I64],
     "bpt_paged_prefill": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, I64, P, P, P, P, P, P, F32, I64, I64, I64, I64,
                           I64, I64, I64, I64, I64, F32, P, P, I64, I32, P],
     "bpt_merge_partials": [P, P, I64, I64, I64, I64, P, I32, P],

@@ -62,7 +62,7 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
         if out is None:
             out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
         if workspace is None:
-            need = int(lib().bpt_paged_prefill_workspace_bytes(t, b, hq, hkv, d, tokens))
+            need = int(lib().bpt_paged_prefill_workspace_bytes(t, b, hq, hkv, d, code, tokens))
             workspace = _zeroed_workspace(need, device) if need else None
         st = lib().bpt_paged_prefill(
             ptr(q), dtype_code(q.dtype), q.stride(0), q.stride(1), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs, ptr(kss),

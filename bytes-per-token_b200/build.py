@@ -23,6 +23,9 @@ INCLUDE = HERE.parent / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "bpt_b200" / "libbpt_b200.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+# Files that take no device code from others: setmaxnreg, which moves registers between a CTA's warps, is dropped by the
+# assembler from relocatable code.
+WHOLE_PROGRAM = {"paged_prefill_tc"}
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
 
@@ -49,7 +52,8 @@ def _compile(src: Path, headers: list[Path], verbose: bool) -> Path:
     obj = BUILD / (src.stem + ".o")
     if not _stale(obj, [src, *headers]):
         return obj
-    cmd = [nvcc(), *ARCH, *FLAGS, f"-I{INCLUDE}", "-c", str(src), "-o", str(obj)]
+    flags = [f for f in FLAGS if f != "-rdc=true" or src.stem not in WHOLE_PROGRAM]
+    cmd = [nvcc(), *ARCH, *flags, f"-I{INCLUDE}", "-c", str(src), "-o", str(obj)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     proc = subprocess.run(cmd, capture_output=True, text=True)

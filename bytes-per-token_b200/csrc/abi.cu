@@ -63,6 +63,8 @@ int set_max_smem(const void* kernel, int bytes) {
   return BPT_OK;
 }
 
+int take_prefill_tc_error();  // the same read-and-clear of csrc/paged_prefill_tc.cu's own flag
+
 }  // namespace bpt
 
 extern "C" int bpt_abi_version(void) { return BPT_ABI_VERSION; }
@@ -71,9 +73,10 @@ extern "C" const char* bpt_last_error(void) { return bpt::t_message; }
 
 extern "C" int bpt_device_error(void) {
   if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+  const int prefill = bpt::take_prefill_tc_error();
   int value = 0;
   const int zero = 0;
   if (cudaMemcpyFromSymbol(&value, bpt::g_device_error, sizeof(int)) != cudaSuccess) return -1;
   if (value != 0) cudaMemcpyToSymbol(bpt::g_device_error, &zero, sizeof(int));
-  return value;
+  return value != 0 ? value : prefill;
 }

@@ -39,7 +39,13 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Kernels never trap. A bounded wait that runs out, or an index that fails its bounds check, records a code here
 // and the kernel skips the work it cannot do; the host reads it with bpt_device_error().
 
+// A file compiled as a whole program (BPT_WHOLE_PROGRAM: setmaxnreg takes effect only there) has a flag of its own, which
+// bpt_device_error() reads too.
+#ifdef BPT_WHOLE_PROGRAM
+static __device__ int g_device_error = 0;
+#else
 extern __device__ int g_device_error;
+#endif
 
 enum DeviceError : int {
   kDevErrNone = 0,

@@ -8,7 +8,8 @@
 // rows (row = token * rep + head), so every key and value brought in serves all of them; a row carries its own interval
 // [lo, hi), and a tile of rows visits only the keys between its smallest lo and largest hi.
 //
-// This kernel multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. A CTA that
+// 16-bit pages with heads of 64 or 128 take csrc/paged_prefill_tc.cu. The kernel here serves the other formats and heads of
+// 256. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. A CTA that
 // has few companions takes a part of its keys only; the parts of a tile are joined by the last of its CTAs to finish.
 #include "paged_prefill.cuh"
 
@@ -306,23 +307,24 @@ int prefill_dim(const PrefillArgs& a, int64_t D, int64_t tiles, int flags, cudaS
   return launch_prefill<KIND, 256>(a, tiles, flags, stream);
 }
 
-// How a call is cut: rows per tile, the most tiles that the rows can make, keys per part and parts.
+// How a call is cut: which kernel, rows per tile, the most tiles that the rows can make, keys per part and parts.
 struct Plan {
+  bool tc;
   int rows;
   int64_t tiles;
   int64_t split, n_splits;
 };
 
-Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t tokens) {
+Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int kind, int64_t tokens) {
   Plan p;
-  p.rows = kRows;
+  p.tc = (kind == BPT_KV_F16 || kind == BPT_KV_BF16) && D <= 128;
+  p.rows = p.tc ? kPrefillTcRows : kRows;
   p.tiles = T * (Hq / Hkv) / p.rows + B;
-  // Fewer CTAs than two per SM: each tile's keys in parts of at least 512 until there are.
-  const int64_t ctas = p.tiles * Hkv, want = 2 * int64_t(num_sms());
-  p.n_splits = ctas >= want ? 1 : std::min((want + ctas - 1) / ctas, (tokens + 511) / 512);
-  p.n_splits = std::max<int64_t>(p.n_splits, 1);
-  p.split = ((tokens + p.n_splits - 1) / p.n_splits + kKeys - 1) / kKeys * kKeys;
-  p.split = std::max<int64_t>(p.split, kKeys);
+  // Fewer CTAs than fill the GPU (one per SM on the tensor-core kernel, two of the other): each tile's keys in parts
+  // of at least 256 until there are.
+  const int64_t ctas = p.tiles * Hkv, want = (p.tc ? 1 : 2) * int64_t(num_sms());
+  p.n_splits = std::max<int64_t>(std::min(want / ctas, (tokens + 255) / 256), 1);
+  p.split = ((tokens + p.n_splits - 1) / p.n_splits + 127) / 128 * 128;
   return p;
 }
 
@@ -336,9 +338,10 @@ int64_t lse_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * p.n_spli
 
 using namespace bpt;
 
-extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
+extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int kind,
+                                                     int64_t tokens) {
   if (T < 1 || B < 1 || Hkv < 1 || Hq < Hkv || tokens < 1) return 0;
-  const Plan p = plan_prefill(T, B, Hq, Hkv, tokens);
+  const Plan p = plan_prefill(T, B, Hq, Hkv, D, kind, tokens);
   return p.n_splits > 1 ? kTicketBytes + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
 }
 
@@ -390,7 +393,7 @@ extern "C" int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t,
   a.D = int(D);
   a.rep = int(Hq / Hkv);
   a.out = out;
-  const Plan p = plan_prefill(T, B, Hq, Hkv, tokens);
+  const Plan p = plan_prefill(T, B, Hq, Hkv, D, kind, tokens);
   a.split = int(p.split);
   a.n_splits = int(p.n_splits);
   BPT_REQUIRE(p.tiles < (1ll << 31) && Hkv < 65536 && p.n_splits < 65536, BPT_ERR_INVALID, "%s: too many rows", who);
@@ -398,7 +401,7 @@ extern "C" int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t,
   a.part_lse = nullptr;
   a.part_out = nullptr;
   if (p.n_splits > 1) {
-    const int64_t need = bpt_paged_prefill_workspace_bytes(T, B, Hq, Hkv, D, tokens);
+    const int64_t need = bpt_paged_prefill_workspace_bytes(T, B, Hq, Hkv, D, kind, tokens);
     BPT_REQUIRE(workspace, BPT_ERR_WORKSPACE, "%s: no workspace", who);
     BPT_REQUIRE(aligned16(workspace), BPT_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", who);
     BPT_REQUIRE(workspace_bytes >= need, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
@@ -409,6 +412,7 @@ extern "C" int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t,
     a.part_out = reinterpret_cast<float*>(ws + kTicketBytes + lse_bytes(p, Hkv));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.tc) return prefill_tc(a, kind, p.tiles, flags, s);
   switch (kind) {
     case BPT_KV_FP8: return prefill_dim<BPT_KV_FP8>(a, D, p.tiles, flags, s);
     case BPT_KV_INT8: return prefill_dim<BPT_KV_INT8>(a, D, p.tiles, flags, s);

@@ -29,6 +29,9 @@ struct PrefillArgs {
   float* part_lse;  // [tiles, Hkv, n_splits, rows], base 2
 };
 
+constexpr int kPrefillTcRows = 256;  // packed rows per CTA of the tensor-core kernel
+int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream);
+
 // A tile of packed rows (token * rep + head) of one sequence.
 struct TileAt {
   int b;        // the sequence, -1 where the grid has more tiles than there are

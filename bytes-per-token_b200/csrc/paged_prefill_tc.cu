@@ -1,0 +1,622 @@
+// Prefill attention on the 5th-generation tensor cores (tcgen05, sm_100a only), for head dims 64 and 128: the same
+// operation, rows, intervals and parts as csrc/paged_prefill.cu.
+//
+// A CTA takes 256 packed rows (token * rep + head) of one KV head as two tiles of 128 and walks their keys 128 at a time:
+//   S = Q K^T    both operands in shared memory (128-byte swizzle), fp32 S in tensor memory;
+//   P = 2^(s - m) rounded to the pages' 16-bit type over S's own columns in tensor memory;
+//   O += P V     P from tensor memory, V as it lies in its pages ([key][dim], the transposed operand form), fp32 O in tensor
+//                memory.
+// Four warpgroups: two do the softmax, each of one tile, a thread per row (so neither maximum nor sum crosses threads); one
+// brings pages into a ring of shared-memory stages, K and V of a step in stages of their own, by cp.async (rows of any page
+// size; keys that are not visible become zeros); of the last, one thread issues the matrix products. While the softmax of
+// one tile runs, the tensor cores work on the other tile: P V of its last step, then Q K^T of its next.
+//
+// The running maximum only moves when a row's true maximum has passed it by 2^8 or more: P then stays below 2^8 (exact in
+// range for both types, and P V is divided by the sum of the same P), and O in tensor memory is rescaled a few times per
+// row instead of every step.
+//
+// Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
+// and the CTA still awaits its copies and products, frees its tensor memory and returns.
+#define BPT_WHOLE_PROGRAM  // compiled without relocatable device code
+#include "paged_prefill.cuh"
+
+namespace bpt {
+namespace {
+
+constexpr int kThreads = 512;     // warpgroups: softmax of tile 0, softmax of tile 1, producer, matrix products
+constexpr int kTileRows = 128;
+constexpr int kRows = 2 * kTileRows;
+static_assert(kRows == kPrefillTcRows, "the tiles that the caller counts");
+constexpr int kKeys = 128;        // per step
+constexpr int kSoftmaxRegs = 200;  // 2 x 128 x 200 + 2 x 128 x 56 = 512 x 128: the split of the registers at launch
+constexpr int kOtherRegs = 56;
+constexpr int kLaunchRegs = 128;
+static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
+constexpr int kFlagSteps = 16;     // steps whose bad-block flags are kept (the ring runs at most 5 steps ahead)
+constexpr float kSlack = 8.f;      // how far, in powers of two, a row's maximum may pass the one in use
+
+template <int D>
+struct TcShape {
+  static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kQ = 2 * kTileBytes;
+  static constexpr int kBars = 2 * kStages + 10;  // an even number: the flags behind them start on 16 bytes
+  static constexpr int kSmem = 1024 + kQ + kStages * kTileBytes + kBars * 8 + kFlagSteps * 16 + 64;
+  static constexpr uint32_t kO = 256;     // columns: S0, S1 at 0, 128; O0, O1 at 256, 256 + D
+  static_assert(256 + 2 * D <= 512, "tensor memory");
+};
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_request32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The registers of a request, once tmem_wait_load has returned: nothing reads them before this.
+__device__ __forceinline__ void tmem_arrived32(uint32_t* v) {
+  asm volatile(""
+      : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+        "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+        "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+        "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+      :
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// Shared-memory descriptors of 128-byte-swizzled tiles whose rows are 128 bytes, in atoms of 8 rows (1024 bytes). With the
+// contraction along the row (Q, K): the next 8 rows 1024 bytes on. With the contraction across rows (V): the next 8 keys
+// 1024 bytes on, the next 64 dims `half` bytes on.
+__device__ __forceinline__ uint64_t desc_along(uint32_t addr) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint64_t desc_across(uint32_t addr, uint32_t half) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(half >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// Instruction descriptor, kind::f16: D f32 (bits 4-5 = 1), A and B f16 or bf16 (bits 7-9, 10-12 = 0 or 1), B's rows across
+// the contraction (bit 16), N >> 3 at bits 17-22, M >> 4 at bits 24-28.
+template <int KIND>
+constexpr uint32_t tc_idesc(int m, int n, bool across) {
+  return (1u << 4) | (KIND == BPT_KV_BF16 ? (1u << 7) | (1u << 10) : 0u) | (across ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(m >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  const uint32_t mask = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(mask), "r"(mask), "r"(mask), "r"(mask)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  const uint32_t mask = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(mask), "r"(mask), "r"(mask), "r"(mask)
+      : "memory");
+}
+
+// Item n of the ring (K of step n / 2 where n is even, V where odd): its stage and the parity of the lap it fills.
+template <int STAGES>
+struct Item {
+  int stage = 0;
+  uint32_t lap = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) {
+      stage = 0;
+      lap ^= 1u;
+    }
+  }
+};
+
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// What a softmax warpgroup does for tile i: its queries into shared memory, then every step's maximum, probabilities and
+// sum, and at the end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
+template <int KIND, int D>
+__device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt& at, const RowAt& row, int hk, int sp, int parts,
+                                             int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
+                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags,
+                                             uint32_t* last_cta) {
+  using S = TcShape<D>;
+  const int r = threadIdx.x & 127, warp = r >> 5, lane = threadIdx.x & 31;
+  {
+    uint8_t* tile = smem + i * S::kTileBytes + r * 128;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + max(row.q, int64_t(0)));
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 x = row.q >= 0 ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (r & 7)) << 4)) = x;
+    }
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_full[i]);
+  }
+  const bool cap = a.softcap > 0.f;
+  const float raw = a.sm_scale * a.src.k_scale;  // a product as a score
+  const float mul = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
+  const float cap_out = a.softcap * kLog2e;
+  const bool sloped = a.slopes != nullptr;
+  const bool shaped = cap || sloped || !(mul > 0.f);  // a score is not just a positive multiple of its product
+  const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
+  const uint32_t lanes = uint32_t(32 * warp) << 16;
+  const uint32_t s_at = tmem + lanes + i * 128, o_at = tmem + lanes + S::kO + i * D;
+
+  float m = -INFINITY;  // the maximum in use
+  float2 l2 = make_float2(0.f, 0.f);
+  uint32_t n = 0;
+  bool ok = true;
+  for (int j = first; j < last; ++j, ++n) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], n & 1u));
+    if (!ok) break;
+    tc_fence_after();
+    uint32_t v[kKeys];
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 32) tmem_request32(s_at + c, v + c);
+    tmem_wait_load();
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 32) tmem_arrived32(v + c);
+    const int key0 = from + j * kKeys;
+    const uint4 bad = *reinterpret_cast<const uint4*>(flags + (j & (kFlagSteps - 1)) * 4);
+    const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
+    const bool masked = any_bad || key0 < all_lo || key0 + kKeys > all_hi;
+    float mul_now = mul;
+    if (shaped) {
+      mul_now = 1.f;
+      if (cap) {
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(capped(__uint_as_float(v[c]) * mul, cap_out));
+      } else {
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * mul);
+      }
+      if (sloped) {
+        const float far = float(key0 - row.pos);
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(fmaf(row.slope, fabsf(far + float(c)), __uint_as_float(v[c])));
+      }
+    }
+    if (masked) {
+      const int below = row.lo - key0, above = row.hi - key0;
+#pragma unroll
+      for (int c = 0; c < kKeys; ++c)
+        if (c < below || c >= above) v[c] = 0xFF800000u;
+      if (any_bad) {
+        const uint32_t w[4] = {bad.x, bad.y, bad.z, bad.w};
+#pragma unroll
+        for (int c = 0; c < kKeys; ++c)
+          if (w[c >> 5] >> ((c >> 3) & 3) & 1u) v[c] = 0xFF800000u;
+      }
+    }
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 8)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        top[e] = fmaxf(top[e], fmaxf(__uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e])));
+    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul_now;
+    const bool moves = now > m + kSlack;
+    if (__any_sync(0xffffffffu, moves)) {
+      float shrink = 1.f;
+      if (moves) {
+        shrink = exp2_approx(m - now);
+        m = now;
+        l2.x *= shrink;
+        l2.y *= shrink;
+      }
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (n - 1) & 1u));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o_at + c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+          tmem_store32(o_at + c, o);
+        }
+      }
+    }
+    // P enters its product rounded to 16 bits (as any operand of these matrix instructions); the sum that divides it is
+    // taken in fp32, before the rounding.
+    const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 32) {
+      uint32_t p[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float2 x = ffma2(make_float2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])),
+                               make_float2(mul_now, mul_now), make_float2(-off, -off));
+        const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+        l2 = fadd2(l2, y);
+        p[e] = pack2<KIND>(y.x, y.y);
+      }
+      tmem_store16(s_at + (c >> 1), p);
+    }
+    tmem_wait_store();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&p_full[i]);
+  }
+  if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (n - 1) & 1u));
+  tc_fence_after();
+  const float l = l2.x + l2.y;
+  const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
+  const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
+  float* part = parts > 1 ? a.part_out + ((tile * a.n_splits + sp) * kRows + i * kTileRows + r) * D : nullptr;
+#pragma unroll 1
+  for (int c = 0; ok && c < D; c += 32) {
+    uint32_t o[32];
+    if (n > 0) {
+      tmem_load32(o_at + c, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0u;
+    }
+    if (parts > 1) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4)
+        *reinterpret_cast<float4*>(part + c + e) =
+            make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv,
+                        __uint_as_float(o[e + 3]) * inv);
+    } else if (row.out >= 0) {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row.out + c);
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = pack2<KIND>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+        dst[e >> 3] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  if (parts <= 1) return;
+  if (ok) a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+  __threadfence();
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (threadIdx.x == 0) *last_cta = atomicAdd(&a.tickets[tile], 1u) == unsigned(parts - 1);
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (!*last_cta) return;
+  __threadfence();
+  join_parts<D>(a, at, hk, tile, parts, kRows, i * 4 + warp, 8, lane);
+  if (threadIdx.x == 0) a.tickets[tile] = 0u;
+}
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillArgs a) {
+  using S = TcShape<D>;
+  constexpr int NS = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* ring = smem + S::kQ;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * S::kTileBytes);
+  uint64_t* full = bars;             // [NS] a stage's rows have landed (one arrival per producer warp)
+  uint64_t* empty = full + NS;       // [NS] the products that read it are done
+  uint64_t* q_full = empty + NS;     // [2] a tile's queries are in shared memory
+  uint64_t* s_full = q_full + 2;     // [2] S is in tensor memory
+  uint64_t* p_full = s_full + 2;     // [2] P is in tensor memory, O rescaled where needed
+  uint64_t* o_done = p_full + 2;     // [2] P V is in O
+  uint64_t* drained = o_done + 2;    // all products are done
+  uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
+  int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
+  uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address; then: is this CTA the last
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+  const int hk = blockIdx.y, sp = blockIdx.z;
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 2);  // the products' completion, and the issuing thread (whose own waits saw the flags)
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+      range[i] = INT_MAX;
+      range[2 + i] = 0;
+    }
+    mbar_init(drained, 1);
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const TileAt at = find_tile(a, kRows, int(blockIdx.x));
+  if (at.b < 0) return;
+  const int b = at.b;
+  const int len = sequence_length(a, b, tid == 0 && hk == 0 && sp == 0);
+  __syncthreads();
+
+  // the tiles' rows: thread r of a softmax warpgroup holds row r
+  RowAt row{-1, -1, 0, 0, 0, 0.f};
+  if (wg < 2) {
+    row = row_at(a, at, at.row0 + wg * kTileRows + (tid & 127), hk, len);
+    const bool any = row.hi > row.lo;
+    const int lo = __reduce_min_sync(0xffffffffu, any ? row.lo : INT_MAX);
+    const int hi = __reduce_max_sync(0xffffffffu, any ? row.hi : 0);
+    if (lane == 0 && hi > 0) {
+      atomicMin(&range[wg], lo);
+      atomicMax(&range[2 + wg], hi);
+    }
+  }
+  __syncthreads();
+  const int lo = min(range[0], range[1]), hi = max(range[2], range[3]);
+  const int base = lo == INT_MAX ? 0 : lo & ~15;
+  const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
+  if (sp >= max(parts, 1)) return;
+  const int from = base + sp * a.split;
+  const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
+  const int steps = (to - from + kKeys - 1) / kKeys;
+  // the steps that tile i has keys in: first[i] <= j < last[i]
+  int first[2], last[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int l = max(range[i], from), h = min(range[2 + i], to);
+    first[i] = h > l ? (l - from) / kKeys : 0;
+    last[i] = h > l ? (h - from + kKeys - 1) / kKeys : 0;
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  if (wg == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    // ---- producer: warp w brings rows 32 w .. 32 w + 31 of every stage, two groups of 16 keys
+    const int w = warp & 3;
+    const int32_t* table = a.src.block_table + int64_t(b) * a.src.bt_stride;
+    const int64_t row_bytes = int64_t(a.src.Hkv) * (2 * D), head_bytes = int64_t(hk) * (2 * D);
+    const bool two = a.src.bs_log2 == 3;
+    const int take_from = max(from, lo);
+    int held = -1, held2 = -1;  // lane n: the block(s) of group n of the current 16 steps
+    auto block_at = [&](int key) -> int {
+      if (key >= to) return -1;
+      const int blk = table[key >> a.src.bs_log2];
+      if (blk < 0 || blk >= a.src.num_blocks) {
+        record_error(kDevErrBlockIndex);
+        return -1;
+      }
+      return blk;
+    };
+    constexpr int CPR = D / 8;  // 16-byte chunks of a row
+    constexpr int kLag = 2;     // items in flight before the oldest is announced
+    Item<NS> in, out;
+    bool ok = true;
+    int announced = 0;
+    auto announce = [&]() {  // the oldest item's copies of this warp have landed: make them the tensor cores' to read
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[out.stage]);
+      out.next();
+      ++announced;
+    };
+    for (int n = 0; n < 2 * steps && ok; ++n) {
+      const int j = n >> 1;
+      if (n >= NS) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+        if (!ok) break;
+      }
+      if ((n & 1) == 0) {
+        if ((j & 15) == 0) {
+          const int key = from + kKeys * (j + (lane >> 1)) + 32 * w + 16 * (lane & 1);
+          held = block_at(key);
+          if (two) held2 = block_at(key + 8);
+        }
+      }
+      const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
+      const uint32_t dst = smem_u32(ring + in.stage * S::kTileBytes);
+      uint32_t bad = 0;
+#pragma unroll
+      for (int grp = 0; grp < 2; ++grp) {
+        const int key0 = from + kKeys * j + 32 * w + 16 * grp;
+        const int blk = __shfl_sync(0xffffffffu, held, 2 * (j & 15) + grp);
+        const int blk2 = two ? __shfl_sync(0xffffffffu, held2, 2 * (j & 15) + grp) : blk;
+        bad |= (blk < 0 && key0 < to ? 1u : 0u) << (2 * grp) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u) << (2 * grp);
+        const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
+        const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
+        const uint8_t* at0 = pool + slot0 * row_bytes + head_bytes;
+        const uint8_t* at1 = pool + slot1 * row_bytes + head_bytes;
+#pragma unroll
+        for (int k = 0; k < 16 * CPR / 32; ++k) {
+          const int idx = lane + 32 * k, r = idx / CPR, c = idx % CPR;
+          const bool take = key0 + r >= take_from && key0 + r < to && (r < 8 ? blk : blk2) >= 0;
+          const uint8_t* src = take ? (r < 8 ? at0 : at1) + r * row_bytes + c * 16 : pool;
+          const int rr = 32 * w + 16 * grp + r;
+          cp_async16(dst + (c >> 3) * (kKeys * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src, take);
+        }
+      }
+      if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
+      cp_async_commit();
+      in.next();
+      if (n >= kLag) {
+        cp_async_wait<kLag>();
+        announce();
+      }
+    }
+    cp_async_wait<0>();
+    while (ok && announced < 2 * steps) announce();
+  } else if (wg == 3) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 12 && lane == 0) {
+      // ---- matrix products
+      constexpr uint32_t id_s = tc_idesc<KIND>(kTileRows, kKeys, false), id_o = tc_idesc<KIND>(kTileRows, D, true);
+      Item<NS> item;  // the ring's next item: K of step j on entering step j
+      Item<NS> v;      // the V of step j - 1
+      uint32_t used[2] = {0, 0};  // products Q K^T issued per tile
+      bool ok = true, v_ready = false;
+      auto pv = [&](int i, bool accumulate) {
+        ok = ok && mbar_wait(&p_full[i], (used[i] - 1) & 1u);
+        if (ok && !v_ready) ok = mbar_wait(&full[v.stage], v.lap);
+        v_ready = true;
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t vs = smem_u32(ring + v.stage * S::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          tc_mma_ts(tmem + S::kO + i * D, tmem + i * 128 + 8 * k, desc_across(vs + k * 2048, kKeys * 128), id_o,
+                    accumulate || k > 0 ? 1u : 0u);
+        tc_commit(&o_done[i]);
+      };
+      for (int j = 0; j <= steps && ok; ++j) {
+        const bool k_here = j < steps;
+        bool k_ready = false;
+        v = item;  // (on entering step j > 0 the ring's next item is V of step j - 1, then K of step j)
+        if (j > 0) item.next();
+        v_ready = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j > 0 && j - 1 >= first[i] && j - 1 < last[i] && ok) pv(i, j - 1 > first[i]);
+          if (k_here && j >= first[i] && j < last[i] && ok) {
+            if (!k_ready) ok = mbar_wait(&full[item.stage], item.lap);
+            k_ready = true;
+            if (used[i] == 0) ok = ok && mbar_wait(&q_full[i], 0u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t qs = smem_u32(smem + i * S::kTileBytes), ks = smem_u32(ring + item.stage * S::kTileBytes);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t at_k = (k >> 2) * (kKeys * 128) + (k & 3) * 32;
+              tc_mma_ss(tmem + i * 128, desc_along(qs + at_k), desc_along(ks + at_k), id_s, k > 0 ? 1u : 0u);
+            }
+            ++used[i];
+            tc_commit(&s_full[i]);
+            mbar_arrive(&s_full[i]);
+          }
+        }
+        if (!ok) break;
+        if (j > 0) {
+          if (!v_ready) ok = mbar_wait(&full[v.stage], v.lap);  // no tile had keys in it: it still has to land
+          tc_commit(&empty[v.stage]);
+        }
+        if (k_here) {
+          if (!k_ready) ok = ok && mbar_wait(&full[item.stage], item.lap);
+          tc_commit(&empty[item.stage]);
+          item.next();
+        }
+      }
+      tc_commit(drained);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    softmax_rows<KIND, D>(a, at, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
+                          flags, slot + 1);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    (void)mbar_wait(drained, 0u);  // every product issued is complete before tensor memory is freed
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <int KIND, int D>
+int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
+  using S = TcShape<D>;
+  const void* kernel = reinterpret_cast<const void*>(paged_prefill_tc_kernel<KIND, D>);
+  // setmaxnreg hands out the registers of the launch: a build whose kernel was compiled to fewer would wait for ever
+  cudaFuncAttributes attr_of;
+  const cudaError_t asked = cudaFuncGetAttributes(&attr_of, kernel);
+  if (asked != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill: %s", cudaGetErrorString(asked));
+  BPT_REQUIRE(attr_of.numRegs == kLaunchRegs, BPT_ERR_CUDA, "paged prefill: kernel built with %d registers, not %d", attr_of.numRegs,
+              kLaunchRegs);
+  const int st = set_max_smem(kernel, S::kSmem);
+  if (st) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_tc_kernel<KIND, D>, a);
+  if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
+  return BPT_OK;
+}
+
+}  // namespace
+
+int take_prefill_tc_error() {
+  int value = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&value, g_device_error, sizeof(int)) != cudaSuccess) return -1;
+  if (value != 0) cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+  return value;
+}
+
+int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream) {
+  if (kind == BPT_KV_F16)
+    return a.D == 64 ? launch_tc<BPT_KV_F16, 64>(a, tiles, flags, stream) : launch_tc<BPT_KV_F16, 128>(a, tiles, flags, stream);
+  return a.D == 64 ? launch_tc<BPT_KV_BF16, 64>(a, tiles, flags, stream) : launch_tc<BPT_KV_BF16, 128>(a, tiles, flags, stream);
+}
+
+}  // namespace bpt

@@ -190,7 +190,8 @@ int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_str
  * `workspace`: bpt_paged_prefill_workspace_bytes(...) bytes (0: none needed), as for bpt_paged_read.
  * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024; rows of q start on 16 bytes.
  * Replaces: the prefill read of PagedKVCache + Attention.forward (engine/kv_cache.py:158-169, engine/attention.py:12-31). */
-int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens);
+int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int kind,
+                                          int64_t tokens);
 int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
                       const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
                       const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,

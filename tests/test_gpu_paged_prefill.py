@@ -258,7 +258,7 @@ def test_refusals_need_no_gpu():
     assert call(tokens=0) == _lib.ERR_INVALID and call(qt=516) == _lib.ERR_ALIGNMENT and call(out=72) == _lib.ERR_ALIGNMENT
     assert call(kind=2) == _lib.ERR_INVALID and call(T=-1) == _lib.ERR_INVALID and call(B=1 << 20) == _lib.ERR_INVALID
     few = {"T": 4, "tokens": 4000, "btw": 4000, "bts": 4000}
-    assert L.bpt_paged_prefill_workspace_bytes(4, 2, 4, 2, 128, 4000) > 0
+    assert L.bpt_paged_prefill_workspace_bytes(4, 2, 4, 2, 128, 4, 4000) > 0
     assert call(**few) == _lib.ERR_WORKSPACE and call(**few, ws=64, wsb=64) == _lib.ERR_WORKSPACE
     assert call(**few, ws=72, wsb=1 << 40) == _lib.ERR_ALIGNMENT
 
