@@ -20,13 +20,14 @@ raises ValueError, as in the reference (kv_attention.py:216-217).
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
 import torch
 
 from bpt_b200 import _lib
-from bpt_b200._lib import as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
+from bpt_b200._lib import addr, as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
 
 
 @dataclass
@@ -125,6 +126,7 @@ def paged_split(batch: int, tokens: int, block_size: int = 16, sms: int = 148) -
     return int(min(max(split, 4 * block_size), 64 * block_size))
 
 
+@functools.cache
 def _sms(device: torch.device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
@@ -145,26 +147,41 @@ _FORMATS = {"fp8": (_lib.KV_FP8, (torch.uint8, torch.float8_e4m3fn)), "int8": (_
 def pool_format(kv: PagedQuantKV):
     """(format code, k scale, v scale, k scale pool, v scale pool, blocks, block size, KV heads, head dim) of a paged cache of
     any kind, checked."""
-    if kv.kind not in _FORMATS:
-        raise ValueError(f"kind must be one of {', '.join(map(repr, _FORMATS))}, got {kv.kind!r}")
-    code, dtypes = _FORMATS[kv.kind]
+    kind = kv.kind
+    if kind not in _FORMATS:
+        raise ValueError(f"kind must be one of {', '.join(map(repr, _FORMATS))}, got {kind!r}")
+    code, dtypes = _FORMATS[kind]
     k, v = kv.k_pool, kv.v_pool
-    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous():
-        raise ValueError(f"pools must be contiguous [num_blocks, block_size, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError(f"pools must be contiguous [num_blocks, block_size, Hkv, D], got {tuple(shape)} and {tuple(v.shape)}")
     if k.dtype not in dtypes or v.dtype not in dtypes:
-        raise ValueError(f"{kv.kind!r} pools must be {dtypes[0]}, got {k.dtype} and {v.dtype}")
-    nb, bs, hkv, d = k.shape
+        raise ValueError(f"{kind!r} pools must be {dtypes[0]}, got {k.dtype} and {v.dtype}")
+    nb, bs, hkv, d = shape
     if kv.block_size != bs:
         raise ValueError(f"block_size is {kv.block_size}, the pools' blocks hold {bs}")
-    if kv.kind == "int8":
+    if kind == "int8":
         for s in (kv.k_scale, kv.v_scale):
-            if not (isinstance(s, torch.Tensor) and s.dtype == torch.float16 and tuple(s.shape) == (nb, bs, hkv)
+            if not (isinstance(s, torch.Tensor) and s.dtype == torch.float16 and s.shape == (nb, bs, hkv)
                     and s.is_contiguous() and s.device == k.device):
                 raise ValueError("int8 pools need fp16 k_scale / v_scale of shape [num_blocks, block_size, Hkv]")
         return code, 1.0, 1.0, kv.k_scale, kv.v_scale, nb, bs, hkv, d
-    if kv.kind == "fp8":
+    if kind == "fp8":
         return code, float(kv.k_scale), float(kv.v_scale), None, None, nb, bs, hkv, d
     return code, 1.0, 1.0, None, None, nb, bs, hkv, d
+
+
+def block_table_of(kv: PagedQuantKV, batch: int | None = None) -> tuple[torch.Tensor, int, int, int]:
+    """(table, rows, row stride, width) of a paged cache's block table, checked."""
+    table = kv.block_table
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != torch.int32 or (batch is not None and shape[0] != batch):
+        raise ValueError(f"the block table must be int32 [{'B' if batch is None else batch}, blocks], got {table.dtype} "
+                         f"{tuple(shape)}")
+    stride = table.stride()
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"the block table's rows must be contiguous, got strides {stride}")
+    return table, shape[0], stride[0] if shape[0] > 1 else shape[1], shape[1]
 
 
 def paged_read_split(batch: int, heads: int, keys: int, sms: int = 148) -> int:
@@ -178,8 +195,10 @@ def _row_tensor(name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dt
     """An optional per-row argument, in the dtype the kernels take."""
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if t.dtype == dtype and t.is_contiguous():
+        return t
     return as_int32(t) if dtype == torch.int32 else t.to(dtype).contiguous()
 
 
@@ -188,13 +207,12 @@ def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_
     """`attend` (or, with partials, `decode_attention`) over a paged cache of any kind with any of the score options."""
     device = require_cuda(q, lengths, kv.k_pool, kv.v_pool, kv.block_table, alibi_slopes, key_starts, out, workspace)
     code, ks, vs, kss, vss, nb, bs, hkv, d = pool_format(kv)
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % hkv:
-        raise ValueError(f"pool shape {tuple(kv.k_pool.shape)} does not match q {tuple(q.shape)}")
-    b, hq, _ = q.shape
-    table = kv.block_table
-    if table.dim() != 2 or table.shape[0] != b or table.dtype != torch.int32 or table.stride(1) != 1:
-        raise ValueError(f"the block table must be int32 [{b}, blocks], got {table.dtype} {tuple(table.shape)}")
-    if tuple(lengths.shape) != (b,):
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % hkv:
+        raise ValueError(f"pool shape {tuple(kv.k_pool.shape)} does not match q {tuple(shape)}")
+    b, hq, _ = shape
+    table, _, table_stride, table_width = block_table_of(kv, b)
+    if lengths.shape != (b,):
         raise ValueError(f"lengths must be [{b}], got {tuple(lengths.shape)}")
     if window < 0 or softcap < 0:
         raise ValueError(f"window and softcap must not be negative, got {window} and {softcap}")
@@ -202,7 +220,7 @@ def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_
         q, lengths = _q_view(q), as_int32(lengths)
         slopes = _row_tensor("alibi_slopes", alibi_slopes, (hq,), torch.float32)
         starts = _row_tensor("key_starts", key_starts, (b,), torch.int32)
-        tokens = kv.tokens if tokens is None else tokens
+        tokens = table_width * bs if tokens is None else tokens
         keys = max(tokens, 1) if partials or not window else max(1, min(tokens, window + 15))  # a window starts anywhere
         if split is None:
             split = paged_read_split(b, hkv * -(-hq // hkv // 8), keys, _sms(device))
@@ -210,23 +228,24 @@ def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_
             raise ValueError(f"split {split} must be a multiple of 16")
         n_splits = -(-keys // split)
         part_out = part_lse = None
-        need = 0
+        room = 0
         if partials:
             part_out = torch.empty((b, hq, n_splits, d), dtype=torch.float32, device=device)
             part_lse = torch.empty((b, hq, n_splits), dtype=torch.float32, device=device)
         else:
             if out is None:
-                out = torch.empty((b, hq, d), dtype=torch.float32, device=device)
-            elif tuple(out.shape) != (b, hq, d) or not out.is_contiguous():
+                out = torch.empty(shape, dtype=torch.float32, device=device)
+            elif out.shape != shape or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{b}, {hq}, {d}] tensor")
             if n_splits > 1 and workspace is None:
                 workspace = _zeroed_workspace(int(lib().bpt_paged_read_workspace_bytes(b, hq, d, n_splits)), device)
-            need = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        st = lib().bpt_paged_read(
-            ptr(q), dtype_code(q.dtype), q.stride(0), q.stride(1), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs, ptr(kss),
-            ptr(vss), ptr(table), table.stride(0) if b > 1 else table.shape[1], table.shape[1], ptr(lengths), ptr(starts),
-            ptr(slopes), float(softcap), int(window), b, hq, hkv, d, bs, nb, split, n_splits, float(scale), ptr(out),
-            dtype_code(out.dtype) if out is not None else 0, ptr(part_out), ptr(part_lse), ptr(workspace), need, flags,
+            room = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        q_stride = q.stride()
+        st = _lib.paged_read(
+            q.data_ptr(), dtype_code(q.dtype), q_stride[0], q_stride[1], kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks,
+            vs, addr(kss), addr(vss), table.data_ptr(), table_stride, table_width, lengths.data_ptr(), addr(starts),
+            addr(slopes), softcap, window, b, hq, hkv, d, bs, nb, split, n_splits, scale, addr(out),
+            0 if out is None else dtype_code(out.dtype), addr(part_out), addr(part_lse), addr(workspace), room, flags,
             stream_of(device))
     check(st, "decode_attention (paged)" if partials else "attend (paged)")
     return (part_out, part_lse) if partials else out

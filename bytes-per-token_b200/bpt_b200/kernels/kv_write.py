@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from bpt_b200 import _lib
-from bpt_b200._lib import FLAG_PDL, as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
+from bpt_b200._lib import FLAG_PDL, addr, as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
 from bpt_b200.kernels.kv_attention import PagedQuantKV, QuantKV, pool_format
 
 
@@ -56,12 +56,13 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 1e6, device="cuda
     return angle.cos().float(), angle.sin().float()
 
 
-def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
-    """x [T, H, D], or a copy of it whose rows start on 16 bytes."""
-    unit = 16 // x.element_size()
-    if x.stride(2) == 1 and x.stride(0) % unit == 0 and x.stride(1) % unit == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _aligned_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """x [T, H, D] and its strides, or a copy's whose rows start on 16 bytes."""
+    unit, stride = 16 // x.element_size(), x.stride()
+    if stride[2] != 1 or stride[0] % unit or stride[1] % unit or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        stride = x.stride()
+    return x, stride
 
 
 def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: PagedQuantKV, positions: torch.Tensor,
@@ -79,39 +80,43 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: PagedQ
     """
     device = require_cuda(q, k, v, kv.k_pool, kv.v_pool, positions, cos, sin, write_blocks, write_offsets, q_norm, k_norm,
                           q_out)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"q must be [T, Hq, D], k and v [T, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)} and "
+    q_shape, k_shape, dtype = q.shape, k.shape, q.dtype
+    if len(q_shape) != 3 or len(k_shape) != 3 or k_shape != v.shape or q_shape[::2] != k_shape[::2]:
+        raise ValueError(f"q must be [T, Hq, D], k and v [T, Hkv, D], got {tuple(q_shape)}, {tuple(k_shape)} and "
                          f"{tuple(v.shape)}")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise ValueError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
-    t, hq, d = q.shape
-    hkv = k.shape[1]
+    if dtype != k.dtype or dtype != v.dtype:
+        raise ValueError(f"q, k and v must share a dtype, got {dtype}, {k.dtype} and {v.dtype}")
+    t, hq, d = q_shape
+    hkv = k_shape[1]
     code, ks, vs, kss, vss, nb, bs, pool_heads, pool_dim = pool_format(kv)
-    if (hkv, d) != (pool_heads, pool_dim):
+    if hkv != pool_heads or d != pool_dim:
         raise ValueError(f"k has {hkv} heads of {d}, the pool {pool_heads} of {pool_dim}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    table = cos.shape
+    if len(table) != 2 or table != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos and sin must be float32 [positions, rotary / 2]")
     for w in (q_norm, k_norm):
-        if w is not None and (tuple(w.shape) != (d,) or w.dtype != q.dtype):
-            raise ValueError(f"norm weights must be [{d}] in {q.dtype}")
-    for x in (positions, write_blocks, write_offsets):
-        if x.numel() != t:
-            raise ValueError(f"positions, write_blocks and write_offsets must hold {t} entries")
-    if q_out is None:
-        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
-    elif tuple(q_out.shape) != (t, hq, d) or q_out.dtype != q.dtype or not q_out.is_contiguous():
-        raise ValueError(f"q_out must be a contiguous [{t}, {hq}, {d}] tensor of {q.dtype}")
+        if w is not None and (w.shape != (d,) or w.dtype != dtype):
+            raise ValueError(f"norm weights must be [{d}] in {dtype}")
+    if positions.numel() != t or write_blocks.numel() != t or write_offsets.numel() != t:
+        raise ValueError(f"positions, write_blocks and write_offsets must hold {t} entries")
+    if q_out is not None and (q_out.shape != q_shape or q_out.dtype != dtype or not q_out.is_contiguous()):
+        raise ValueError(f"q_out must be a contiguous [{t}, {hq}, {d}] tensor of {dtype}")
     with on_device(device):
-        q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+        if q_out is None:
+            q_out = torch.empty(q_shape, dtype=dtype, device=device)
+        q, q_stride = _aligned_rows(q)
+        k, k_stride = _aligned_rows(k)
+        v, v_stride = _aligned_rows(v)
         cos, sin = cos.contiguous(), sin.contiguous()
         q_norm = q_norm if q_norm is None else q_norm.contiguous()
         k_norm = k_norm if k_norm is None else k_norm.contiguous()
         pos, wb, wo = as_int32(positions), as_int32(write_blocks), as_int32(write_offsets)
-        st = lib().bpt_rope_kv_append(
-            ptr(q), ptr(k), ptr(v), dtype_code(q.dtype), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), t, hq, hkv, d, 2 * cos.shape[1], ptr(pos), ptr(cos), ptr(sin), cos.shape[0], int(interleaved),
-            ptr(q_norm), ptr(k_norm), float(eps), ptr(q_out), ptr(wb), ptr(wo), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs,
-            ptr(kss), ptr(vss), bs, nb, FLAG_PDL if pdl else 0, stream_of(device))
+        st = _lib.rope_kv_append(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(dtype), q_stride[0], q_stride[1], k_stride[0], k_stride[1],
+            v_stride[0], v_stride[1], t, hq, hkv, d, 2 * table[1], pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), table[0],
+            interleaved, addr(q_norm), addr(k_norm), eps, q_out.data_ptr(), wb.data_ptr(), wo.data_ptr(),
+            kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks, vs, addr(kss), addr(vss), bs, nb,
+            FLAG_PDL if pdl else 0, stream_of(device))
     check(st, "rope_kv_append")
     return q_out
 

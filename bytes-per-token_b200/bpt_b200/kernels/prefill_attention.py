@@ -9,8 +9,9 @@ from __future__ import annotations
 
 import torch
 
-from bpt_b200._lib import FLAG_PDL, as_int32, check, dtype_code, lib, on_device, ptr, require_cuda, stream_of
-from bpt_b200.kernels.kv_attention import PagedQuantKV, _row_tensor, _zeroed_workspace, pool_format
+from bpt_b200 import _lib
+from bpt_b200._lib import FLAG_PDL, addr, as_int32, check, dtype_code, lib, on_device, require_cuda, stream_of
+from bpt_b200.kernels.kv_attention import PagedQuantKV, _row_tensor, _zeroed_workspace, block_table_of, pool_format
 
 
 def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, lengths: torch.Tensor, scale: float, *,
@@ -34,42 +35,41 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
     device = require_cuda(q, kv.k_pool, kv.v_pool, kv.block_table, cu_seqlens, lengths, positions, alibi_slopes, key_starts,
                           prefix_lens, out, workspace)
     code, ks, vs, kss, vss, nb, bs, hkv, d = pool_format(kv)
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % hkv:
-        raise ValueError(f"pool shape {tuple(kv.k_pool.shape)} does not match q {tuple(q.shape)}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % hkv:
+        raise ValueError(f"pool shape {tuple(kv.k_pool.shape)} does not match q {tuple(shape)}")
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"q must be float16 or bfloat16, got {q.dtype}")
-    t, hq, _ = q.shape
-    table = kv.block_table
-    b = table.shape[0]
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
-        raise ValueError(f"the block table must be int32 [B, blocks], got {table.dtype} {tuple(table.shape)}")
-    if tuple(cu_seqlens.shape) != (b + 1,) or tuple(lengths.shape) != (b,):
+    t, hq, _ = shape
+    table, b, table_stride, table_width = block_table_of(kv)
+    if cu_seqlens.shape != (b + 1,) or lengths.shape != (b,):
         raise ValueError(f"cu_seqlens must be [{b + 1}] and lengths [{b}], got {tuple(cu_seqlens.shape)} and "
                          f"{tuple(lengths.shape)}")
     if window < 0 or softcap < 0:
         raise ValueError(f"window and softcap must not be negative, got {window} and {softcap}")
-    if out is not None and (tuple(out.shape) != (t, hq, d) or out.dtype != q.dtype or not out.is_contiguous()):
+    if out is not None and (out.shape != shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous [{t}, {hq}, {d}] tensor of {q.dtype}")
-    tokens = max(kv.tokens if tokens is None else int(tokens), 1)
+    tokens = max(table_width * bs if tokens is None else int(tokens), 1)
     with on_device(device):
-        if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        stride = q.stride()
+        if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
+            stride = q.stride()
         cu, lengths = as_int32(cu_seqlens), as_int32(lengths)
         positions = _row_tensor("positions", positions, (t,), torch.int32)
         starts = _row_tensor("key_starts", key_starts, (t,), torch.int32)
         prefix = _row_tensor("prefix_lens", prefix_lens, (b,), torch.int32)
         slopes = _row_tensor("alibi_slopes", alibi_slopes, (hq,), torch.float32)
         if out is None:
-            out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
+            out = torch.empty(shape, dtype=q.dtype, device=device)
         if workspace is None:
             need = int(lib().bpt_paged_prefill_workspace_bytes(t, b, hq, hkv, d, code, tokens))
             workspace = _zeroed_workspace(need, device) if need else None
-        st = lib().bpt_paged_prefill(
-            ptr(q), dtype_code(q.dtype), q.stride(0), q.stride(1), ptr(kv.k_pool), ptr(kv.v_pool), code, ks, vs, ptr(kss),
-            ptr(vss), ptr(table), table.stride(0) if b > 1 else table.shape[1], table.shape[1], ptr(cu), ptr(lengths),
-            ptr(positions), ptr(starts), ptr(prefix), ptr(slopes), float(softcap), int(window), t, b, hq, hkv, d, bs, nb, tokens,
-            float(scale), ptr(out), ptr(workspace),
-            0 if workspace is None else workspace.numel() * workspace.element_size(), FLAG_PDL if pdl else 0,
-            stream_of(device))
+        st = _lib.paged_prefill(
+            q.data_ptr(), dtype_code(q.dtype), stride[0], stride[1], kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks, vs,
+            addr(kss), addr(vss), table.data_ptr(), table_stride, table_width, cu.data_ptr(), lengths.data_ptr(),
+            addr(positions), addr(starts), addr(prefix), addr(slopes), softcap, window, t, b, hq, hkv, d, bs, nb, tokens, scale,
+            out.data_ptr(), addr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            FLAG_PDL if pdl else 0, stream_of(device))
     check(st, "prefill_attend")
     return out

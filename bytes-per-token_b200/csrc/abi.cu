@@ -63,6 +63,16 @@ int set_max_smem(const void* kernel, int bytes) {
   return BPT_OK;
 }
 
+int set_max_smem_once(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_max_smem(kernel, bytes);
+  const uint64_t bit = uint64_t(1) << dev;
+  if (done.load(std::memory_order_relaxed) & bit) return BPT_OK;
+  const int st = set_max_smem(kernel, bytes);
+  if (st == BPT_OK) done.fetch_or(bit, std::memory_order_relaxed);
+  return st;
+}
+
 int take_prefill_tc_error();  // the same read-and-clear of csrc/paged_prefill_tc.cu's own flag
 
 }  // namespace bpt

@@ -11,6 +11,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/bpt_b200.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -25,6 +27,8 @@ int set_error(int status, const char* fmt, ...);
 int check_launch(const char* what);
 int num_sms();
 int set_max_smem(const void* kernel, int bytes);
+// The same, once per device: `done` (one per kernel, zero at first) has a bit for each of the first 64.
+int set_max_smem_once(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 // The driver's cuTensorMapEncodeTiled (a PFN_cuTensorMapEncodeTiled_v12000), or null if the driver lacks it.
 void* tensor_map_encoder();
 

@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
 template <int KIND, int D>
 int launch_prefill(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
   using S = PrefillShape<KIND, D>;
-  const int st = set_max_smem(reinterpret_cast<const void*>(paged_prefill_kernel<KIND, D>), S::kSmem);
+  static std::atomic<uint64_t> ready{0};
+  const int st = set_max_smem_once(reinterpret_cast<const void*>(paged_prefill_kernel<KIND, D>), S::kSmem, ready);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
@@ -345,14 +346,44 @@ extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64
   return p.n_splits > 1 ? kTicketBytes + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
 }
 
-extern "C" int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
-                                 const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
-                                 const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
-                                 const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions,
-                                 const int32_t* key_starts, const int32_t* prefix_lens, const float* alibi_slopes,
-                                 float softcap, int64_t window, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                                 int64_t block_size, int64_t num_blocks, int64_t tokens, float sm_scale, void* out,
-                                 void* workspace, int64_t workspace_bytes, int flags, void* stream) {
+extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
+  BPT_REQUIRE(args, BPT_ERR_INVALID, "paged prefill: null arguments");
+  const void* const q = args->q;
+  const int q_dtype = int(args->q_dtype);
+  const int64_t q_stride_t = args->q_stride_t;
+  const int64_t q_stride_h = args->q_stride_h;
+  const void* const k_pool = args->k_pool;
+  const void* const v_pool = args->v_pool;
+  const int kind = int(args->kind);
+  const float k_scale = float(args->k_scale);
+  const float v_scale = float(args->v_scale);
+  const void* const k_scales = args->k_scales;
+  const void* const v_scales = args->v_scales;
+  const int32_t* const block_table = args->block_table;
+  const int64_t bt_stride = args->bt_stride;
+  const int64_t bt_width = args->bt_width;
+  const int32_t* const cu_seqlens = args->cu_seqlens;
+  const int32_t* const lengths = args->lengths;
+  const int32_t* const positions = args->positions;
+  const int32_t* const key_starts = args->key_starts;
+  const int32_t* const prefix_lens = args->prefix_lens;
+  const float* const alibi_slopes = args->alibi_slopes;
+  const float softcap = float(args->softcap);
+  const int64_t window = args->window;
+  const int64_t T = args->T;
+  const int64_t B = args->B;
+  const int64_t Hq = args->Hq;
+  const int64_t Hkv = args->Hkv;
+  const int64_t D = args->D;
+  const int64_t block_size = args->block_size;
+  const int64_t num_blocks = args->num_blocks;
+  const int64_t tokens = args->tokens;
+  const float sm_scale = float(args->sm_scale);
+  void* const out = args->out;
+  void* const workspace = args->workspace;
+  const int64_t workspace_bytes = args->workspace_bytes;
+  const int flags = int(args->flags);
+  void* const stream = args->stream;
   const char* who = "paged prefill";
   BPT_REQUIRE(T >= 0 && T < (1ll << 30) && B >= 0 && B < (1 << 20), BPT_ERR_INVALID, "%s: T=%lld B=%lld", who, (long long)T,
               (long long)B);

@@ -580,13 +580,16 @@ template <int KIND, int D>
 int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
   using S = TcShape<D>;
   const void* kernel = reinterpret_cast<const void*>(paged_prefill_tc_kernel<KIND, D>);
-  // setmaxnreg hands out the registers of the launch: a build whose kernel was compiled to fewer would wait for ever
-  cudaFuncAttributes attr_of;
-  const cudaError_t asked = cudaFuncGetAttributes(&attr_of, kernel);
-  if (asked != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill: %s", cudaGetErrorString(asked));
-  BPT_REQUIRE(attr_of.numRegs == kLaunchRegs, BPT_ERR_CUDA, "paged prefill: kernel built with %d registers, not %d", attr_of.numRegs,
-              kLaunchRegs);
-  const int st = set_max_smem(kernel, S::kSmem);
+  static std::atomic<uint64_t> ready{0};
+  if (ready.load(std::memory_order_relaxed) == 0) {
+    // setmaxnreg hands out the registers of the launch: a build whose kernel was compiled to fewer would wait for ever
+    cudaFuncAttributes attr_of;
+    const cudaError_t asked = cudaFuncGetAttributes(&attr_of, kernel);
+    if (asked != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill: %s", cudaGetErrorString(asked));
+    BPT_REQUIRE(attr_of.numRegs == kLaunchRegs, BPT_ERR_CUDA, "paged prefill: kernel built with %d registers, not %d",
+                attr_of.numRegs, kLaunchRegs);
+  }
+  const int st = set_max_smem_once(kernel, S::kSmem, ready);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));

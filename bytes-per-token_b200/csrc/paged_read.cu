@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
 template <int KIND, int D>
 int launch_read(const ReadArgs& a, int flags, cudaStream_t stream) {
   using S = ReadShape<KIND, D>;
-  const int st = set_max_smem(reinterpret_cast<const void*>(paged_read_kernel<KIND, D>), S::kSmem);
+  static std::atomic<uint64_t> ready{0};
+  const int st = set_max_smem_once(reinterpret_cast<const void*>(paged_read_kernel<KIND, D>), S::kSmem, ready);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.n_splits), unsigned(a.src.Hkv * a.tiles), unsigned(a.B));
@@ -382,14 +383,44 @@ extern "C" int64_t bpt_paged_read_workspace_bytes(int64_t B, int64_t Hq, int64_t
   return n_splits > 1 ? read_workspace(B, Hq, D, n_splits) : 0;
 }
 
-extern "C" int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, const void* k_pool,
-                              const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
-                              const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
-                              const int32_t* lengths, const int32_t* key_starts, const float* alibi_slopes, float softcap,
-                              int64_t window, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size,
-                              int64_t num_blocks, int64_t split, int64_t n_splits, float sm_scale, void* out, int out_dtype,
-                              float* out_partial, float* lse_partial, void* workspace, int64_t workspace_bytes, int flags,
-                              void* stream) {
+extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
+  BPT_REQUIRE(args, BPT_ERR_INVALID, "paged read: null arguments");
+  const void* const q = args->q;
+  const int q_dtype = int(args->q_dtype);
+  const int64_t q_stride_b = args->q_stride_b;
+  const int64_t q_stride_h = args->q_stride_h;
+  const void* const k_pool = args->k_pool;
+  const void* const v_pool = args->v_pool;
+  const int kind = int(args->kind);
+  const float k_scale = float(args->k_scale);
+  const float v_scale = float(args->v_scale);
+  const void* const k_scales = args->k_scales;
+  const void* const v_scales = args->v_scales;
+  const int32_t* const block_table = args->block_table;
+  const int64_t bt_stride = args->bt_stride;
+  const int64_t bt_width = args->bt_width;
+  const int32_t* const lengths = args->lengths;
+  const int32_t* const key_starts = args->key_starts;
+  const float* const alibi_slopes = args->alibi_slopes;
+  const float softcap = float(args->softcap);
+  const int64_t window = args->window;
+  const int64_t B = args->B;
+  const int64_t Hq = args->Hq;
+  const int64_t Hkv = args->Hkv;
+  const int64_t D = args->D;
+  const int64_t block_size = args->block_size;
+  const int64_t num_blocks = args->num_blocks;
+  const int64_t split = args->split;
+  const int64_t n_splits = args->n_splits;
+  const float sm_scale = float(args->sm_scale);
+  void* const out = args->out;
+  const int out_dtype = int(args->out_dtype);
+  float* const out_partial = args->out_partial;
+  float* const lse_partial = args->lse_partial;
+  void* const workspace = args->workspace;
+  const int64_t workspace_bytes = args->workspace_bytes;
+  const int flags = int(args->flags);
+  void* const stream = args->stream;
   const char* who = "paged read";
   BPT_REQUIRE(B >= 0 && B < 65536, BPT_ERR_INVALID, "%s: B=%lld", who, (long long)B);
   if (B == 0) return BPT_OK;

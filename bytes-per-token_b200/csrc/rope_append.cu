@@ -278,14 +278,45 @@ int append_dim(const AppendArgs& a, int64_t D, int kind, bool interleaved, int f
 
 using namespace bpt;
 
-extern "C" int bpt_rope_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_t,
-                                  int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
-                                  int64_t v_stride_h, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rotary,
-                                  const int32_t* positions, const float* cos, const float* sin, int64_t table_rows,
-                                  int interleaved, const void* q_norm, const void* k_norm, float eps, void* q_out,
-                                  const int32_t* write_blocks, const int32_t* write_offsets, void* k_pool, void* v_pool,
-                                  int kind, float k_scale, float v_scale, void* k_scales, void* v_scales,
-                                  int64_t block_size, int64_t num_blocks, int flags, void* stream) {
+extern "C" int bpt_rope_kv_append(const bpt_rope_kv_append_args* args) {
+  BPT_REQUIRE(args, BPT_ERR_INVALID, "rope_kv_append: null arguments");
+  const void* const q = args->q;
+  const void* const k = args->k;
+  const void* const v = args->v;
+  const int dtype = int(args->dtype);
+  const int64_t q_stride_t = args->q_stride_t;
+  const int64_t q_stride_h = args->q_stride_h;
+  const int64_t k_stride_t = args->k_stride_t;
+  const int64_t k_stride_h = args->k_stride_h;
+  const int64_t v_stride_t = args->v_stride_t;
+  const int64_t v_stride_h = args->v_stride_h;
+  const int64_t T = args->T;
+  const int64_t Hq = args->Hq;
+  const int64_t Hkv = args->Hkv;
+  const int64_t D = args->D;
+  const int64_t rotary = args->rotary;
+  const int32_t* const positions = args->positions;
+  const float* const cos = args->cos;
+  const float* const sin = args->sin;
+  const int64_t table_rows = args->table_rows;
+  const int interleaved = int(args->interleaved);
+  const void* const q_norm = args->q_norm;
+  const void* const k_norm = args->k_norm;
+  const float eps = float(args->eps);
+  void* const q_out = args->q_out;
+  const int32_t* const write_blocks = args->write_blocks;
+  const int32_t* const write_offsets = args->write_offsets;
+  void* const k_pool = args->k_pool;
+  void* const v_pool = args->v_pool;
+  const int kind = int(args->kind);
+  const float k_scale = float(args->k_scale);
+  const float v_scale = float(args->v_scale);
+  void* const k_scales = args->k_scales;
+  void* const v_scales = args->v_scales;
+  const int64_t block_size = args->block_size;
+  const int64_t num_blocks = args->num_blocks;
+  const int flags = int(args->flags);
+  void* const stream = args->stream;
   BPT_REQUIRE(T >= 0 && T < (1ll << 31), BPT_ERR_INVALID, "rope_kv_append: T=%lld", (long long)T);
   if (T == 0) return BPT_OK;
   BPT_REQUIRE(q && k && v && positions && cos && sin && q_out && write_blocks && write_offsets && k_pool && v_pool,

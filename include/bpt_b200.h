@@ -169,13 +169,28 @@ int bpt_paged_attend(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_s
  * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024, split a multiple of 16.
  * Replaces: as bpt_paged_attend, for the reference's unquantized pages too (engine/kv_cache.py:98-169). */
 int64_t bpt_paged_read_workspace_bytes(int64_t B, int64_t Hq, int64_t D, int64_t n_splits);
-int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_stride_h, const void* k_pool,
-                   const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales, const void* v_scales,
-                   const int32_t* block_table, int64_t bt_stride, int64_t bt_width, const int32_t* lengths,
-                   const int32_t* key_starts, const float* alibi_slopes, float softcap, int64_t window, int64_t B,
-                   int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size, int64_t num_blocks, int64_t split,
-                   int64_t n_splits, float sm_scale, void* out, int out_dtype, float* out_partial, float* lse_partial,
-                   void* workspace, int64_t workspace_bytes, int flags, void* stream);
+typedef struct {
+  const void *q;
+  int64_t q_dtype, q_stride_b, q_stride_h;
+  const void *k_pool, *v_pool;
+  int64_t kind;
+  double k_scale, v_scale;
+  const void *k_scales, *v_scales;
+  const int32_t *block_table;
+  int64_t bt_stride, bt_width;
+  const int32_t *lengths, *key_starts;
+  const float *alibi_slopes;
+  double softcap;
+  int64_t window, B, Hq, Hkv, D, block_size, num_blocks, split, n_splits;
+  double sm_scale;
+  void *out;
+  int64_t out_dtype;
+  float *out_partial, *lse_partial;
+  void *workspace;
+  int64_t workspace_bytes, flags;
+  void *stream;
+} bpt_paged_read_args;
+int bpt_paged_read(const bpt_paged_read_args* args);
 
 /* Prefill attention over a paged cache of any format: q [T, Hq, D] (f16 or bf16; the pages' own type where they are 16-bit)
  * holds the new tokens of B sequences, sequence b's in rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]; rows of
@@ -192,14 +207,25 @@ int bpt_paged_read(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_str
  * Replaces: the prefill read of PagedKVCache + Attention.forward (engine/kv_cache.py:158-169, engine/attention.py:12-31). */
 int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int kind,
                                           int64_t tokens);
-int bpt_paged_prefill(const void* q, int q_dtype, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
-                      const void* v_pool, int kind, float k_scale, float v_scale, const void* k_scales,
-                      const void* v_scales, const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
-                      const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions,
-                      const int32_t* key_starts, const int32_t* prefix_lens, const float* alibi_slopes, float softcap,
-                      int64_t window, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size,
-                      int64_t num_blocks, int64_t tokens, float sm_scale, void* out, void* workspace,
-                      int64_t workspace_bytes, int flags, void* stream);
+typedef struct {
+  const void *q;
+  int64_t q_dtype, q_stride_t, q_stride_h;
+  const void *k_pool, *v_pool;
+  int64_t kind;
+  double k_scale, v_scale;
+  const void *k_scales, *v_scales;
+  const int32_t *block_table;
+  int64_t bt_stride, bt_width;
+  const int32_t *cu_seqlens, *lengths, *positions, *key_starts, *prefix_lens;
+  const float *alibi_slopes;
+  double softcap;
+  int64_t window, T, B, Hq, Hkv, D, block_size, num_blocks, tokens;
+  double sm_scale;
+  void *out, *workspace;
+  int64_t workspace_bytes, flags;
+  void *stream;
+} bpt_paged_prefill_args;
+int bpt_paged_prefill(const bpt_paged_prefill_args* args);
 
 /* bpt_paged_attend without a workspace argument, for callers that cannot allocate device memory: serving
  * engines that hand all free HBM to their paged KV pool at start-up (so a later cudaMalloc fails or fragments
@@ -300,13 +326,24 @@ int bpt_qk_norm_rope_kv_write(const void* qkv, int64_t ld, int64_t B, int64_t Hq
  * one call must be distinct. D in {64, 128, 256}, rotary a multiple of 16 from 16 to D; rows of q, k, v start
  * on 16 bytes. Replaces: rope.apply (engine/rope.py:31-43), q_norm / k_norm (engine/model.py:63-70) and the cache write
  * (engine/kv_cache.py:150-161) for any number of tokens and any of the cache's formats. */
-int bpt_rope_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_t, int64_t q_stride_h,
-                       int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, int64_t T,
-                       int64_t Hq, int64_t Hkv, int64_t D, int64_t rotary, const int32_t* positions, const float* cos,
-                       const float* sin, int64_t table_rows, int interleaved, const void* q_norm, const void* k_norm,
-                       float eps, void* q_out, const int32_t* write_blocks, const int32_t* write_offsets, void* k_pool,
-                       void* v_pool, int kind, float k_scale, float v_scale, void* k_scales, void* v_scales,
-                       int64_t block_size, int64_t num_blocks, int flags, void* stream);
+typedef struct {
+  const void *q, *k, *v;
+  int64_t dtype, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, T, Hq, Hkv, D, rotary;
+  const int32_t *positions;
+  const float *cos, *sin;
+  int64_t table_rows, interleaved;
+  const void *q_norm, *k_norm;
+  double eps;
+  void *q_out;
+  const int32_t *write_blocks, *write_offsets;
+  void *k_pool, *v_pool;
+  int64_t kind;
+  double k_scale, v_scale;
+  void *k_scales, *v_scales;
+  int64_t block_size, num_blocks, flags;
+  void *stream;
+} bpt_rope_kv_append_args;
+int bpt_rope_kv_append(const bpt_rope_kv_append_args* args);
 
 /* RMSNorm fused with per-token symmetric INT8 quantization (the activation quantizer before a W8A8 linear):
  * for every row of x [rows, d] (x_dtype, row stride x_row_stride elements, unit inner stride) and weight [d]

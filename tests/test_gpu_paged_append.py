@@ -199,7 +199,7 @@ def test_refusals_need_no_gpu():
              "Hq": 4, "Hkv": 2, "D": 128, "rotary": 128, "pos": 64, "cos": 64, "sin": 64, "rows": 8, "il": 0, "qn": None,
              "kn": None, "eps": 1e-6, "out": 64, "wb": 64, "wo": 64, "kp": 64, "vp": 64, "kind": 4, "ksc": 1.0, "vsc": 1.0,
              "kss": None, "vss": None, "bs": 16, "nb": 4, "flags": 0, "stream": None} | kw
-        return L.bpt_rope_kv_append(*a.values())
+        return _lib.rope_kv_append(*(0 if x is None else x for x in a.values()))
 
     assert call(T=0) == _lib.OK
     assert call(T=-1) == _lib.ERR_INVALID

@@ -247,7 +247,7 @@ def test_refusals_need_no_gpu():
              "bt": 64, "bts": 4, "btw": 4, "cu": 64, "len": 64, "pos": None, "starts": None, "prefix": None, "slopes": None,
              "cap": 0.0, "window": 0, "T": 20000, "B": 2, "Hq": 4, "Hkv": 2, "D": 128, "bs": 16, "nb": 8, "tokens": 64,
              "scale": 1.0, "out": 64, "ws": None, "wsb": 0, "flags": 0, "stream": None} | kw
-        return L.bpt_paged_prefill(*a.values())
+        return _lib.paged_prefill(*(0 if x is None else x for x in a.values()))
 
     assert call(T=0) == _lib.OK and call(B=0) == _lib.OK
     for name in ("q", "kp", "vp", "bt", "cu", "len", "out"):

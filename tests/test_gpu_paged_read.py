@@ -229,7 +229,7 @@ def test_refusals_need_no_gpu():
              "bt": 64, "bts": 4, "btw": 4, "len": 64, "starts": None, "slopes": None, "cap": 0.0, "window": 0, "B": 2, "Hq": 4,
              "Hkv": 2, "D": 128, "bs": 16, "nb": 8, "split": 64, "n": 1, "scale": 1.0, "out": 64, "od": 2, "po": None,
              "pl": None, "ws": None, "wsb": 0, "flags": 0, "stream": None} | kw
-        return L.bpt_paged_read(*a.values())
+        return _lib.paged_read(*(0 if x is None else x for x in a.values()))
 
     assert call(B=0) == _lib.OK
     for name in ("q", "kp", "vp", "bt", "len", "out"):
