@@ -47,7 +47,7 @@ SIGNATURES: dict[str, list] = {
                          F32, P, I32, P, I64, I32, P],
     "bpt_paged_attend_noalloc": [P, I32, I64, I64, P, P, I32, F32, F32, P, P, P, I64, P, I64, I64, I64, I64, I64, I64,
                                  I64, I64, F32, P, I32, I32, P],
-    "bpt_paged_read_workspace_bytes": [I64, I64, I64, I64],
+    "bpt_paged_read_workspace_bytes": [I64, I64, I64, I32],
     "bpt_paged_read": [ctypes.c_char_p],
     "bpt_paged_prefill_workspace_bytes": [I64, I64, I64, I64, I64, I32, I64],
     "bpt_paged_prefill": [ctypes.c_char_p],
@@ -101,7 +101,7 @@ paged_read = ArgStruct(
     "bpt_paged_read", (
         "q:P q_dtype:q q_stride_b:q q_stride_h:q k_pool:P v_pool:P kind:q k_scale:d v_scale:d k_scales:P v_scales:P "
         "block_table:P bt_stride:q bt_width:q lengths:P key_starts:P alibi_slopes:P softcap:d window:q B:q Hq:q Hkv:q "
-        "D:q block_size:q num_blocks:q split:q n_splits:q sm_scale:d out:P out_dtype:q out_partial:P lse_partial:P "
+        "D:q block_size:q num_blocks:q split:q n_splits:q tokens:q sm_scale:d out:P out_dtype:q out_partial:P lse_partial:P "
         "workspace:P workspace_bytes:q flags:q stream:P"))
 paged_prefill = ArgStruct(
     "bpt_paged_prefill", (

@@ -185,8 +185,8 @@ def block_table_of(kv: PagedQuantKV, batch: int | None = None) -> tuple[torch.Te
 
 
 def paged_read_split(batch: int, heads: int, keys: int, sms: int = 148) -> int:
-    """Keys per CTA of the any-format decode read, whose CTA covers one KV head (eight query heads) of one sequence: about
-    six CTAs per SM at the longest length, at least 128 keys (two groups of 16 for each of its four warps)."""
+    """Keys per part of the any-format decode read's partial outputs, a warp's work for one KV head (eight query heads): about
+    six parts per SM at the longest length, at least 128 keys."""
     split = -(-batch * heads * keys // (6 * sms))
     return max(128, -(-split // 64) * 64)
 
@@ -220,31 +220,31 @@ def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_
         q, lengths = _q_view(q), as_int32(lengths)
         slopes = _row_tensor("alibi_slopes", alibi_slopes, (hq,), torch.float32)
         starts = _row_tensor("key_starts", key_starts, (b,), torch.int32)
-        tokens = table_width * bs if tokens is None else tokens
-        keys = max(tokens, 1) if partials or not window else max(1, min(tokens, window + 15))  # a window starts anywhere
-        if split is None:
-            split = paged_read_split(b, hkv * -(-hq // hkv // 8), keys, _sms(device))
-        if split % 16 or split <= 0:
-            raise ValueError(f"split {split} must be a multiple of 16")
-        n_splits = -(-keys // split)
+        tokens = max(table_width * bs if tokens is None else int(tokens), 1)
         part_out = part_lse = None
-        room = 0
+        n_splits = 1
         if partials:
+            if split is None:
+                split = paged_read_split(b, hkv * -(-hq // hkv // 8), tokens, _sms(device))
+            if split % 16 or split <= 0:
+                raise ValueError(f"split {split} must be a multiple of 16")
+            n_splits = -(-tokens // split)
             part_out = torch.empty((b, hq, n_splits, d), dtype=torch.float32, device=device)
             part_lse = torch.empty((b, hq, n_splits), dtype=torch.float32, device=device)
         else:
+            split = 16
             if out is None:
                 out = torch.empty(shape, dtype=torch.float32, device=device)
             elif out.shape != shape or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{b}, {hq}, {d}] tensor")
-            if n_splits > 1 and workspace is None:
-                workspace = _zeroed_workspace(int(lib().bpt_paged_read_workspace_bytes(b, hq, d, n_splits)), device)
-            room = 0 if workspace is None else workspace.numel() * workspace.element_size()
+            if workspace is None:
+                workspace = _scratch(_read_scratch_bytes(hq, hkv, d, code, device), device)
+        room = 0 if workspace is None else workspace.numel() * workspace.element_size()
         q_stride = q.stride()
         st = _lib.paged_read(
             q.data_ptr(), dtype_code(q.dtype), q_stride[0], q_stride[1], kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks,
             vs, addr(kss), addr(vss), table.data_ptr(), table_stride, table_width, lengths.data_ptr(), addr(starts),
-            addr(slopes), softcap, window, b, hq, hkv, d, bs, nb, split, n_splits, scale, addr(out),
+            addr(slopes), float(softcap), int(window), b, hq, hkv, d, bs, nb, split, n_splits, tokens, float(scale), addr(out),
             0 if out is None else dtype_code(out.dtype), addr(part_out), addr(part_lse), addr(workspace), room, flags,
             stream_of(device))
     check(st, "decode_attention (paged)" if partials else "attend (paged)")
@@ -380,16 +380,24 @@ def attend_workspace(batch: int, q_heads: int, head_dim: int, n_splits: int, dev
     return ws
 
 
-def _zeroed_workspace(need: int, device: torch.device) -> torch.Tensor:
-    """A workspace whose tickets are zero. While a CUDA graph is captured it is the graph's own (zeroed by every replay), so
-    that two graphs never share one; otherwise the device's and stream's cached one (`attend_workspace`)."""
+_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _scratch(need: int, device: torch.device) -> torch.Tensor:
+    """`need` bytes that nothing is kept in from one call to the next. While a CUDA graph is captured they are the graph's own,
+    so that two graphs never share them; otherwise the device's and stream's, grown on demand."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    key = (device.index or 0, stream_of(device))
-    ws = _WORKSPACES.get(key)
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    key = (device.index, stream_of(device))
+    ws = _SCRATCH.get(key)
     if ws is None or ws.numel() < need:
-        ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+        ws = _SCRATCH[key] = torch.empty(need, dtype=torch.uint8, device=device)
     return ws
+
+
+@functools.cache
+def _read_scratch_bytes(hq: int, hkv: int, d: int, code: int, device: torch.device) -> int:
+    return int(lib().bpt_paged_read_workspace_bytes(hq, hkv, d, code))
 
 
 def _any_format(kv, softcap, window, alibi_slopes, key_starts) -> bool:

@@ -114,7 +114,7 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: PagedQ
         st = _lib.rope_kv_append(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(dtype), q_stride[0], q_stride[1], k_stride[0], k_stride[1],
             v_stride[0], v_stride[1], t, hq, hkv, d, 2 * table[1], pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), table[0],
-            interleaved, addr(q_norm), addr(k_norm), eps, q_out.data_ptr(), wb.data_ptr(), wo.data_ptr(),
+            bool(interleaved), addr(q_norm), addr(k_norm), float(eps), q_out.data_ptr(), wb.data_ptr(), wo.data_ptr(),
             kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks, vs, addr(kss), addr(vss), bs, nb,
             FLAG_PDL if pdl else 0, stream_of(device))
     check(st, "rope_kv_append")

@@ -11,7 +11,7 @@ import torch
 
 from bpt_b200 import _lib
 from bpt_b200._lib import FLAG_PDL, addr, as_int32, check, dtype_code, lib, on_device, require_cuda, stream_of
-from bpt_b200.kernels.kv_attention import PagedQuantKV, _row_tensor, _zeroed_workspace, block_table_of, pool_format
+from bpt_b200.kernels.kv_attention import PagedQuantKV, _row_tensor, _scratch, block_table_of, pool_format
 
 
 def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, lengths: torch.Tensor, scale: float, *,
@@ -64,11 +64,11 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
             out = torch.empty(shape, dtype=q.dtype, device=device)
         if workspace is None:
             need = int(lib().bpt_paged_prefill_workspace_bytes(t, b, hq, hkv, d, code, tokens))
-            workspace = _zeroed_workspace(need, device) if need else None
+            workspace = _scratch(need, device) if need else None
         st = _lib.paged_prefill(
             q.data_ptr(), dtype_code(q.dtype), stride[0], stride[1], kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks, vs,
             addr(kss), addr(vss), table.data_ptr(), table_stride, table_width, cu.data_ptr(), lengths.data_ptr(),
-            addr(positions), addr(starts), addr(prefix), addr(slopes), softcap, window, t, b, hq, hkv, d, bs, nb, tokens, scale,
+            addr(positions), addr(starts), addr(prefix), addr(slopes), float(softcap), int(window), t, b, hq, hkv, d, bs, nb, tokens, float(scale),
             out.data_ptr(), addr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
             FLAG_PDL if pdl else 0, stream_of(device))
     check(st, "prefill_attend")

@@ -9,8 +9,8 @@
 // [lo, hi), and a tile of rows visits only the keys between its smallest lo and largest hi.
 //
 // 16-bit pages with heads of 64 or 128 take csrc/paged_prefill_tc.cu. The kernel here serves the other formats and heads of
-// 256. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. A CTA that
-// has few companions takes a part of its keys only; the parts of a tile are joined by the last of its CTAs to finish.
+// 256. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. Where there
+// are few tiles, each takes several CTAs, with a part of its keys each; a second kernel, launched dependently, joins them.
 #include "paged_prefill.cuh"
 
 namespace bpt {
@@ -37,13 +37,16 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   constexpr int RB = S::RB;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_range[2][kWarps];
-  __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int hk = blockIdx.y, sp = blockIdx.z;
   pdl_launch_dependents();
   pdl_wait();
   const TileAt at = find_tile(a, kRows, int(blockIdx.x));
-  if (at.b < 0) return;
+  const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
+  if (at.b < 0) {
+    if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = 0;
+    return;
+  }
   const int b = at.b;
   const int len = sequence_length(a, b, tid == 0 && hk == 0 && sp == 0);
 
@@ -77,6 +80,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   }
   const int base = lo == INT_MAX ? 0 : lo & ~15;
   const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
+  if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = parts;
   if (sp >= max(parts, 1)) return;
   const int from = base + sp * a.split;  // of the part; keys below lo are masked by the rows
   const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
@@ -89,7 +93,8 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   };
   auto flag_of = [&](int st) { return reinterpret_cast<uint32_t*>(smem + st * S::kStage + 2 * kKeys * RB + S::kScaleBytes); };
   // warp w brings keys 16 w .. 16 w + 15 of a step
-  GroupLoader<KIND, D> loader(a.src, b, hk, from + 16 * warp, kKeys, steps, max(from, lo), to, lane);
+  GroupLoader<KIND, D> loader(a.src, hk, kKeys, lane);
+  loader.begin(b, from + 16 * warp, steps, max(from, lo), to);
   auto request = [&](int i, int st) {
     if (i < steps)
       loader.request(i, stage(st) + warp * 16 * RB, stage(st) + (kKeys + warp * 16) * RB, flag_of(st) + warp);
@@ -257,11 +262,11 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
     return;
   }
   // a part: [rows][D] and the rows' log2-sum-exp2 of tile (blockIdx.x, hk), part sp
-  const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
   float* part = a.part_out + (tile * a.n_splits + sp) * (kRows * D);
   float* part_lse = a.part_lse + (tile * a.n_splits + sp) * kRows;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    if (row[i].out < 0) continue;
     const int r = warp * 16 + g + 8 * i;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
@@ -270,14 +275,59 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
     }
     if (t == 0) part_lse[r] = l[i] == 0.f ? -INFINITY : (m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i]);
   }
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) s_last = atomicAdd(&a.tickets[tile], 1u) == unsigned(parts - 1);
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  join_parts<D>(a, at, hk, tile, parts, kRows, warp, kWarps, lane);
-  if (tid == 0) a.tickets[tile] = 0u;
+}
+
+// Joins the parts of a tile into out: a warp per row, D / 32 columns per lane.
+template <int D>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const PrefillArgs a, int rows) {
+  constexpr int V = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = int(blockIdx.y) * 8 + warp;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t tile = blockIdx.x;
+  const int x = int(tile / a.src.Hkv), hk = int(tile - int64_t(x) * a.src.Hkv);
+  const int parts = a.part_count[tile];
+  if (parts <= 1) return;
+  const TileAt at = find_tile(a, rows, x);
+  const int pr = at.row0 + r, t = pr / a.rep;
+  if (t >= at.tokens) return;
+  const float* lse = a.part_lse + tile * a.n_splits * rows + r;
+  const float* outs = a.part_out + (tile * a.n_splits * rows + r) * D + lane;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[int64_t(i) * rows]);
+  top = warp_max(top);
+  const float off = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float f = exp2_approx(lse[int64_t(i) * rows] - off);
+    sum += f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = fmaf(f, outs[int64_t(i) * rows * D + 32 * e], acc[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t dst = (int64_t(at.token0 + t) * a.Hq + hk * a.rep + pr - t * a.rep) * D + lane;
+#pragma unroll
+  for (int e = 0; e < V; ++e) store_16(a.out, a.q_dtype, dst + 32 * e, acc[e] * inv);
+}
+
+int launch_join(const PrefillArgs& a, int64_t tiles, int rows, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles * a.src.Hkv), unsigned((rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = a.D == 64    ? cudaLaunchKernelEx(&cfg, prefill_join_kernel<64>, a, rows)
+                          : a.D == 128 ? cudaLaunchKernelEx(&cfg, prefill_join_kernel<128>, a, rows)
+                                       : cudaLaunchKernelEx(&cfg, prefill_join_kernel<256>, a, rows);
+  if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
+  return BPT_OK;
 }
 
 template <int KIND, int D>
@@ -329,9 +379,7 @@ Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int 
   return p;
 }
 
-constexpr int64_t kTickets = 65536;  // of a workspace that other merging kernels use too
-constexpr int64_t kTicketBytes = kTickets * 4;
-
+int64_t count_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * 4 + 255) / 256 * 256; }
 int64_t lse_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * p.n_splits * p.rows * 4 + 255) / 256 * 256; }
 
 }  // namespace
@@ -343,7 +391,7 @@ extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64
                                                      int64_t tokens) {
   if (T < 1 || B < 1 || Hkv < 1 || Hq < Hkv || tokens < 1) return 0;
   const Plan p = plan_prefill(T, B, Hq, Hkv, D, kind, tokens);
-  return p.n_splits > 1 ? kTicketBytes + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
+  return p.n_splits > 1 ? count_bytes(p, Hkv) + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
 }
 
 extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
@@ -428,7 +476,7 @@ extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
   a.split = int(p.split);
   a.n_splits = int(p.n_splits);
   BPT_REQUIRE(p.tiles < (1ll << 31) && Hkv < 65536 && p.n_splits < 65536, BPT_ERR_INVALID, "%s: too many rows", who);
-  a.tickets = nullptr;
+  a.part_count = nullptr;
   a.part_lse = nullptr;
   a.part_out = nullptr;
   if (p.n_splits > 1) {
@@ -438,16 +486,15 @@ extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
     BPT_REQUIRE(workspace_bytes >= need, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
                 (long long)workspace_bytes, (long long)need);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    a.tickets = reinterpret_cast<unsigned int*>(ws);
-    a.part_lse = reinterpret_cast<float*>(ws + kTicketBytes);
-    a.part_out = reinterpret_cast<float*>(ws + kTicketBytes + lse_bytes(p, Hkv));
+    a.part_count = reinterpret_cast<int*>(ws);
+    a.part_lse = reinterpret_cast<float*>(ws + count_bytes(p, Hkv));
+    a.part_out = reinterpret_cast<float*>(ws + count_bytes(p, Hkv) + lse_bytes(p, Hkv));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.tc) return prefill_tc(a, kind, p.tiles, flags, s);
-  switch (kind) {
-    case BPT_KV_FP8: return prefill_dim<BPT_KV_FP8>(a, D, p.tiles, flags, s);
-    case BPT_KV_INT8: return prefill_dim<BPT_KV_INT8>(a, D, p.tiles, flags, s);
-    case BPT_KV_F16: return prefill_dim<BPT_KV_F16>(a, D, p.tiles, flags, s);
-    default: return prefill_dim<BPT_KV_BF16>(a, D, p.tiles, flags, s);
-  }
+  const int st = p.tc                  ? prefill_tc(a, kind, p.tiles, flags, s)
+                 : kind == BPT_KV_FP8  ? prefill_dim<BPT_KV_FP8>(a, D, p.tiles, flags, s)
+                 : kind == BPT_KV_INT8 ? prefill_dim<BPT_KV_INT8>(a, D, p.tiles, flags, s)
+                 : kind == BPT_KV_F16  ? prefill_dim<BPT_KV_F16>(a, D, p.tiles, flags, s)
+                                       : prefill_dim<BPT_KV_BF16>(a, D, p.tiles, flags, s);
+  return st || p.n_splits == 1 ? st : launch_join(a, p.tiles, p.rows, s);
 }

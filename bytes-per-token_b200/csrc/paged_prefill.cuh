@@ -24,7 +24,7 @@ struct PrefillArgs {
   int T, B, Hq, D, rep;
   int split, n_splits;
   void* out;  // [T, Hq, D] in q's type
-  unsigned int* tickets;
+  int* part_count;  // [tiles, Hkv]: the parts that a tile was cut into (1: it is in out already)
   float* part_out;  // [tiles, Hkv, n_splits, rows, D]
   float* part_lse;  // [tiles, Hkv, n_splits, rows], base 2
 };
@@ -115,38 +115,6 @@ __device__ __forceinline__ float load_16(const void* p, int dtype, int64_t i) {
 __device__ __forceinline__ void store_16(void* p, int dtype, int64_t i, float v) {
   if (dtype == BPT_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-// Joins the `parts` parts of a tile into out: a warp per row, D / 32 columns per lane.
-template <int D>
-__device__ __forceinline__ void join_parts(const PrefillArgs& a, const TileAt& at, int hk, int64_t tile, int parts, int rows,
-                                           int warp, int warps, int lane) {
-  constexpr int V = D / 32;
-  const float* lse = a.part_lse + tile * a.n_splits * rows;
-  const float* outs = a.part_out + tile * a.n_splits * (int64_t(rows) * D);
-  for (int r = warp; r < rows; r += warps) {
-    const int pr = at.row0 + r, t = pr / a.rep;
-    if (t >= at.tokens) break;
-    const int64_t dst = (int64_t(at.token0 + t) * a.Hq + hk * a.rep + pr - t * a.rep) * D;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(lse + int64_t(i) * rows + r));
-    top = warp_max(top);
-    const float off = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float f = exp2_approx(__ldcg(lse + int64_t(i) * rows + r) - off);
-      sum += f;
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        acc[e] = fmaf(f, __ldcg(outs + (int64_t(i) * rows + r) * D + lane + 32 * e), acc[e]);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int e = 0; e < V; ++e) store_16(a.out, a.q_dtype, dst + lane + 32 * e, acc[e] * inv);
-  }
 }
 
 }  // namespace bpt

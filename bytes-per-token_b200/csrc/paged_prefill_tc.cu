@@ -173,10 +173,9 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 // What a softmax warpgroup does for tile i: its queries into shared memory, then every step's maximum, probabilities and
 // sum, and at the end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
 template <int KIND, int D>
-__device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt& at, const RowAt& row, int hk, int sp, int parts,
+__device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& row, int hk, int sp, int parts,
                                              int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
-                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags,
-                                             uint32_t* last_cta) {
+                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags) {
   using S = TcShape<D>;
   const int r = threadIdx.x & 127, warp = r >> 5, lane = threadIdx.x & 31;
   {
@@ -313,13 +312,14 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
 #pragma unroll
       for (int e = 0; e < 32; ++e) o[e] = 0u;
     }
-    if (parts > 1) {
+    if (row.out < 0) {
+    } else if (parts > 1) {
 #pragma unroll
       for (int e = 0; e < 32; e += 4)
         *reinterpret_cast<float4*>(part + c + e) =
             make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv,
                         __uint_as_float(o[e + 3]) * inv);
-    } else if (row.out >= 0) {
+    } else {
       uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row.out + c);
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
@@ -331,16 +331,8 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
       }
     }
   }
-  if (parts <= 1) return;
-  if (ok) a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
-  __threadfence();
-  asm volatile("bar.sync 1, 256;" ::: "memory");
-  if (threadIdx.x == 0) *last_cta = atomicAdd(&a.tickets[tile], 1u) == unsigned(parts - 1);
-  asm volatile("bar.sync 1, 256;" ::: "memory");
-  if (!*last_cta) return;
-  __threadfence();
-  join_parts<D>(a, at, hk, tile, parts, kRows, i * 4 + warp, 8, lane);
-  if (threadIdx.x == 0) a.tickets[tile] = 0u;
+  if (ok && parts > 1 && row.out >= 0)
+    a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
 }
 
 template <int KIND, int D>
@@ -360,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   uint64_t* drained = o_done + 2;    // all products are done
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
   int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
-  uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address; then: is this CTA the last
+  uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
   const int hk = blockIdx.y, sp = blockIdx.z;
 
@@ -383,7 +375,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   pdl_launch_dependents();
   pdl_wait();
   const TileAt at = find_tile(a, kRows, int(blockIdx.x));
-  if (at.b < 0) return;
+  const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
+  if (at.b < 0) {
+    if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = 0;
+    return;
+  }
   const int b = at.b;
   const int len = sequence_length(a, b, tid == 0 && hk == 0 && sp == 0);
   __syncthreads();
@@ -404,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   const int lo = min(range[0], range[1]), hi = max(range[2], range[3]);
   const int base = lo == INT_MAX ? 0 : lo & ~15;
   const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
+  if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = parts;
   if (sp >= max(parts, 1)) return;
   const int from = base + sp * a.split;
   const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
@@ -563,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_rows<KIND, D>(a, at, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
-                          flags, slot + 1);
+    softmax_rows<KIND, D>(a, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
+                          flags);
   }
   __syncwarp();
   tc_fence_before();

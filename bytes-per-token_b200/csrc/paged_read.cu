@@ -4,24 +4,30 @@
 //   s_j = cap tanh(scale q.k_j / cap) - slope |p - j|,  out = sum_j softmax(s)_j v_j  over  max(0, start, p - window + 1) <= j
 //   <= p, p = length - 1; no visible key gives 0.
 //
-// Bound by memory: each visible key and value is read once. A CTA takes a run of keys of one (sequence, KV head, eight of its
-// query heads) with four warps that never wait for one another until the end: each walks every fourth group of 16 keys with
-// its own ring of cp.async stages, its own running maximum and sum. A group's rows arrive whole (D elements of one head);
-// rows outside the visible run are not read, their places hold zeros. The eight query heads fill only half of an MMA's 16
-// rows, so the other half carries what rounding takes off: rows 0-7 hold q (then the probabilities) rounded to the product's
-// 16-bit type, rows 8-15 the rounded-off rest, and both halves' sums are added in fp32. Products are thus good to 16 (bf16)
-// or 22 bits at no cost. The warps join in shared memory; where a sequence takes several CTAs, each writes its part and the
-// last to finish (a ticket) joins them.
+// Bound by memory: each visible key and value is read once. Work is cut into equal shares, one per warp of a full GPU (8 warps
+// per SM): a warp takes a contiguous range of groups of 16 keys, of one KV head (and eight of its query heads), across the
+// sequences of the batch, so that ragged lengths leave no SM idle; the warps of a CTA hold the heads of one range, whose rows
+// lie next to each other in the pages. A warp never waits for another: it has its own ring of cp.async stages, running on
+// into its next sequence, and its own running maximum and sum. A group's rows arrive whole (D elements of one head); rows
+// outside the visible run are not read, their places hold zeros.
+//
+// The eight query heads fill only half of an MMA's 16 rows, so the other half carries what rounding takes off: rows 0-7 hold q
+// (then the probabilities) rounded to the product's 16-bit type, rows 8-15 the rounded-off rest, and both halves' sums
+// are added in fp32. Products are thus good to 16 (bf16) or 22 bits at no cost.
+//
+// A sequence inside one range goes straight to out. One that crosses ranges leaves a part per range, and a second kernel,
+// launched dependently, joins them: a CTA per range, whose sequence starts there.
+#include <algorithm>
+
 #include "paged_read.cuh"
 
 namespace bpt {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int64_t kTickets = 65536;
-constexpr int64_t kTicketBytes = kTickets * 4;
+constexpr int kWarps = 4;          // per CTA, at most
+constexpr int kStartCost = 4;      // what a sequence's start costs a range, in groups of 16 keys
+constexpr int kLeastShare = 4;     // groups; a smaller share would be all start and join
 
 struct ReadArgs {
   PagedSource src;
@@ -33,14 +39,19 @@ struct ReadArgs {
   const float* slopes;        // [Hq] or null
   float softcap, sm_scale;
   int window;
-  int B, Hq, rep, tiles;  // tiles: groups of 8 query heads per KV head
-  int split, n_splits;
-  int merge;  // 1: parts start at the first visible key's group and are joined into out; 0: parts start at key 0
+  int B, Hq, rep, tiles, heads;  // tiles: groups of 8 query heads per KV head; heads = Hkv * tiles
+  int ranges;
   void* out;
   int out_dtype;
-  float* part_out;  // [B, Hq, n_splits, D]
-  float* part_lse;  // [B, Hq, n_splits], natural logarithm
-  unsigned int* tickets;
+  // merged: parts[ranges][heads][2] (0: of the sequence that a range continues, 1: of the one it leaves unfinished), each
+  // o [8][D] and base-2 log-sum-exps [8]; meta[ranges][heads]: the unfinished sequence and its last range (sequence -1: none)
+  float* ws_out;
+  float* ws_lse;
+  int2* ws_meta;
+  // partials: out [B, Hq, n_splits, D], lse [B, Hq, n_splits] (natural logarithm) of `split` keys each
+  float* part_out;
+  float* part_lse;
+  int split, n_splits;
 };
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
@@ -61,64 +72,177 @@ struct ReadShape {
   static constexpr int kStage = 2 * 16 * RB + kScaleBytes + 16;  // keys, values, scales, the bad-block flag
   // Stages per warp: what keeps the memory busy. 16-bit heads of 128: 3 stages x 8 KB x 4 warps = 96 KB, two CTAs per SM.
   static constexpr int kStages = RB >= 512 ? 3 : RB == 256 ? 3 : 4;
-  static constexpr int kRing = kStages * kStage;
-  static constexpr int kJoin = 8 * D * 4 + 8 * 8;  // a warp's part: o [8][D], m and l [8]
-  static constexpr int kPerWarp = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kSmem = kWarps * kPerWarp;
+  static constexpr int kPerWarp = kStages * kStage;
+  static constexpr int kSmem = kWarps * kPerWarp;  // two CTAs per SM, one at 16-bit heads of 256
+  static constexpr int kWarpsPerSm = RB >= 512 ? 4 : 8;  // the warps that share the work
 };
 
-template <int KIND, int D>
-__global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) {
+// The visible keys of a sequence, cut to the pages that its table has.
+struct Visible {
+  int pos, lo, hi, base, groups;  // base: lo rounded down to a group; groups of 16 keys from there to hi
+};
+__device__ __forceinline__ Visible visible_keys(const ReadArgs& a, int b, bool tells = false) {
+  Visible v;
+  const int room = int(min(int64_t(a.src.bt_width) << a.src.bs_log2, int64_t(1) << 30));
+  const int whole = a.lengths[b], len = min(whole, room);
+  if (tells && whole > room) record_error(kDevErrBlockIndex);  // more tokens than the table has pages for
+  v.pos = len - 1;
+  v.lo = a.key_starts ? max(a.key_starts[b], 0) : 0;
+  if (a.window > 0) v.lo = max(v.lo, v.pos - a.window + 1);
+  v.hi = max(len, 0);
+  v.base = v.lo & ~15;
+  v.groups = v.hi > v.lo ? (v.hi - v.base + 15) >> 4 : 0;
+  return v;
+}
+
+// A warp's walk over the sequences of its range [begin, end) of costs: sequence b starts at cost `at`, its groups at
+// at + kStartCost.
+struct Walk {
+  int b;
+  int64_t at;
+  Visible v;
+  int g0, g1;  // its groups in the range
+  __device__ __forceinline__ void enter(const ReadArgs& a, int64_t begin, int64_t end) {
+    v = visible_keys(a, b);
+    const int64_t start = at + kStartCost;
+    g0 = int(min(max(begin - start, int64_t(0)), int64_t(v.groups)));
+    g1 = int(min(max(end - start, int64_t(0)), int64_t(v.groups)));
+  }
+  __device__ __forceinline__ void leave() {
+    at += kStartCost + v.groups;
+    ++b;
+  }
+};
+
+template <int KIND, int D, bool MERGE>
+__global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs a) {
   using S = ReadShape<KIND, D>;
   constexpr int RB = S::RB, NST = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int s_last;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.z, hk = int(blockIdx.y) / a.tiles, tile = int(blockIdx.y) - hk * a.tiles, sp = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
   pdl_wait();
-  const int room = int(min(int64_t(a.src.bt_width) << a.src.bs_log2, int64_t(1) << 30));
-  int len = a.lengths[b];
-  if (len > room) {  // more tokens than the table has pages for
-    if (tid == 0) record_error(kDevErrBlockIndex);
-    len = room;
-  }
-  const int pos = len - 1;
-  int lo = a.key_starts ? max(a.key_starts[b], 0) : 0;
-  if (a.window > 0) lo = max(lo, pos - a.window + 1);
-  const int hi = max(len, 0);
-  const int base = a.merge ? lo & ~15 : 0;
-  const int parts = hi > lo ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
-  const int h0 = hk * a.rep + tile * 8;        // this CTA's first query head
+  const int64_t id = int64_t(blockIdx.x) * (blockDim.x >> 5) + warp;
+  const int64_t unit = id / a.heads;
+  const int ht = int(id - unit * a.heads), hk = ht / a.tiles, tile = ht - hk * a.tiles;
+  if (unit >= (MERGE ? int64_t(a.ranges) : int64_t(a.B) * a.n_splits)) return;
+  const int h0 = hk * a.rep + tile * 8;        // this warp's first query head
   const int heads = min(8, a.rep - tile * 8);  // and how many
-  if (a.merge && sp >= max(parts, 1)) return;
-  const int64_t from64 = int64_t(base) + int64_t(sp) * a.split;
-  const int from = max(lo, int(min(from64, int64_t(hi))));
-  const int to = sp == a.n_splits - 1 ? hi : int(min(int64_t(hi), from64 + a.split));
-  const int first = from & ~15;
-  const int groups = to > from ? (to - first + 15) / 16 : 0;
-  const int mine = groups > warp ? (groups - warp + kWarps - 1) / kWarps : 0;  // this warp's groups: warp, warp + 4, ...
+
+  Walk use;  // the sequence whose groups are multiplied
+  int64_t begin = 0, end = 0, share = 1;
+  const int range = int(unit);
+  int sp = 0;
+  if constexpr (MERGE) {
+    int64_t total = 0;
+    int mine = 0;  // of the first 32 sequences
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int groups = b0 + lane < a.B ? kStartCost + visible_keys(a, b0 + lane, id == 0).groups : 0;
+      if (b0 == 0) mine = groups;
+      total += groups;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    share = max((total + a.ranges - 1) / a.ranges, int64_t(kStartCost + kLeastShare));
+    begin = range * share;
+    end = min(begin + share, total);
+    if (a.ranges > 1 && lane == 0) a.ws_meta[id] = make_int2(-1, 0);
+    if (begin >= total) return;
+    int64_t before = 0;  // the sequence that holds cost `begin`
+    for (int b0 = 0;; b0 += 32) {
+      int upto = b0 == 0 ? mine : b0 + lane < a.B ? kStartCost + visible_keys(a, b0 + lane).groups : 0;
+      const int own = upto;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > begin);
+      if (hit) {
+        const int w = __ffs(hit) - 1;
+        use.b = b0 + w;
+        use.at = before + __shfl_sync(0xffffffffu, upto - own, w);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    use.enter(a, begin, end);
+  } else {
+    use.b = int(unit / a.n_splits);
+    use.at = 0;
+    sp = int(unit - int64_t(use.b) * a.n_splits);
+    use.v = visible_keys(a, use.b, lane == 0 && sp == 0 && ht == 0);
+    const int64_t from = int64_t(sp) * a.split, to = sp == a.n_splits - 1 ? int64_t(use.v.hi) : from + a.split;
+    use.v.lo = int(max(int64_t(use.v.lo), min(from, int64_t(use.v.hi))));
+    use.v.hi = int(min(int64_t(use.v.hi), to));
+    use.v.base = use.v.lo & ~15;
+    use.v.groups = use.v.hi > use.v.lo ? (use.v.hi - use.v.base + 15) >> 4 : 0;
+    use.g0 = 0;
+    use.g1 = use.v.groups;
+  }
 
   uint8_t* ring = smem + warp * S::kPerWarp;
   const uint32_t ring_u = smem_u32(ring);
   auto scales_of = [&](int st) { return reinterpret_cast<uint16_t*>(ring + st * S::kStage + 32 * RB); };
   auto flag_of = [&](int st) { return reinterpret_cast<uint32_t*>(ring + st * S::kStage + 32 * RB + S::kScaleBytes); };
-  GroupLoader<KIND, D> loader(a.src, b, hk, first + 16 * warp, 16 * kWarps, mine, from, to, lane);
-  auto request = [&](int i, int st) {
-    if (i < mine) loader.request(i, ring_u + st * S::kStage, ring_u + st * S::kStage + 16 * RB, flag_of(st));
+  // The loader runs NST - 1 groups ahead of the products, into the sequences that follow.
+  GroupLoader<KIND, D> loader(a.src, hk, 16, lane);
+  Walk fetch = use;
+  int fetched = 0;        // groups of `fetch` requested so far
+  bool placed = true;     // int8: the scales requested last are in shared memory
+  auto open = [&]() {     // begins the next sequence that has groups in the range
+    for (;;) {
+      if (fetch.g1 > fetch.g0) {
+        loader.begin(fetch.b, fetch.v.base + 16 * fetch.g0, fetch.g1 - fetch.g0, fetch.v.lo, fetch.v.hi);
+        fetched = 0;
+        return true;
+      }
+      if (!MERGE) return false;
+      fetch.leave();
+      if (fetch.b >= a.B || fetch.at >= end) return false;
+      fetch.enter(a, begin, end);
+    }
+  };
+  bool more = open();
+  auto request = [&](int st) {
+    if (more) {
+      loader.request(fetched, ring_u + st * S::kStage, ring_u + st * S::kStage + 16 * RB, flag_of(st));
+      placed = false;
+      if (++fetched == loader.count) {
+        fetch.g1 = fetch.g0;  // done with it
+        more = open();
+      }
+    }
     cp_async_commit();
+  };
+  auto place = [&](int st) {
+    if (KIND == BPT_KV_INT8 && !placed) {
+      loader.place(scales_of(st));
+      placed = true;
+    }
   };
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i) {
-    request(i, i);
-    if (i < NST - 2) loader.place(scales_of(i));
+    request(i);
+    if (i < NST - 2) place(i);
   }
+  const bool cap = a.softcap > 0.f;
+  const float cap_out = a.softcap * kLog2e;
+  const float slope = a.slopes && g < heads ? a.slopes[h0 + g] * kLog2e : 0.f;
+  int st = 0, st_in = NST - 1;
 
+  for (;;) {  // the range's sequences
+    if (MERGE && use.g1 == use.g0 && use.v.groups == 0 && use.at >= begin && lane < D / 8) {  // nothing visible: zeros
+      for (int r = 0; r < heads; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_any(a.out, a.out_dtype, (int64_t(use.b) * a.Hq + h0 + r) * D + lane * 8 + i, 0.f);
+    }
+    if (!MERGE || use.g1 > use.g0) {
   // q: the A fragments of head h0 + g, rounded in rows 0-7 and what rounding took off in rows 8-15
   uint32_t qf[D / 16][4];
   float q_unit = 1.f;
   {
-    const int64_t at = int64_t(b) * a.q_sb + int64_t(h0 + g) * a.q_sh;
+    const int64_t at = int64_t(use.b) * a.q_sb + int64_t(h0 + g) * a.q_sh;
     float amax = 0.f;
     if constexpr (KIND != BPT_KV_BF16) {  // f16 products: q scaled by a power of two into [-1, 1]
       if (g < heads)
@@ -148,10 +272,7 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
     }
   }
   const float raw = a.sm_scale * q_unit * a.src.k_scale;  // a product as a score
-  const bool cap = a.softcap > 0.f;
   const float mul = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
-  const float cap_out = a.softcap * kLog2e;
-  const float slope = a.slopes && g < heads ? a.slopes[h0 + g] * kLog2e : 0.f;
 
   float m = -INFINITY, l = 0.f;
   float o[D / 8][4];
@@ -160,13 +281,13 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
 
-  int st = 0, st_in = NST - 1;
-  for (int i = 0; i < mine; ++i) {
+  const int from = use.v.lo, to = use.v.hi, pos = use.v.pos;
+  for (int i = use.g0; i < use.g1; ++i) {
     cp_async_wait<NST - 2>();
-    if (i + NST - 2 < mine) loader.place(scales_of(st_in == 0 ? NST - 1 : st_in - 1));  // the group requested last
+    place(st_in == 0 ? NST - 1 : st_in - 1);
     __syncwarp();  // every lane's copies of this group have landed; everyone is done with the stage refilled next
-    request(i + NST - 1, st_in);
-    const int key0 = first + 16 * (warp + kWarps * i);
+    request(st_in);
+    const int key0 = use.v.base + 16 * i;
     const uint32_t tile_u = ring_u + st * S::kStage;
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
     scores16<KIND, D>(tile_u, lane, [&](int j) { return MmaRows{{qf[j][0], qf[j][1], qf[j][2], qf[j][3]}}; }, s0, s1);
@@ -222,122 +343,179 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) 
     st = st + 1 == NST ? 0 : st + 1;
     st_in = st_in + 1 == NST ? 0 : st_in + 1;
   }
-  cp_async_wait<0>();
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
-  __syncwarp();
-
-  // the four warps' parts, joined: o [8][D] and (m, l) [8] of each in its own ring's place
-  float* my = reinterpret_cast<float*>(ring);
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) my[g * D + v_dim<KIND, D>(n, t, e)] = o[n][e] + o[n][2 + e];
-  if (t == 0) {
-    my[8 * D + g] = m;
-    my[8 * D + 8 + g] = l;
+  const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
+  const float lse = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+  // where the rows go: straight to out, or to a part
+  const int64_t row = int64_t(use.b) * a.Hq + h0 + g;
+  float* dst = nullptr;
+  if constexpr (MERGE) {
+    const bool starts = use.g0 == 0, ends = use.g1 == use.v.groups;
+    if (!(starts && ends)) {
+      const int64_t part = id * 2 + (starts ? 1 : 0);
+      dst = a.ws_out + (part * 8 + g) * D;
+      if (t == 0) a.ws_lse[part * 8 + g] = lse;
+      if (starts && lane == 0)
+        a.ws_meta[id] = make_int2(use.b, int((use.at + kStartCost + use.v.groups - 1) / share));
+    }
+  } else if (g < heads) {
+    dst = a.part_out + (row * a.n_splits + sp) * D;
+    if (t == 0) a.part_lse[row * a.n_splits + sp] = lse / kLog2e;
   }
-  __syncthreads();
-  const bool direct = a.merge && parts <= 1;
-  constexpr int V = D / 32;  // a warp writes rows warp and warp + 4, V columns (32 apart) per lane
-  for (int r = warp; r < heads; r += kWarps) {
-    float ms[kWarps], top = -INFINITY, sum = 0.f, acc[V];
+  if (g < heads) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      ms[w] = reinterpret_cast<const float*>(smem + w * S::kPerWarp)[8 * D + r];
-      top = fmaxf(top, ms[w]);
-    }
-    const float off = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float* part = reinterpret_cast<const float*>(smem + w * S::kPerWarp);
-      const float f = exp2_approx(ms[w] - off);
-      sum = fmaf(f, part[8 * D + 8 + r], sum);
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(f, part[r * D + lane + 32 * i], acc[i]);
-    }
-    const float inv = sum == 0.f ? 0.f : a.src.v_scale / sum;
-    const int64_t row = int64_t(b) * a.Hq + h0 + r;
-    if (direct) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) store_any(a.out, a.out_dtype, row * D + lane + 32 * i, acc[i] * inv);
-    } else {
-      float* dst = a.part_out + (row * a.n_splits + sp) * D;
-#pragma unroll
-      for (int i = 0; i < V; ++i) dst[lane + 32 * i] = acc[i] * inv;
-      if (lane == 0) a.part_lse[row * a.n_splits + sp] = sum == 0.f ? -INFINITY : (off + log2f(sum)) / kLog2e;
+    for (int n = 0; n < D / 8; ++n) {
+      const float x = (o[n][0] + o[n][2]) * inv, y = (o[n][1] + o[n][3]) * inv;
+      const int dx = v_dim<KIND, D>(n, t, 0), dy = v_dim<KIND, D>(n, t, 1);
+      if (dst) {
+        if constexpr (kIs16<KIND>) {
+          *reinterpret_cast<float2*>(dst + dx) = make_float2(x, y);
+        } else {
+          dst[dx] = x;
+          dst[dy] = y;
+        }
+      } else {
+        store_any(a.out, a.out_dtype, row * D + dx, x);
+        store_any(a.out, a.out_dtype, row * D + dy, y);
+      }
     }
   }
-  if (!a.merge || direct) return;
-
-  // the last CTA of this (sequence, heads) to finish joins the parts
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    const unsigned int ticket = atomicAdd(&a.tickets[(int64_t(b) * a.src.Hkv + hk) * a.tiles + tile], 1u);
-    s_last = ticket == unsigned(parts - 1);
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  for (int r = warp; r < heads; r += kWarps) {
-    const int64_t row = int64_t(b) * a.Hq + h0 + r;
-    const float* lse = a.part_lse + row * a.n_splits;
-    const float* outs = a.part_out + row * a.n_splits * D;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(lse + i));
-    top = warp_max(top);
-    const float off = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float f = exp2_approx((__ldcg(lse + i) - off) * kLog2e);
-      sum += f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = fmaf(f, __ldcg(outs + int64_t(i) * D + lane + 32 * e), acc[e]);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int e = 0; e < V; ++e) store_any(a.out, a.out_dtype, row * D + lane + 32 * e, acc[e] * inv);
+    if (!MERGE) break;
+    use.leave();
+    if (use.b >= a.B || use.at >= end) break;
+    use.enter(a, begin, end);
   }
-  if (tid == 0) a.tickets[(int64_t(b) * a.src.Hkv + hk) * a.tiles + tile] = 0u;
+  cp_async_wait<0>();
 }
 
-template <int KIND, int D>
-int launch_read(const ReadArgs& a, int flags, cudaStream_t stream) {
-  using S = ReadShape<KIND, D>;
-  static std::atomic<uint64_t> ready{0};
-  const int st = set_max_smem_once(reinterpret_cast<const void*>(paged_read_kernel<KIND, D>), S::kSmem, ready);
-  if (st) return st;
+// Joins the parts of the sequence that range x of a head leaves unfinished. Eight warps: as many per row as fit.
+template <int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const ReadArgs a) {
+  __shared__ float s_sum[8], s_top[8];
+  __shared__ float s_acc[8][D];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t id = blockIdx.x;
+  const int2 meta = a.ws_meta[id];
+  if (meta.x < 0) return;
+  const int range = int(id / a.heads), ht = int(id - int64_t(range) * a.heads), hk = ht / a.tiles, tile = ht - hk * a.tiles;
+  const int h0 = hk * a.rep + tile * 8, heads = min(8, a.rep - tile * 8), rows = gridDim.y == 1 ? heads : 1;
+  if (int(blockIdx.y) >= heads) return;
+  const int per_row = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = warp / per_row, first = warp % per_row;
+  const int row = rows == 1 ? int(blockIdx.y) : r;
+  const int parts = meta.y - range + 1;
+  constexpr int V = D / 32;
+  float top = -INFINITY, sum = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  auto part_at = [&](int i) { return ((int64_t(range + i) * a.heads + ht) * 2 + (i == 0 ? 1 : 0)) * 8 + row; };
+  if (r < rows) {
+    for (int i = first + per_row * lane; i < parts; i += per_row * 32) top = fmaxf(top, a.ws_lse[part_at(i)]);
+    top = warp_max(top);
+    const float off = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+    for (int i = first; i < parts; i += per_row) {
+      const int64_t at = part_at(i);
+      const float f = exp2_approx(a.ws_lse[at] - off);
+      sum += f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(f, a.ws_out[at * D + lane + 32 * e], acc[e]);
+    }
+  }
+  if (lane == 0) {
+    s_top[warp] = top;
+    s_sum[warp] = sum;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) s_acc[warp][lane + 32 * e] = acc[e];
+  __syncthreads();
+  if (r >= rows || first != 0) return;
+  float all = top;
+  for (int w = 1; w < per_row; ++w) all = fmaxf(all, s_top[warp + w]);
+  const float off = all == -INFINITY ? 0.f : all;
+  float total = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  for (int w = 0; w < per_row; ++w) {
+    const float f = exp2_approx(s_top[warp + w] - off);
+    total = fmaf(f, s_sum[warp + w], total);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = fmaf(f, s_acc[warp + w][lane + 32 * e], acc[e]);
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    store_any(a.out, a.out_dtype, (int64_t(meta.x) * a.Hq + h0 + row) * D + lane + 32 * e, acc[e] * inv);
+}
+
+int launch(const void* kernel, dim3 grid, int threads, int smem, bool dependent, const ReadArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.n_splits), unsigned(a.src.Hkv * a.tiles), unsigned(a.B));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_read_kernel<KIND, D>, a);
+  cfg.numAttrs = dependent ? 1 : 0;
+  ReadArgs copy = a;
+  void* args[] = {&copy};
+  const cudaError_t err = cudaLaunchKernelExC(&cfg, kernel, args);
   if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged read launch: %s", cudaGetErrorString(err));
   return BPT_OK;
 }
 
-template <int KIND>
-int read_dim(const ReadArgs& a, int64_t D, int flags, cudaStream_t stream) {
-  if (D == 64) return launch_read<KIND, 64>(a, flags, stream);
-  if (D == 128) return launch_read<KIND, 128>(a, flags, stream);
-  return launch_read<KIND, 256>(a, flags, stream);
+// The most ranges of a merged read: as many as give every warp of a full GPU one head of one range.
+int64_t read_ranges(int64_t heads, int64_t D, int kind) {
+  const bool wide = D == 256 && (kind == BPT_KV_F16 || kind == BPT_KV_BF16);
+  return std::max<int64_t>(int64_t(num_sms()) * (wide ? ReadShape<BPT_KV_F16, 256>::kWarpsPerSm : 8) / heads, 1);
 }
 
-int64_t read_workspace(int64_t B, int64_t Hq, int64_t D, int64_t n_splits) {
-  const int64_t lse = ((B * Hq * n_splits * 4 + 255) / 256) * 256;
-  return kTicketBytes + lse + B * Hq * n_splits * D * 4;
+template <int KIND, int D, bool MERGE>
+int launch_read(const ReadArgs& a, int flags, cudaStream_t stream) {
+  using S = ReadShape<KIND, D>;
+  const void* kernel = reinterpret_cast<const void*>(paged_read_kernel<KIND, D, MERGE>);
+  static std::atomic<uint64_t> ready{0};
+  int st = set_max_smem_once(kernel, S::kSmem, ready);
+  if (st) return st;
+  const int64_t warps = (MERGE ? int64_t(a.ranges) : int64_t(a.B) * a.n_splits) * a.heads;
+  // few warps are spread over the SMs
+  const int per_cta = int(std::min<int64_t>(kWarps, (warps + num_sms() - 1) / num_sms()));
+  const int64_t ctas = (warps + per_cta - 1) / per_cta;
+  BPT_REQUIRE(ctas < (1ll << 31), BPT_ERR_INVALID, "paged read: too many parts");
+  st = launch(kernel, dim3(unsigned(ctas)), 32 * per_cta, per_cta * S::kPerWarp, (flags & BPT_FLAG_PDL) != 0, a, stream);
+  if (st || !MERGE || a.ranges == 1) return st;
+  // many ranges per sequence: a CTA per row, so that no warp reads a long row of parts
+  const unsigned rows = a.ranges >= 16 * int64_t(a.B) ? unsigned(std::min(a.rep, 8)) : 1u;
+  return launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(unsigned(warps), rows), 256, 0, true, a, stream);
+}
+
+template <int KIND>
+int read_dim(const ReadArgs& a, int64_t D, bool merge, int flags, cudaStream_t stream) {
+  if (merge) {
+    if (D == 64) return launch_read<KIND, 64, true>(a, flags, stream);
+    if (D == 128) return launch_read<KIND, 128, true>(a, flags, stream);
+    return launch_read<KIND, 256, true>(a, flags, stream);
+  }
+  if (D == 64) return launch_read<KIND, 64, false>(a, flags, stream);
+  if (D == 128) return launch_read<KIND, 128, false>(a, flags, stream);
+  return launch_read<KIND, 256, false>(a, flags, stream);
+}
+
+struct ReadWorkspace {
+  int64_t meta, lse, total;  // offsets of the second and third part, the size
+};
+ReadWorkspace read_workspace(int64_t Hq, int64_t Hkv, int64_t D, int kind) {
+  const int64_t heads = Hkv * ((Hq / Hkv + 7) / 8), warps = read_ranges(heads, D, kind) * heads;
+  ReadWorkspace w;
+  w.meta = (warps * 8 + 255) / 256 * 256;
+  w.lse = w.meta + (warps * 2 * 8 * 4 + 255) / 256 * 256;
+  w.total = w.lse + warps * 2 * 8 * D * 4;
+  return w;
 }
 
 }  // namespace
@@ -379,8 +557,8 @@ int paged_source(PagedSource& s, const char* who, const void* k_pool, const void
 
 using namespace bpt;
 
-extern "C" int64_t bpt_paged_read_workspace_bytes(int64_t B, int64_t Hq, int64_t D, int64_t n_splits) {
-  return n_splits > 1 ? read_workspace(B, Hq, D, n_splits) : 0;
+extern "C" int64_t bpt_paged_read_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int kind) {
+  return Hkv >= 1 && Hq >= Hkv && D >= 1 ? read_workspace(Hq, Hkv, D, kind).total : 0;
 }
 
 extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
@@ -412,6 +590,7 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   const int64_t num_blocks = args->num_blocks;
   const int64_t split = args->split;
   const int64_t n_splits = args->n_splits;
+  const int64_t tokens = args->tokens;
   const float sm_scale = float(args->sm_scale);
   void* const out = args->out;
   const int out_dtype = int(args->out_dtype);
@@ -422,7 +601,7 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   const int flags = int(args->flags);
   void* const stream = args->stream;
   const char* who = "paged read";
-  BPT_REQUIRE(B >= 0 && B < 65536, BPT_ERR_INVALID, "%s: B=%lld", who, (long long)B);
+  BPT_REQUIRE(B >= 0 && B < (1 << 24), BPT_ERR_INVALID, "%s: B=%lld", who, (long long)B);
   if (B == 0) return BPT_OK;
   BPT_REQUIRE(q && lengths, BPT_ERR_INVALID, "%s: null pointer argument", who);
   BPT_REQUIRE(q_dtype == BPT_DTYPE_F32 || q_dtype == BPT_DTYPE_F16 || q_dtype == BPT_DTYPE_BF16, BPT_ERR_INVALID,
@@ -433,11 +612,9 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   if (bad) return bad;
   BPT_REQUIRE(Hq >= 1 && Hq % Hkv == 0 && Hq < (1 << 15), BPT_ERR_INVALID, "%s: Hq=%lld is not a multiple of Hkv=%lld", who,
               (long long)Hq, (long long)Hkv);
-  BPT_REQUIRE(split >= 16 && split % 16 == 0 && split < (1ll << 30) && n_splits >= 1 && n_splits < (1 << 20), BPT_ERR_INVALID,
-              "%s: split=%lld (a multiple of 16), n_splits=%lld", who, (long long)split, (long long)n_splits);
   BPT_REQUIRE(window >= 0, BPT_ERR_INVALID, "%s: window=%lld", who, (long long)window);
   BPT_REQUIRE(softcap >= 0.f && softcap < INFINITY, BPT_ERR_INVALID, "%s: softcap must be finite and not negative", who);
-  a.merge = out_partial == nullptr;
+  const bool merge = out_partial == nullptr;
   a.q = q;
   a.q_dtype = q_dtype;
   a.q_sb = q_stride_b;
@@ -452,39 +629,46 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   a.Hq = int(Hq);
   a.rep = int(Hq / Hkv);
   a.tiles = (a.rep + 7) / 8;
-  a.split = int(split);
-  a.n_splits = int(n_splits);
+  BPT_REQUIRE(Hkv * a.tiles < 65536, BPT_ERR_INVALID, "%s: too many heads", who);
+  a.heads = int(Hkv * a.tiles);
   a.out = out;
   a.out_dtype = out_dtype;
   a.part_out = out_partial;
   a.part_lse = lse_partial;
-  a.tickets = nullptr;
-  BPT_REQUIRE(Hkv * a.tiles < 65536, BPT_ERR_INVALID, "%s: too many heads", who);
-  if (a.merge) {
+  a.split = a.n_splits = a.ranges = 1;
+  a.ws_out = a.ws_lse = nullptr;
+  a.ws_meta = nullptr;
+  if (merge) {
     BPT_REQUIRE(out, BPT_ERR_INVALID, "%s: null output", who);
     BPT_REQUIRE(out_dtype == BPT_DTYPE_F32 || out_dtype == BPT_DTYPE_F16 || out_dtype == BPT_DTYPE_BF16, BPT_ERR_INVALID,
                 "%s: out dtype %d", who, out_dtype);
-    if (n_splits > 1) {
-      BPT_REQUIRE(B * Hkv * a.tiles <= kTickets, BPT_ERR_UNSUPPORTED, "%s: %lld sequence heads to join (at most %lld)", who,
-                  (long long)(B * Hkv * a.tiles), (long long)kTickets);
+    BPT_REQUIRE(tokens >= 1, BPT_ERR_INVALID, "%s: tokens=%lld", who, (long long)tokens);
+    const int64_t keys = a.window > 0 ? std::min<int64_t>(tokens, int64_t(a.window) + 15) : tokens;
+    const int64_t cost = (std::min<int64_t>(keys, 1 << 30) + 15) / 16 + kStartCost;
+    a.ranges = int(std::min(read_ranges(a.heads, D, kind), std::max<int64_t>(B * cost / (kStartCost + kLeastShare), 1)));
+    if (a.ranges > 1) {
+      const ReadWorkspace w = read_workspace(Hq, Hkv, D, kind);
       BPT_REQUIRE(workspace, BPT_ERR_WORKSPACE, "%s: no workspace", who);
       BPT_REQUIRE(aligned16(workspace), BPT_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", who);
-      const int64_t need = read_workspace(B, Hq, D, n_splits);
-      BPT_REQUIRE(workspace_bytes >= need, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
-                  (long long)workspace_bytes, (long long)need);
+      BPT_REQUIRE(workspace_bytes >= w.total, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
+                  (long long)workspace_bytes, (long long)w.total);
       uint8_t* ws = static_cast<uint8_t*>(workspace);
-      a.tickets = reinterpret_cast<unsigned int*>(ws);
-      a.part_lse = reinterpret_cast<float*>(ws + kTicketBytes);
-      a.part_out = reinterpret_cast<float*>(ws + kTicketBytes + ((B * Hq * n_splits * 4 + 255) / 256) * 256);
+      a.ws_meta = reinterpret_cast<int2*>(ws);
+      a.ws_lse = reinterpret_cast<float*>(ws + w.meta);
+      a.ws_out = reinterpret_cast<float*>(ws + w.lse);
     }
   } else {
     BPT_REQUIRE(lse_partial, BPT_ERR_INVALID, "%s: null output", who);
+    BPT_REQUIRE(split >= 16 && split % 16 == 0 && split < (1ll << 30) && n_splits >= 1 && n_splits < (1 << 20),
+                BPT_ERR_INVALID, "%s: split=%lld (a multiple of 16), n_splits=%lld", who, (long long)split, (long long)n_splits);
+    a.split = int(split);
+    a.n_splits = int(n_splits);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (kind) {
-    case BPT_KV_FP8: return read_dim<BPT_KV_FP8>(a, D, flags, s);
-    case BPT_KV_INT8: return read_dim<BPT_KV_INT8>(a, D, flags, s);
-    case BPT_KV_F16: return read_dim<BPT_KV_F16>(a, D, flags, s);
-    default: return read_dim<BPT_KV_BF16>(a, D, flags, s);
+    case BPT_KV_FP8: return read_dim<BPT_KV_FP8>(a, D, merge, flags, s);
+    case BPT_KV_INT8: return read_dim<BPT_KV_INT8>(a, D, merge, flags, s);
+    case BPT_KV_F16: return read_dim<BPT_KV_F16>(a, D, merge, flags, s);
+    default: return read_dim<BPT_KV_BF16>(a, D, merge, flags, s);
   }
 }

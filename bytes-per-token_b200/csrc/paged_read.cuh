@@ -228,12 +228,18 @@ struct GroupLoader {
   int held = -1, held2 = -1;
   uint32_t scale_bits = 0;
 
-  __device__ __forceinline__ GroupLoader(const PagedSource& s, int b, int hk_, int first_, int step_, int count_, int from_,
-                                         int to_, int lane_)
-      : src(s), table(s.block_table + int64_t(b) * s.bt_stride), row_bytes(int64_t(s.Hkv) * RB),
-        head_bytes(int64_t(hk_) * RB), first(first_), step(step_), count(count_), from(from_), to(to_), hk(hk_),
-        lane(lane_) {}
+  __device__ __forceinline__ GroupLoader(const PagedSource& s, int hk_, int step_, int lane_)
+      : src(s), table(nullptr), row_bytes(int64_t(s.Hkv) * RB), head_bytes(int64_t(hk_) * RB), first(0), step(step_), count(0),
+        from(0), to(0), hk(hk_), lane(lane_) {}
 
+  // `count` groups of sequence b from key `first_` on.
+  __device__ __forceinline__ void begin(int b, int first_, int count_, int from_, int to_) {
+    table = src.block_table + int64_t(b) * src.bt_stride;
+    first = first_;
+    count = count_;
+    from = from_;
+    to = to_;
+  }
   __device__ __forceinline__ int block_at(int key) const {
     if (key >= to) return -1;
     const int blk = table[key >> src.bs_log2];

@@ -161,14 +161,13 @@ int bpt_paged_attend(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_s
  * softcap 0: no cap; window 0: no window; key_starts (int32 [B]) and alibi_slopes (fp32 [Hq]) may be NULL. No visible key
  * gives 0. block_table int32 [B, bt_width], row stride bt_stride; a length beyond the table's pages is cut to them and
  * recorded (device error 2), keys of a block out of range are left out and recorded.
- * With out_partial NULL: the merged attention out [B, Hq, D] in out_dtype; a sequence takes up to n_splits CTAs of `split`
- * keys per KV head (the last takes the rest, whatever its length), joined by the last to finish. n_splits > 1 needs
- * `workspace`: bpt_paged_read_workspace_bytes(...) bytes, ZEROED before its first use, tickets left at zero by every call;
- * calls that may overlap need workspaces of their own. Otherwise out_partial f32 [B, Hq, n_splits, D] and lse_partial f32
- * [B, Hq, n_splits] receive the parts (keys [i split, (i + 1) split); out 0, lse -inf where none is visible).
+ * With out_partial NULL: the merged attention out [B, Hq, D] in out_dtype. `tokens` bounds the longest length (it sizes the
+ * launch, not the result); `workspace`: bpt_paged_read_workspace_bytes(...) bytes of any content, not shared by calls that
+ * may overlap. Otherwise out_partial f32 [B, Hq, n_splits, D] and lse_partial f32 [B, Hq, n_splits] receive the parts (keys
+ * [i split, (i + 1) split), the last part the rest; out 0, lse -inf where none is visible).
  * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024, split a multiple of 16.
  * Replaces: as bpt_paged_attend, for the reference's unquantized pages too (engine/kv_cache.py:98-169). */
-int64_t bpt_paged_read_workspace_bytes(int64_t B, int64_t Hq, int64_t D, int64_t n_splits);
+int64_t bpt_paged_read_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int kind);
 typedef struct {
   const void *q;
   int64_t q_dtype, q_stride_b, q_stride_h;
@@ -181,7 +180,7 @@ typedef struct {
   const int32_t *lengths, *key_starts;
   const float *alibi_slopes;
   double softcap;
-  int64_t window, B, Hq, Hkv, D, block_size, num_blocks, split, n_splits;
+  int64_t window, B, Hq, Hkv, D, block_size, num_blocks, split, n_splits, tokens;
   double sm_scale;
   void *out;
   int64_t out_dtype;

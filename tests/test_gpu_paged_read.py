@@ -151,7 +151,7 @@ def test_bad_blocks_and_lengths_are_left_out_and_recorded():
 
 @pytest.mark.gpu
 def test_a_wrong_tokens_hint_and_repeated_calls_give_the_same():
-    """`tokens` bounds the launch, not the result; a workspace is clean after every call, whatever its shape."""
+    """`tokens` bounds the launch, not the result; nothing of one call's workspace shows in the next."""
     from bpt_b200.kernels.kv_attention import attend
 
     lengths = [3000, 10, 1500]
@@ -227,7 +227,7 @@ def test_refusals_need_no_gpu():
     def call(**kw):
         a = {"q": 64, "qd": 2, "qb": 512, "qh": 128, "kp": 64, "vp": 64, "kind": 4, "ks": 1.0, "vs": 1.0, "kss": None, "vss": None,
              "bt": 64, "bts": 4, "btw": 4, "len": 64, "starts": None, "slopes": None, "cap": 0.0, "window": 0, "B": 2, "Hq": 4,
-             "Hkv": 2, "D": 128, "bs": 16, "nb": 8, "split": 64, "n": 1, "scale": 1.0, "out": 64, "od": 2, "po": None,
+             "Hkv": 2, "D": 128, "bs": 16, "nb": 8, "split": 64, "n": 1, "tokens": 8, "scale": 1.0, "out": 64, "od": 2, "po": None,
              "pl": None, "ws": None, "wsb": 0, "flags": 0, "stream": None} | kw
         return _lib.paged_read(*(0 if x is None else x for x in a.values()))
 
@@ -236,21 +236,22 @@ def test_refusals_need_no_gpu():
         assert call(**{name: None}) == _lib.ERR_INVALID and b"null" in L.bpt_last_error()
     assert call(D=96) == _lib.ERR_UNSUPPORTED and call(bs=24) == _lib.ERR_UNSUPPORTED and call(bs=4) == _lib.ERR_UNSUPPORTED
     assert call(kind=0) == _lib.ERR_INVALID and call(qd=7) == _lib.ERR_INVALID and call(od=7) == _lib.ERR_INVALID
-    assert call(Hq=3) == _lib.ERR_INVALID and call(split=24) == _lib.ERR_INVALID and call(split=0) == _lib.ERR_INVALID
+    assert call(Hq=3) == _lib.ERR_INVALID and call(tokens=0) == _lib.ERR_INVALID
+    for bad in ({"split": 24}, {"split": 0}, {"n": 0}):
+        assert call(po=64, pl=64, **bad) == _lib.ERR_INVALID and b"split" in L.bpt_last_error()
     assert call(window=-1) == _lib.ERR_INVALID and call(cap=-1.0) == _lib.ERR_INVALID and call(cap=float("nan")) == _lib.ERR_INVALID
     assert call(bts=3) == _lib.ERR_INVALID and call(btw=0) == _lib.ERR_INVALID
-    assert call(n=2) == _lib.ERR_WORKSPACE
-    assert call(n=2, ws=64, wsb=100) == _lib.ERR_WORKSPACE and call(n=2, ws=72, wsb=1 << 30) == _lib.ERR_ALIGNMENT
+    assert call(tokens=4000) == _lib.ERR_WORKSPACE
+    assert call(tokens=4000, ws=64, wsb=100) == _lib.ERR_WORKSPACE and call(tokens=4000, ws=72, wsb=1 << 30) == _lib.ERR_ALIGNMENT
     assert call(po=64) == _lib.ERR_INVALID  # partials without their log-sum-exps
     assert call(kind=1, ks=0.0) == _lib.ERR_INVALID and call(kind=2) == _lib.ERR_INVALID
     assert call(kp=72) == _lib.ERR_ALIGNMENT
-    assert L.bpt_paged_read_workspace_bytes(2, 16, 128, 1) == 0
-    assert L.bpt_paged_read_workspace_bytes(2, 16, 128, 4) >= 2 * 16 * 4 * 129 * 4
+    assert L.bpt_paged_read_workspace_bytes(16, 8, 128, 4) >= 2 * 8 * 8 * 129 * 4
 
 
 @pytest.mark.gpu
 def test_python_refusals():
-    from bpt_b200.kernels.kv_attention import QuantKV, attend
+    from bpt_b200.kernels.kv_attention import QuantKV, attend, decode_attention
 
     kv, _, _, q, _ = case("bf16", [20], 4, 2, 64, 16, q_dtype=torch.bfloat16)
     n, q = torch.tensor([20], dtype=torch.int32).cuda(), q.cuda()
@@ -259,6 +260,8 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             attend(q, kv, n, 1.0, **kw)
 
+    with pytest.raises(ValueError):
+        decode_attention(q, kv, n, 1.0, split=24)
     refused(q=q.cpu())
     refused(q=q[:, :3])
     refused(q=q.double())
@@ -266,7 +269,6 @@ def test_python_refusals():
     refused(n=n.repeat(2))
     refused(window=-1)
     refused(softcap=-2.0)
-    refused(split=24)
     refused(alibi_slopes=torch.ones(3, device="cuda"))
     refused(key_starts=torch.zeros(2, dtype=torch.int32, device="cuda"))
     refused(out=torch.empty(1, 4, 32, device="cuda"))
