@@ -241,6 +241,9 @@ def _paged_read(q, kv, lengths, scale, *, tokens, split, softcap, window, alibi_
                 workspace = _scratch(_read_scratch_bytes(hq, hkv, d, code, device), device)
         room = 0 if workspace is None else workspace.numel() * workspace.element_size()
         q_stride = q.stride()
+        if q_stride[0] % 2 or q_stride[1] % 2 or q.data_ptr() % (2 * q.element_size()):
+            q = q.clone(memory_format=torch.contiguous_format)  # rows that start inside a pair
+            q_stride = q.stride()
         st = _lib.paged_read(
             q.data_ptr(), dtype_code(q.dtype), q_stride[0], q_stride[1], kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), code, ks,
             vs, addr(kss), addr(vss), table.data_ptr(), table_stride, table_width, lengths.data_ptr(), addr(starts),

@@ -9,11 +9,13 @@
 // Four warpgroups: two do the softmax, each of one tile, a thread per row (so neither maximum nor sum crosses threads); one
 // brings pages into a ring of shared-memory stages, K and V of a step in stages of their own, by cp.async (rows of any page
 // size; keys that are not visible become zeros); of the last, one thread issues the matrix products. While the softmax of
-// one tile runs, the tensor cores work on the other tile: P V of its last step, then Q K^T of its next.
+// one tile runs, the tensor cores work on the other tile: P V of its last step (in
+// two halves, the first while the powers of the second are still taken), then Q K^T of its next.
 //
-// The running maximum only moves when a row's true maximum has passed it by 2^8 or more: P then stays below 2^8 (exact in
-// range for both types, and P V is divided by the sum of the same P), and O in tensor memory is rescaled a few times per
-// row instead of every step.
+// A row's m is the true maximum of its first 64 keys and moves only when the sum of 2^(s - m) over 64 keys passes 2^15: until then
+// every P is below 2^15, which both 16-bit types hold, and is divided by the sum of the same powers, so nothing is lost by
+// an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
+// times per row, if at all.
 //
 // Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
 // and the CTA still awaits its copies and products, frees its tensor memory and returns.
@@ -33,14 +35,14 @@ constexpr int kOtherRegs = 56;
 constexpr int kLaunchRegs = 128;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kFlagSteps = 16;     // steps whose bad-block flags are kept (the ring runs at most 5 steps ahead)
-constexpr float kSlack = 8.f;      // how far, in powers of two, a row's maximum may pass the one in use
+constexpr float kMostSum = 32768.f;  // a step's sum of powers beyond which a row's maximum moves
 
 template <int D>
 struct TcShape {
   static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kQ = 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 10;  // an even number: the flags behind them start on 16 bytes
+  static constexpr int kBars = 2 * kStages + 14;  // an even number: the flags behind them start on 16 bytes
   static constexpr int kSmem = 1024 + kQ + kStages * kTileBytes + kBars * 8 + kFlagSteps * 16 + 64;
   static constexpr uint32_t kO = 256;     // columns: S0, S1 at 0, 128; O0, O1 at 256, 256 + D
   static_assert(256 + 2 * D <= 512, "tensor memory");
@@ -78,14 +80,6 @@ __device__ __forceinline__ void tmem_arrived32(uint32_t* v) {
         "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
         "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
       :
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};" ::"r"(addr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
@@ -126,22 +120,32 @@ constexpr uint32_t tc_idesc(int m, int n, bool across) {
   return (1u << 4) | (KIND == BPT_KV_BF16 ? (1u << 7) | (1u << 10) : 0u) | (across ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) |
          (uint32_t(m >> 4) << 24);
 }
+// One thread of a converged warp. The products are issued under it, with everything they take computed by the whole warp: the
+// descriptors then stay in uniform registers, where the instruction wants them (issued by `lane == 0` they are moved
+// there one by one: 100 cycles a product instead of a few).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  const uint32_t mask = 0u;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(mask), "r"(mask), "r"(mask), "r"(mask)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  const uint32_t mask = 0u;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(mask), "r"(mask), "r"(mask), "r"(mask)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 
@@ -201,105 +205,118 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
   const uint32_t s_at = tmem + lanes + i * 128, o_at = tmem + lanes + S::kO + i * D;
 
   float m = -INFINITY;  // the maximum in use
-  float2 l2 = make_float2(0.f, 0.f);
+  float l = 0.f;
   uint32_t n = 0;
   bool ok = true;
   for (int j = first; j < last; ++j, ++n) {
     ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], n & 1u));
     if (!ok) break;
     tc_fence_after();
-    uint32_t v[kKeys];
-#pragma unroll
-    for (int c = 0; c < kKeys; c += 32) tmem_request32(s_at + c, v + c);
-    tmem_wait_load();
-#pragma unroll
-    for (int c = 0; c < kKeys; c += 32) tmem_arrived32(v + c);
     const int key0 = from + j * kKeys;
     const uint4 bad = *reinterpret_cast<const uint4*>(flags + (j & (kFlagSteps - 1)) * 4);
     const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
     const bool masked = any_bad || key0 < all_lo || key0 + kKeys > all_hi;
-    float mul_now = mul;
-    if (shaped) {
-      mul_now = 1.f;
-      if (cap) {
+    // Columns c .. c + 31 of S, as scores but for the factor mul_now.
+    const float mul_now = shaped ? 1.f : mul;
+    auto shape = [&](int c, uint32_t* x) {
+      if (shaped) {
+        if (cap) {
 #pragma unroll
-        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(capped(__uint_as_float(v[c]) * mul, cap_out));
-      } else {
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(capped(__uint_as_float(x[e]) * mul, cap_out));
+        } else {
 #pragma unroll
-        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * mul);
-      }
-      if (sloped) {
-        const float far = float(key0 - row.pos);
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * mul);
+        }
+        if (sloped) {
+          const float far = float(key0 + c - row.pos);
 #pragma unroll
-        for (int c = 0; c < kKeys; ++c) v[c] = __float_as_uint(fmaf(row.slope, fabsf(far + float(c)), __uint_as_float(v[c])));
-      }
-    }
-    if (masked) {
-      const int below = row.lo - key0, above = row.hi - key0;
-#pragma unroll
-      for (int c = 0; c < kKeys; ++c)
-        if (c < below || c >= above) v[c] = 0xFF800000u;
-      if (any_bad) {
-        const uint32_t w[4] = {bad.x, bad.y, bad.z, bad.w};
-#pragma unroll
-        for (int c = 0; c < kKeys; ++c)
-          if (w[c >> 5] >> ((c >> 3) & 3) & 1u) v[c] = 0xFF800000u;
-      }
-    }
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int c = 0; c < kKeys; c += 8)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        top[e] = fmaxf(top[e], fmaxf(__uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e])));
-    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul_now;
-    const bool moves = now > m + kSlack;
-    if (__any_sync(0xffffffffu, moves)) {
-      float shrink = 1.f;
-      if (moves) {
-        shrink = exp2_approx(m - now);
-        m = now;
-        l2.x *= shrink;
-        l2.y *= shrink;
-      }
-      if (n > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (n - 1) & 1u));
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_load32(o_at + c, o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-          tmem_store32(o_at + c, o);
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(row.slope, fabsf(far + float(e)), __uint_as_float(x[e])));
         }
       }
-    }
-    // P enters its product rounded to 16 bits (as any operand of these matrix instructions); the sum that divides it is
-    // taken in fp32, before the rounding.
-    const float off = m == -INFINITY ? 0.f : m;
+      if (masked) {
+        const int below = row.lo - key0 - c, above = row.hi - key0 - c;
+        const uint32_t w = c == 0 ? bad.x : c == 32 ? bad.y : c == 64 ? bad.z : bad.w;
 #pragma unroll
-    for (int c = 0; c < kKeys; c += 32) {
-      uint32_t p[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float2 x = ffma2(make_float2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])),
-                               make_float2(mul_now, mul_now), make_float2(-off, -off));
-        const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-        l2 = fadd2(l2, y);
-        p[e] = pack2<KIND>(y.x, y.y);
+        for (int e = 0; e < 32; ++e)
+          if (e < below || e >= above || (w >> (e >> 3) & 1u)) x[e] = 0xFF800000u;
       }
-      tmem_store16(s_at + (c >> 1), p);
+    };
+    // The step's keys in halves h: P = 2^(s - m), rounded to 16 bits (as any operand of these matrix instructions), and the
+    // fp32 sum of what was rounded. P V of the first half runs while the powers of the second are taken.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t p[32];
+      auto powers = [&](float off) {
+        float2 sum = make_float2(0.f, 0.f);
+        uint32_t x[2][32];
+        tmem_request32(s_at + 64 * h, x[0]);
+        tmem_request32(s_at + 64 * h + 32, x[1]);
+        tmem_wait_load();
+        tmem_arrived32(x[0]);
+        tmem_arrived32(x[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          shape(64 * h + 32 * k, x[k]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 y = ffma2(make_float2(__uint_as_float(x[k][2 * e]), __uint_as_float(x[k][2 * e + 1])),
+                                   make_float2(mul_now, mul_now), make_float2(-off, -off));
+            const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            sum = fadd2(sum, z);
+            p[16 * k + e] = pack2<KIND>(z.x, z.y);
+          }
+        }
+        return sum.x + sum.y;
+      };
+      // a row that has met no key yet meets some in this half: its first maximum
+      const int half0 = key0 + 64 * h;
+      const bool fresh = m == -INFINITY && row.lo < half0 + 64 && row.hi > half0;
+      float sum = 0.f;
+      if (!__all_sync(0xffffffffu, fresh)) sum = powers(m == -INFINITY ? 0.f : m);
+      const bool moves = fresh || !(sum <= kMostSum);
+      if (__any_sync(0xffffffffu, moves)) {  // a first half-step, and a few later ones: the row's maximum moves
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 64 * h; c < 64 * h + 64; c += 32) {
+          uint32_t x[32];
+          tmem_load32(s_at + c, x);
+          shape(c, x);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+        }
+        top *= mul_now;
+        float shrink = 1.f;
+        if (moves && top > m) {
+          shrink = exp2_approx(m - top);
+          m = top;
+          l *= shrink;
+        }
+        if (n > 0 || h > 0) {  // the half-step before this one is in O
+          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * i + (h ^ 1)], (h ? n : n - 1) & 1u));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o_at + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+            tmem_store32(o_at + c, o);
+          }
+        }
+        sum = powers(m == -INFINITY ? 0.f : m);
+      }
+      l += sum;
+      tmem_store32(s_at + 32 * h, p);
+      tmem_wait_store();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
     }
-    tmem_wait_store();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&p_full[i]);
+    if (!ok) break;
   }
-  if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (n - 1) & 1u));
+  if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * i + 1], (n - 1) & 1u));
   tc_fence_after();
-  const float l = l2.x + l2.y;
   const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
   const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
   float* part = parts > 1 ? a.part_out + ((tile * a.n_splits + sp) * kRows + i * kTileRows + r) * D : nullptr;
@@ -347,9 +364,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   uint64_t* empty = full + NS;       // [NS] the products that read it are done
   uint64_t* q_full = empty + NS;     // [2] a tile's queries are in shared memory
   uint64_t* s_full = q_full + 2;     // [2] S is in tensor memory
-  uint64_t* p_full = s_full + 2;     // [2] P is in tensor memory, O rescaled where needed
-  uint64_t* o_done = p_full + 2;     // [2] P V is in O
-  uint64_t* drained = o_done + 2;    // all products are done
+  uint64_t* p_full = s_full + 2;     // [2][2] a half of P is in tensor memory, O rescaled where needed
+  uint64_t* o_done = p_full + 4;     // [2][2] that half's P V is in O
+  uint64_t* drained = o_done + 4;    // all products are done
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
   int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
   uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address
@@ -364,8 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 2);  // the products' completion, and the issuing thread (whose own waits saw the flags)
-      mbar_init(&p_full[i], 4);
-      mbar_init(&o_done[i], 1);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
+      mbar_init(&o_done[2 * i], 1);
+      mbar_init(&o_done[2 * i + 1], 1);
       range[i] = INT_MAX;
       range[2 + i] = 0;
     }
@@ -468,6 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
       const uint32_t dst = smem_u32(ring + in.stage * S::kTileBytes);
       uint32_t bad = 0;
+      // this lane's chunk of the first rows of each group, and its place: rows 32 / CPR further on are constants away
+      const int r0 = lane / CPR, c0 = lane % CPR;
+      const uint32_t dst0 = dst + (c0 >> 3) * (kKeys * 128) + (32 * w + r0) * 128, x0 = uint32_t((c0 & 7) ^ r0);
 #pragma unroll
       for (int grp = 0; grp < 2; ++grp) {
         const int key0 = from + kKeys * j + 32 * w + 16 * grp;
@@ -476,15 +498,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
         bad |= (blk < 0 && key0 < to ? 1u : 0u) << (2 * grp) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u) << (2 * grp);
         const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
         const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
-        const uint8_t* at0 = pool + slot0 * row_bytes + head_bytes;
-        const uint8_t* at1 = pool + slot1 * row_bytes + head_bytes;
+        constexpr int STEP = 32 / CPR;  // rows per pass of the warp
+        const uint8_t* src0 = pool + (slot0 + r0) * row_bytes + head_bytes + c0 * 16;
+        const uint8_t* src1 = pool + (slot1 + r0) * row_bytes + head_bytes + c0 * 16;
+        const bool whole = key0 >= take_from && key0 + 16 <= to && blk >= 0 && blk2 >= 0;
 #pragma unroll
-        for (int k = 0; k < 16 * CPR / 32; ++k) {
-          const int idx = lane + 32 * k, r = idx / CPR, c = idx % CPR;
-          const bool take = key0 + r >= take_from && key0 + r < to && (r < 8 ? blk : blk2) >= 0;
-          const uint8_t* src = take ? (r < 8 ? at0 : at1) + r * row_bytes + c * 16 : pool;
-          const int rr = 32 * w + 16 * grp + r;
-          cp_async16(dst + (c >> 3) * (kKeys * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src, take);
+        for (int k = 0; k < 16 / STEP; ++k) {
+          const uint32_t d = dst0 + (16 * grp + STEP * k) * 128 + ((x0 ^ uint32_t((STEP * k) & 7)) << 4);
+          const uint8_t* src = (STEP * k < 8 ? src0 : src1) + STEP * k * row_bytes;
+          if (whole) {
+            cp_async16(d, src);
+          } else {
+            const int key = key0 + STEP * k + r0;
+            const bool take = key >= take_from && key < to && (STEP * k < 8 ? blk : blk2) >= 0;
+            cp_async16(d, take ? src : pool, take);
+          }
         }
       }
       if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
@@ -499,64 +527,79 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     while (ok && announced < 2 * steps) announce();
   } else if (wg == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 12 && lane == 0) {
-      // ---- matrix products
+    if (warp == 12) {
+      // ---- matrix products: the whole warp waits, one of its threads issues
       constexpr uint32_t id_s = tc_idesc<KIND>(kTileRows, kKeys, false), id_o = tc_idesc<KIND>(kTileRows, D, true);
+      const uint64_t q_desc = desc_along(smem_u32(smem)), k_desc = desc_along(smem_u32(ring)),
+                     v_desc = desc_across(smem_u32(ring), kKeys * 128);
       Item<NS> item;  // the ring's next item: K of step j on entering step j
-      Item<NS> v;      // the V of step j - 1
       uint32_t used[2] = {0, 0};  // products Q K^T issued per tile
-      bool ok = true, v_ready = false;
-      auto pv = [&](int i, bool accumulate) {
-        ok = ok && mbar_wait(&p_full[i], (used[i] - 1) & 1u);
-        if (ok && !v_ready) ok = mbar_wait(&full[v.stage], v.lap);
-        v_ready = true;
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t vs = smem_u32(ring + v.stage * S::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          tc_mma_ts(tmem + S::kO + i * D, tmem + i * 128 + 8 * k, desc_across(vs + k * 2048, kKeys * 128), id_o,
-                    accumulate || k > 0 ? 1u : 0u);
-        tc_commit(&o_done[i]);
-      };
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
       for (int j = 0; j <= steps && ok; ++j) {
+        // on entering step j > 0 the ring's next item is V of step j - 1, then K of step j
+        const int v_stage = item.stage;
+        if (j > 0) {
+          wait(&full[v_stage], item.lap);
+          if (!ok) break;
+          item.next();
+        }
         const bool k_here = j < steps;
         bool k_ready = false;
-        v = item;  // (on entering step j > 0 the ring's next item is V of step j - 1, then K of step j)
-        if (j > 0) item.next();
-        v_ready = false;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (j > 0 && j - 1 >= first[i] && j - 1 < last[i] && ok) pv(i, j - 1 > first[i]);
-          if (k_here && j >= first[i] && j < last[i] && ok) {
-            if (!k_ready) ok = mbar_wait(&full[item.stage], item.lap);
+          if (j > first[i] && j <= last[i]) {  // P V of step j - 1, in two halves of its keys as the powers arrive
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              wait(&p_full[2 * i + h], (used[i] - 1) & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t vd = v_desc + uint32_t(v_stage * (S::kTileBytes >> 4));
+                const uint32_t more = h > 0 || j - 1 > first[i] ? 1u : 0u;
+#pragma unroll
+                for (int k = h * (kKeys / 32); k < (h + 1) * (kKeys / 32); ++k)
+                  tc_mma_ts(tmem + S::kO + i * D, tmem + i * 128 + 8 * k, vd + k * (2048 >> 4), id_o,
+                            k > h * (kKeys / 32) ? 1u : more);
+                tc_commit(&o_done[2 * i + h]);
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+          }
+          if (k_here && j >= first[i] && j < last[i]) {  // Q K^T of step j
+            if (!k_ready) wait(&full[item.stage], item.lap);
             k_ready = true;
-            if (used[i] == 0) ok = ok && mbar_wait(&q_full[i], 0u);
+            if (ok && used[i] == 0) wait(&q_full[i], 0u);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t qs = smem_u32(smem + i * S::kTileBytes), ks = smem_u32(ring + item.stage * S::kTileBytes);
+            if (elect_one()) {
+              const uint64_t qd = q_desc + uint32_t(i * (S::kTileBytes >> 4)),
+                             kd = k_desc + uint32_t(item.stage * (S::kTileBytes >> 4));
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t at_k = (k >> 2) * (kKeys * 128) + (k & 3) * 32;
-              tc_mma_ss(tmem + i * 128, desc_along(qs + at_k), desc_along(ks + at_k), id_s, k > 0 ? 1u : 0u);
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t at_k = ((k >> 2) * (kKeys * 128) + (k & 3) * 32) >> 4;
+                tc_mma_ss(tmem + i * 128, qd + at_k, kd + at_k, id_s, k > 0 ? 1u : 0u);
+              }
+              tc_commit(&s_full[i]);
+              mbar_arrive(&s_full[i]);
             }
+            __syncwarp();
             ++used[i];
-            tc_commit(&s_full[i]);
-            mbar_arrive(&s_full[i]);
           }
         }
         if (!ok) break;
-        if (j > 0) {
-          if (!v_ready) ok = mbar_wait(&full[v.stage], v.lap);  // no tile had keys in it: it still has to land
-          tc_commit(&empty[v.stage]);
+        if (k_here && !k_ready) wait(&full[item.stage], item.lap);  // a step that neither tile has keys in: it still lands
+        if (!ok) break;
+        if (elect_one()) {
+          if (j > 0) tc_commit(&empty[v_stage]);
+          if (k_here) tc_commit(&empty[item.stage]);
         }
-        if (k_here) {
-          if (!k_ready) ok = ok && mbar_wait(&full[item.stage], item.lap);
-          tc_commit(&empty[item.stage]);
-          item.next();
-        }
+        __syncwarp();
+        if (k_here) item.next();
       }
-      tc_commit(drained);
+      if (elect_one()) tc_commit(drained);
+      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));

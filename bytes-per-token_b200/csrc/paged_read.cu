@@ -54,15 +54,55 @@ struct ReadArgs {
   int split, n_splits;
 };
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  if (dtype == BPT_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == BPT_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
 __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
   if (dtype == BPT_DTYPE_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == BPT_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Two neighbouring elements (the first at an even index) as floats.
+template <int DT>
+__device__ __forceinline__ float2 load_pair(const void* p, int64_t i) {
+  if constexpr (DT == BPT_DTYPE_F32) return *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+  return DT == BPT_DTYPE_F16 ? unpack2<BPT_KV_F16>(u) : unpack2<BPT_KV_BF16>(u);
+}
+
+// The A fragments of one query row per lane quad: rounded to the product's type in rows 0-7, what rounding took off in rows
+// 8-15. For f16 products q is scaled by a power of two into [-1, 1]; returns what undoes it. Every load of a pass is in flight
+// at once (the second pass finds the row in L1).
+template <int KIND, int D, int DT>
+__device__ __forceinline__ float query_rows(const void* q, int64_t at, int t, bool here, uint32_t (&qf)[D / 16][4]) {
+  constexpr bool kExact = DT == BPT_DTYPE_BF16 || (DT == BPT_DTYPE_F16 && KIND != BPT_KV_BF16);  // rounding takes nothing off
+  float2 unit = make_float2(1.f, 1.f);
+  if constexpr (KIND != BPT_KV_BF16 && DT != BPT_DTYPE_F16) {
+    float amax = 0.f;
+    if (here) {
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 x = load_pair<DT>(q, at + q_dim<KIND>(j, t, 2 * i));
+          amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    unit = unit_range(amax);
+  }
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 x = make_float2(0.f, 0.f);
+      if (here) x = load_pair<DT>(q, at + q_dim<KIND>(j, t, 2 * i));
+      x.x *= unit.x;
+      x.y *= unit.x;
+      qf[j][2 * i] = pack2<KIND>(x.x, x.y);
+      const float2 r = unpack2<KIND>(qf[j][2 * i]);
+      qf[j][2 * i + 1] = kExact ? 0u : pack2<KIND>(x.x - r.x, x.y - r.y);
+    }
+  return unit.y;
 }
 
 template <int KIND, int D>
@@ -238,39 +278,11 @@ __global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs 
         for (int i = 0; i < 8; ++i) store_any(a.out, a.out_dtype, (int64_t(use.b) * a.Hq + h0 + r) * D + lane * 8 + i, 0.f);
     }
     if (!MERGE || use.g1 > use.g0) {
-  // q: the A fragments of head h0 + g, rounded in rows 0-7 and what rounding took off in rows 8-15
   uint32_t qf[D / 16][4];
-  float q_unit = 1.f;
-  {
-    const int64_t at = int64_t(use.b) * a.q_sb + int64_t(h0 + g) * a.q_sh;
-    float amax = 0.f;
-    if constexpr (KIND != BPT_KV_BF16) {  // f16 products: q scaled by a power of two into [-1, 1]
-      if (g < heads)
-        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(load_any(a.q, a.q_dtype, at + q_dim<KIND>(j, t, i))));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    }
-    const float2 unit = KIND == BPT_KV_BF16 ? make_float2(1.f, 1.f) : unit_range(amax);
-    q_unit = unit.y;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x = 0.f, y = 0.f;
-        if (g < heads) {
-          x = load_any(a.q, a.q_dtype, at + q_dim<KIND>(j, t, 2 * i)) * unit.x;
-          y = load_any(a.q, a.q_dtype, at + q_dim<KIND>(j, t, 2 * i + 1)) * unit.x;
-        }
-        const uint32_t hi2 = pack2<KIND>(x, y);
-        const float2 r = unpack2<KIND>(hi2);
-        qf[j][2 * i] = hi2;
-        qf[j][2 * i + 1] = a.q_dtype == BPT_DTYPE_F32 || KIND == BPT_KV_BF16 && a.q_dtype == BPT_DTYPE_F16
-                               ? pack2<KIND>(x - r.x, y - r.y) : 0u;
-      }
-    }
-  }
+  const int64_t q_at = int64_t(use.b) * a.q_sb + int64_t(h0 + g) * a.q_sh;
+  const float q_unit = a.q_dtype == BPT_DTYPE_BF16  ? query_rows<KIND, D, BPT_DTYPE_BF16>(a.q, q_at, t, g < heads, qf)
+                       : a.q_dtype == BPT_DTYPE_F16 ? query_rows<KIND, D, BPT_DTYPE_F16>(a.q, q_at, t, g < heads, qf)
+                                                    : query_rows<KIND, D, BPT_DTYPE_F32>(a.q, q_at, t, g < heads, qf);
   const float raw = a.sm_scale * q_unit * a.src.k_scale;  // a product as a score
   const float mul = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
 
@@ -613,6 +625,8 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   BPT_REQUIRE(Hq >= 1 && Hq % Hkv == 0 && Hq < (1 << 15), BPT_ERR_INVALID, "%s: Hq=%lld is not a multiple of Hkv=%lld", who,
               (long long)Hq, (long long)Hkv);
   BPT_REQUIRE(window >= 0, BPT_ERR_INVALID, "%s: window=%lld", who, (long long)window);
+  BPT_REQUIRE(q_stride_b % 2 == 0 && q_stride_h % 2 == 0 && reinterpret_cast<uintptr_t>(q) % (q_dtype == BPT_DTYPE_F32 ? 8 : 4) == 0,
+              BPT_ERR_ALIGNMENT, "%s: q's rows must start on pairs of elements", who);
   BPT_REQUIRE(softcap >= 0.f && softcap < INFINITY, BPT_ERR_INVALID, "%s: softcap must be finite and not negative", who);
   const bool merge = out_partial == nullptr;
   a.q = q;

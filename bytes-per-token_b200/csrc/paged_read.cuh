@@ -35,6 +35,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
   const int bytes = take ? 16 : 0;  // nothing is read where not taken: the 16 bytes become zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -132,10 +135,12 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   return v;
 }
 
-// s0, s1 (+)= q . K^T for 16 keys at `tile` (rows 0-7 -> s0, 8-15 -> s1). q(j): the A fragment of k-step j.
+// s0, s1 += q . K^T for 16 keys at `tile` (rows 0-7 -> s0, 8-15 -> s1). q(j): the A fragment of k-step j. Even and odd
+// k-steps are summed apart: four chains of dependent products instead of two, half as long.
 template <int KIND, int D, typename Q>
 __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, float (&s0)[4], float (&s1)[4]) {
   constexpr int RB = D * kElemBytes<KIND>;
+  float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
   if constexpr (kIs16<KIND>) {
     const int row = (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
     const uint32_t base = tile + row * RB;
@@ -144,8 +149,8 @@ __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, fl
       uint32_t b[4];
       ldmatrix4(b, base + swizzled<KIND, D>(row, 2 * j + c) * 16);
       const MmaRows qj = q(j);
-      mma_16816<KIND>(s0, qj.v, b[0], b[1]);
-      mma_16816<KIND>(s1, qj.v, b[2], b[3]);
+      mma_16816<KIND>(j & 1 ? t0 : s0, qj.v, b[0], b[1]);
+      mma_16816<KIND>(j & 1 ? t1 : s1, qj.v, b[2], b[3]);
     }
   } else {
     const int g = lane >> 2, t = lane & 3;
@@ -157,10 +162,15 @@ __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, fl
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const MmaRows qj = q(4 * j4 + i);
-        mma_16816<KIND>(s0, qj.v, codes_to_f16<KIND>(xs[i] & 0xFFFFu), codes_to_f16<KIND>(xs[i] >> 16));
-        mma_16816<KIND>(s1, qj.v, codes_to_f16<KIND>(ys[i] & 0xFFFFu), codes_to_f16<KIND>(ys[i] >> 16));
+        mma_16816<KIND>(i & 1 ? t0 : s0, qj.v, codes_to_f16<KIND>(xs[i] & 0xFFFFu), codes_to_f16<KIND>(xs[i] >> 16));
+        mma_16816<KIND>(i & 1 ? t1 : s1, qj.v, codes_to_f16<KIND>(ys[i] & 0xFFFFu), codes_to_f16<KIND>(ys[i] >> 16));
       }
     }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    s0[e] += t0[e];
+    s1[e] += t1[e];
   }
 }
 
