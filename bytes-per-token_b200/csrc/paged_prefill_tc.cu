@@ -8,9 +8,7 @@
 //                memory.
 // Four warpgroups: two do the softmax, each of one tile, a thread per row (so neither maximum nor sum crosses threads); one
 // brings pages into a ring of shared-memory stages, K and V of a step in stages of their own, by cp.async (rows of any page
-// size; keys that are not visible become zeros); of the last, one thread issues the matrix products. While the softmax of
-// one tile runs, the tensor cores work on the other tile: P V of its last step (in
-// two halves, the first while the powers of the second are still taken), then Q K^T of its next.
+// size; keys that are not visible become zeros); of the last, one thread issues the XX
 //
 // A row's m is the true maximum of its first 64 keys and moves only when the sum of 2^(s - m) over 64 keys passes 2^15: until then
 // every P is below 2^15, which both 16-bit types hold, and is divided by the sum of the same powers, so nothing is lost by
@@ -20,6 +18,8 @@
 // Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
 // and the CTA still awaits its copies and products, frees its tensor memory and returns.
 #define BPT_WHOLE_PROGRAM  // compiled without relocatable device code
+#include <type_traits>
+
 #include "paged_prefill.cuh"
 
 namespace bpt {
@@ -42,7 +42,7 @@ struct TcShape {
   static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kQ = 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 14;  // an even number: the flags behind them start on 16 bytes
+  static constexpr int kBars = 2 * kStages + 16;  // an even number: the flags behind them start on 16 bytes
   static constexpr int kSmem = 1024 + kQ + kStages * kTileBytes + kBars * 8 + kFlagSteps * 16 + 64;
   static constexpr uint32_t kO = 256;     // columns: S0, S1 at 0, 128; O0, O1 at 256, 256 + D
   static_assert(256 + 2 * D <= 512, "tensor memory");
@@ -176,7 +176,7 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 
 // What a softmax warpgroup does for tile i: its queries into shared memory, then every step's maximum, probabilities and
 // sum, and at the end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
-template <int KIND, int D>
+template <int KIND, int D, bool CAP, bool SLOPED>
 __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& row, int hk, int sp, int parts,
                                              int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
                                              uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags) {
@@ -194,12 +194,10 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_full[i]);
   }
-  const bool cap = a.softcap > 0.f;
   const float raw = a.sm_scale * a.src.k_scale;  // a product as a score
-  const float mul = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
+  const float mul = CAP ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
   const float cap_out = a.softcap * kLog2e;
-  const bool sloped = a.slopes != nullptr;
-  const bool shaped = cap || sloped || !(mul > 0.f);  // a score is not just a positive multiple of its product
+  const float mul_now = CAP || SLOPED ? 1.f : mul;  // what is left to multiply once a product has its shape
   const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
   const uint32_t lanes = uint32_t(32 * warp) << 16;
   const uint32_t s_at = tmem + lanes + i * 128, o_at = tmem + lanes + S::kO + i * D;
@@ -209,31 +207,27 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
   uint32_t n = 0;
   bool ok = true;
   for (int j = first; j < last; ++j, ++n) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], n & 1u));
-    if (!ok) break;
-    tc_fence_after();
     const int key0 = from + j * kKeys;
+    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i], n & 1u));
+    if (!ok) break;
     const uint4 bad = *reinterpret_cast<const uint4*>(flags + (j & (kFlagSteps - 1)) * 4);
     const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
     const bool masked = any_bad || key0 < all_lo || key0 + kKeys > all_hi;
     // Columns c .. c + 31 of S, as scores but for the factor mul_now.
-    const float mul_now = shaped ? 1.f : mul;
-    auto shape = [&](int c, uint32_t* x) {
-      if (shaped) {
-        if (cap) {
+    auto shape = [&](int c, uint32_t* x, auto with_mask) {
+      if constexpr (CAP) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(capped(__uint_as_float(x[e]) * mul, cap_out));
-        } else {
+        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(capped(__uint_as_float(x[e]) * mul, cap_out));
+      } else if constexpr (SLOPED) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * mul);
-        }
-        if (sloped) {
-          const float far = float(key0 + c - row.pos);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(row.slope, fabsf(far + float(e)), __uint_as_float(x[e])));
-        }
+        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * mul);
       }
-      if (masked) {
+      if constexpr (SLOPED) {
+        const float far = float(key0 + c - row.pos);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(row.slope, fabsf(far + float(e)), __uint_as_float(x[e])));
+      }
+      if constexpr (decltype(with_mask)::value) {
         const int below = row.lo - key0 - c, above = row.hi - key0 - c;
         const uint32_t w = c == 0 ? bad.x : c == 32 ? bad.y : c == 64 ? bad.z : bad.w;
 #pragma unroll
@@ -245,8 +239,11 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     // fp32 sum of what was rounded. P V of the first half runs while the powers of the second are taken.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if (h) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i + 1], n & 1u));
+      if (!ok) break;
+      tc_fence_after();
       uint32_t p[32];
-      auto powers = [&](float off) {
+      auto powers = [&](float off, auto with_mask) {
         float2 sum = make_float2(0.f, 0.f);
         uint32_t x[2][32];
         tmem_request32(s_at + 64 * h, x[0]);
@@ -256,7 +253,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
         tmem_arrived32(x[1]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          shape(64 * h + 32 * k, x[k]);
+          shape(64 * h + 32 * k, x[k], with_mask);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 y = ffma2(make_float2(__uint_as_float(x[k][2 * e]), __uint_as_float(x[k][2 * e + 1])),
@@ -272,15 +269,22 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
       const int half0 = key0 + 64 * h;
       const bool fresh = m == -INFINITY && row.lo < half0 + 64 && row.hi > half0;
       float sum = 0.f;
-      if (!__all_sync(0xffffffffu, fresh)) sum = powers(m == -INFINITY ? 0.f : m);
-      const bool moves = fresh || !(sum <= kMostSum);
-      if (__any_sync(0xffffffffu, moves)) {  // a first half-step, and a few later ones: the row's maximum moves
+      bool looked = false, known = !__all_sync(0xffffffffu, fresh);  // some row has a maximum to begin with
+      for (;;) {
+        // (two bodies: as one, its masks would be taken on every step)
+        if (known) {
+          const float off = m == -INFINITY ? 0.f : m;
+          sum = masked ? powers(off, std::true_type()) : powers(off, std::false_type());
+        }
+        const bool moves = fresh ? m == -INFINITY : !(sum <= kMostSum);
+        if (looked || !__any_sync(0xffffffffu, moves)) break;
+        // a first half-step, and a few later ones: the row's maximum is looked up and moves
         float top = -INFINITY;
 #pragma unroll 1
         for (int c = 64 * h; c < 64 * h + 64; c += 32) {
           uint32_t x[32];
           tmem_load32(s_at + c, x);
-          shape(c, x);
+          shape(c, x, std::true_type());
 #pragma unroll
           for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
         }
@@ -304,10 +308,11 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
             tmem_store32(o_at + c, o);
           }
         }
-        sum = powers(m == -INFINITY ? 0.f : m);
+        known = looked = true;
       }
+      if (!ok) break;
       l += sum;
-      tmem_store32(s_at + 32 * h, p);
+      tmem_store32(s_at + 64 * h, p);
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
@@ -352,7 +357,9 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
 }
 
-template <int KIND, int D>
+// CAP: scores are capped. SLOPED: they fall with distance, or their factor is not positive (a maximum of products is then no
+// maximum of scores).
+template <int KIND, int D, bool CAP, bool SLOPED>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillArgs a) {
   using S = TcShape<D>;
   constexpr int NS = S::kStages;
@@ -361,10 +368,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   uint8_t* ring = smem + S::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * S::kTileBytes);
   uint64_t* full = bars;             // [NS] a stage's rows have landed (one arrival per producer warp)
-  uint64_t* empty = full + NS;       // [NS] the products that read it are done
+  uint64_t* empty = full + NS;       // [NS] both tiles' products that read it are done
   uint64_t* q_full = empty + NS;     // [2] a tile's queries are in shared memory
-  uint64_t* s_full = q_full + 2;     // [2] S is in tensor memory
-  uint64_t* p_full = s_full + 2;     // [2][2] a half of P is in tensor memory, O rescaled where needed
+  uint64_t* s_full = q_full + 2;     // [2][2] a tile's half-step of S is in tensor memory
+  uint64_t* p_full = s_full + 4;     // [2][2] a half of P is in tensor memory, O rescaled where needed
   uint64_t* o_done = p_full + 4;     // [2][2] that half's P V is in O
   uint64_t* drained = o_done + 4;    // all products are done
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
@@ -376,11 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 4);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
-      mbar_init(&s_full[i], 2);  // the products' completion, and the issuing thread (whose own waits saw the flags)
+      for (int h = 0; h < 2; ++h) mbar_init(&s_full[2 * i + h], 2);  // the products' completion, and the issuing thread (whose own waits saw the flags)
       mbar_init(&p_full[2 * i], 4);
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_done[2 * i], 1);
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       range[i] = INT_MAX;
       range[2 + i] = 0;
     }
-    mbar_init(drained, 1);
+    mbar_init(drained, 2);
     fence_mbar_init();
   }
   pdl_launch_dependents();
@@ -527,83 +534,73 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     while (ok && announced < 2 * steps) announce();
   } else if (wg == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 12) {
-      // ---- matrix products: the whole warp waits, one of its threads issues
-      constexpr uint32_t id_s = tc_idesc<KIND>(kTileRows, kKeys, false), id_o = tc_idesc<KIND>(kTileRows, D, true);
-      const uint64_t q_desc = desc_along(smem_u32(smem)), k_desc = desc_along(smem_u32(ring)),
+    if (warp < 14) {
+      // ---- matrix products: a warp per tile; the whole warp waits, one of its threads issues. A step's keys go in halves:
+      // S of the next step's half overwrites the columns of this step's half as soon as its P V has been issued.
+      constexpr uint32_t id_s = tc_idesc<KIND>(kTileRows, kKeys / 2, false), id_o = tc_idesc<KIND>(kTileRows, D, true);
+      const int i = warp - 12, begin = i ? first[1] : first[0], end = i ? last[1] : last[0];
+      const uint64_t q_desc = desc_along(smem_u32(smem + i * S::kTileBytes)), k_desc = desc_along(smem_u32(ring)),
                      v_desc = desc_across(smem_u32(ring), kKeys * 128);
-      Item<NS> item;  // the ring's next item: K of step j on entering step j
-      uint32_t used[2] = {0, 0};  // products Q K^T issued per tile
+      const uint32_t s_at = tmem + i * 128, o_at = tmem + S::kO + i * D;
+      Item<NS> item;  // the ring's next item: K of step j on entering step j = 0, else V of step j - 1, then K of step j
+      uint32_t n = 0;  // steps whose Q K^T has been issued
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      if (end > begin) wait(&q_full[i], 0u);
       for (int j = 0; j <= steps && ok; ++j) {
-        // on entering step j > 0 the ring's next item is V of step j - 1, then K of step j
         const int v_stage = item.stage;
         if (j > 0) {
           wait(&full[v_stage], item.lap);
           if (!ok) break;
           item.next();
         }
-        const bool k_here = j < steps;
-        bool k_ready = false;
+        const int k_stage = item.stage;
+        if (j < steps) {
+          wait(&full[k_stage], item.lap);
+          if (!ok) break;
+          item.next();
+        }
+        const bool pv = j > begin && j <= end, qk = j >= begin && j < end;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (j > first[i] && j <= last[i]) {  // P V of step j - 1, in two halves of its keys as the powers arrive
+        for (int h = 0; h < 2; ++h) {
+          if (pv) wait(&p_full[2 * i + h], (n - 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            if (pv) {  // P V of step j - 1
+              const uint64_t vd = v_desc + uint32_t(v_stage * (S::kTileBytes >> 4) + h * (kKeys / 2 * 128 >> 4));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              wait(&p_full[2 * i + h], (used[i] - 1) & 1u);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint64_t vd = v_desc + uint32_t(v_stage * (S::kTileBytes >> 4));
-                const uint32_t more = h > 0 || j - 1 > first[i] ? 1u : 0u;
-#pragma unroll
-                for (int k = h * (kKeys / 32); k < (h + 1) * (kKeys / 32); ++k)
-                  tc_mma_ts(tmem + S::kO + i * D, tmem + i * 128 + 8 * k, vd + k * (2048 >> 4), id_o,
-                            k > h * (kKeys / 32) ? 1u : more);
-                tc_commit(&o_done[2 * i + h]);
-              }
-              __syncwarp();
+              for (int k = 0; k < kKeys / 32; ++k)
+                tc_mma_ts(o_at, s_at + 64 * h + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || h > 0 || j - 1 > begin ? 1u : 0u);
+              tc_commit(&o_done[2 * i + h]);
             }
-            if (!ok) break;
-          }
-          if (k_here && j >= first[i] && j < last[i]) {  // Q K^T of step j
-            if (!k_ready) wait(&full[item.stage], item.lap);
-            k_ready = true;
-            if (ok && used[i] == 0) wait(&q_full[i], 0u);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t qd = q_desc + uint32_t(i * (S::kTileBytes >> 4)),
-                             kd = k_desc + uint32_t(item.stage * (S::kTileBytes >> 4));
+            if (qk) {  // Q K^T of step j
+              const uint64_t kd = k_desc + uint32_t(k_stage * (S::kTileBytes >> 4) + h * (kKeys / 2 * 128 >> 4));
 #pragma unroll
               for (int k = 0; k < D / 16; ++k) {
-                const uint32_t at_k = ((k >> 2) * (kKeys * 128) + (k & 3) * 32) >> 4;
-                tc_mma_ss(tmem + i * 128, qd + at_k, kd + at_k, id_s, k > 0 ? 1u : 0u);
+                const uint32_t at_k = (k & 3) * (32 >> 4), at_q = (k >> 2) * (kTileRows * 128 >> 4) + at_k;
+                tc_mma_ss(s_at + 64 * h, q_desc + at_q, kd + (k >> 2) * (kKeys * 128 >> 4) + at_k, id_s, k > 0 ? 1u : 0u);
               }
-              tc_commit(&s_full[i]);
-              mbar_arrive(&s_full[i]);
+              tc_commit(&s_full[2 * i + h]);
+              mbar_arrive(&s_full[2 * i + h]);
             }
-            __syncwarp();
-            ++used[i];
           }
+          __syncwarp();
         }
         if (!ok) break;
-        if (k_here && !k_ready) wait(&full[item.stage], item.lap);  // a step that neither tile has keys in: it still lands
-        if (!ok) break;
+        if (qk) ++n;
         if (elect_one()) {
           if (j > 0) tc_commit(&empty[v_stage]);
-          if (k_here) tc_commit(&empty[item.stage]);
+          if (j < steps) tc_commit(&empty[k_stage]);
         }
         __syncwarp();
-        if (k_here) item.next();
       }
       if (elect_one()) tc_commit(drained);
       __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_rows<KIND, D>(a, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
+    softmax_rows<KIND, D, CAP, SLOPED>(a, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
                           flags);
   }
   __syncwarp();
@@ -616,10 +613,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   }
 }
 
-template <int KIND, int D>
+template <int KIND, int D, bool CAP, bool SLOPED>
 int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
   using S = TcShape<D>;
-  const void* kernel = reinterpret_cast<const void*>(paged_prefill_tc_kernel<KIND, D>);
+  const void* kernel = reinterpret_cast<const void*>(paged_prefill_tc_kernel<KIND, D, CAP, SLOPED>);
   static std::atomic<uint64_t> ready{0};
   if (ready.load(std::memory_order_relaxed) == 0) {
     // setmaxnreg hands out the registers of the launch: a build whose kernel was compiled to fewer would wait for ever
@@ -641,9 +638,16 @@ int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t strea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_tc_kernel<KIND, D>, a);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_tc_kernel<KIND, D, CAP, SLOPED>, a);
   if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
   return BPT_OK;
+}
+
+template <int KIND, int D>
+int launch_shape(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
+  const bool cap = a.softcap > 0.f, sloped = a.slopes != nullptr || !(a.sm_scale > 0.f);
+  if (cap) return sloped ? launch_tc<KIND, D, true, true>(a, tiles, flags, stream) : launch_tc<KIND, D, true, false>(a, tiles, flags, stream);
+  return sloped ? launch_tc<KIND, D, false, true>(a, tiles, flags, stream) : launch_tc<KIND, D, false, false>(a, tiles, flags, stream);
 }
 
 }  // namespace
@@ -658,8 +662,8 @@ int take_prefill_tc_error() {
 
 int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream) {
   if (kind == BPT_KV_F16)
-    return a.D == 64 ? launch_tc<BPT_KV_F16, 64>(a, tiles, flags, stream) : launch_tc<BPT_KV_F16, 128>(a, tiles, flags, stream);
-  return a.D == 64 ? launch_tc<BPT_KV_BF16, 64>(a, tiles, flags, stream) : launch_tc<BPT_KV_BF16, 128>(a, tiles, flags, stream);
+    return a.D == 64 ? launch_shape<BPT_KV_F16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_F16, 128>(a, tiles, flags, stream);
+  return a.D == 64 ? launch_shape<BPT_KV_BF16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_BF16, 128>(a, tiles, flags, stream);
 }
 
 }  // namespace bpt
