@@ -42,7 +42,7 @@ struct TcShape {
   static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kQ = 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 16;  // an even number: the flags behind them start on 16 bytes
+  static constexpr int kBars = 2 * kStages + 18;  // an even number: the flags behind them start on 16 bytes
   static constexpr int kSmem = 1024 + kQ + kStages * kTileBytes + kBars * 8 + kFlagSteps * 16 + 64;
   static constexpr uint32_t kO = 256;     // columns: S0, S1 at 0, 128; O0, O1 at 256, 256 + D
   static_assert(256 + 2 * D <= 512, "tensor memory");
@@ -179,16 +179,25 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 template <int KIND, int D, bool CAP, bool SLOPED>
 __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& row, int hk, int sp, int parts,
                                              int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
-                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags) {
+                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
+                                             uint64_t* started, const uint32_t* flags) {
   using S = TcShape<D>;
   const int r = threadIdx.x & 127, warp = r >> 5, lane = threadIdx.x & 31;
   {
-    uint8_t* tile = smem + i * S::kTileBytes + r * 128;
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + max(row.q, int64_t(0)));
+    // 32 / CPR rows per pass of the warp, a row's 16-byte chunks side by side
+    constexpr int CPR = D / 8;
+    uint8_t* tile = smem + i * S::kTileBytes;
+    const int c = lane % CPR;
+    uint4 x[CPR];
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      const uint4 x = row.q >= 0 ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (r & 7)) << 4)) = x;
+    for (int k = 0; k < CPR; ++k) {
+      const int64_t at = __shfl_sync(0xffffffffu, row.q, 32 / CPR * k + lane / CPR);
+      x[k] = at >= 0 ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at)[c] : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < CPR; ++k) {
+      const int rr = 32 * warp + 32 / CPR * k + lane / CPR;
+      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kTileRows * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[k];
     }
     fence_proxy_async_shared();
     __syncwarp();
@@ -317,41 +326,69 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+      if (i == 0 && n == 0 && h == 0 && lane == 0) mbar_arrive(started);
     }
     if (!ok) break;
   }
+  if (i == 0 && n == 0 && lane == 0) mbar_arrive(started);  // (a tile that sees no key)
   if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * i + 1], (n - 1) & 1u));
   tc_fence_after();
   const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
   const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
-  float* part = parts > 1 ? a.part_out + ((tile * a.n_splits + sp) * kRows + i * kTileRows + r) * D : nullptr;
+  // Rows to memory through the warp's share of the tile's queries (which the last products have read), so that a row's
+  // 16-byte chunks are stored side by side: 2 D bytes of 32 rows at a time, all of them in 16 bits or half of a part in fp32.
+  constexpr int CPR = D / 8;
+  uint8_t* stage = smem + i * S::kTileBytes + warp * (32 * 2 * D);
+  const int c = lane % CPR;
 #pragma unroll 1
-  for (int c = 0; ok && c < D; c += 32) {
-    uint32_t o[32];
-    if (n > 0) {
-      tmem_load32(o_at + c, o);
-    } else {
+  for (int half = 0; half < (parts > 1 ? 2 : 1); ++half) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0u;
-    }
-    if (row.out < 0) {
-    } else if (parts > 1) {
+    for (int b = 0; b < CPR; b += 8) {  // eight chunks: 64 values of 16 bits or 32 of fp32
+      uint32_t o[32];
 #pragma unroll
-      for (int e = 0; e < 32; e += 4)
-        *reinterpret_cast<float4*>(part + c + e) =
-            make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv,
-                        __uint_as_float(o[e + 3]) * inv);
-    } else {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row.out + c);
+      for (int q = 0; q < 2; ++q) {
+        if (parts > 1 && q == 1) break;
+        const int col = parts > 1 ? half * (D / 2) + 4 * b : 8 * b + 32 * q;
+        if (n > 0) {
+          tmem_load32(o_at + col, o);
+        } else {
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        uint32_t w[4];
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (parts > 1) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = pack2<KIND>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-        dst[e >> 3] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stage + lane * (2 * D) + (((b + e) ^ (lane & 7)) << 4)) =
+                make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                            __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = pack2<KIND>(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(stage + lane * (2 * D) + (((b + 4 * q + e) ^ (lane & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
       }
     }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < CPR; ++k) {
+      const int rr = 32 / CPR * k + lane / CPR;
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * (2 * D) + ((c ^ (rr & 7)) << 4));
+      const int64_t to = __shfl_sync(0xffffffffu, row.out, rr);
+      if (!ok || to < 0) continue;
+      if (parts > 1) {
+        float* part = a.part_out + ((tile * a.n_splits + sp) * kRows + i * kTileRows + 32 * warp + rr) * D + half * (D / 2);
+        reinterpret_cast<uint4*>(part)[c] = x;
+      } else {
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to)[c] = x;
+      }
+    }
+    __syncwarp();
   }
   if (ok && parts > 1 && row.out >= 0)
     a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
@@ -374,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   uint64_t* p_full = s_full + 4;     // [2][2] a half of P is in tensor memory, O rescaled where needed
   uint64_t* o_done = p_full + 4;     // [2][2] that half's P V is in O
   uint64_t* drained = o_done + 4;    // all products are done
+  uint64_t* started = drained + 1;   // tile 0 has taken its first powers
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
   int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
   uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address
@@ -396,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       range[2 + i] = 0;
     }
     mbar_init(drained, 2);
+    mbar_init(started, 4);
     fence_mbar_init();
   }
   pdl_launch_dependents();
@@ -481,8 +520,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     for (int n = 0; n < 2 * steps && ok; ++n) {
       const int j = n >> 1;
       if (n >= NS) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
-        if (!ok) break;
+        // before waiting for a stage, announce what is in flight: the products that free it may need just that
+        if (!__all_sync(0xffffffffu, mbar_test(&empty[in.stage], in.lap ^ 1u))) {
+          cp_async_wait<0>();
+          while (announced < n) announce();
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+          if (!ok) break;
+        }
       }
       if ((n & 1) == 0) {
         if ((j & 15) == 0) {
@@ -525,10 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
       cp_async_commit();
       in.next();
-      if (n >= kLag) {
-        cp_async_wait<kLag>();
-        announce();
-      }
+      cp_async_wait<kLag>();
+      if (announced + kLag <= n) announce();
     }
     cp_async_wait<0>();
     while (ok && announced < 2 * steps) announce();
@@ -547,6 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
       if (end > begin) wait(&q_full[i], 0u);
+      // Tile 1 starts half a step late, and stays so: in step, both tiles would take powers at once and then wait at once.
+      if (i == 1 && ok && end > begin) wait(started, 0u);
       for (int j = 0; j <= steps && ok; ++j) {
         const int v_stage = item.stage;
         if (j > 0) {
@@ -601,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_rows<KIND, D, CAP, SLOPED>(a, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
-                          flags);
+                          started, flags);
   }
   __syncwarp();
   tc_fence_before();
