@@ -60,26 +60,22 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_request32(uint32_t addr, uint32_t* v) {
+__device__ __forceinline__ void tmem_load64(uint32_t addr, uint32_t (&v)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, "
+      "%36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, "
+      "%57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+        "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
+        "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
       : "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// The registers of a request, once tmem_wait_load has returned: nothing reads them before this.
-__device__ __forceinline__ void tmem_arrived32(uint32_t* v) {
-  asm volatile(""
-      : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-        "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-        "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
-        "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-      :
       : "memory");
 }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
@@ -254,18 +250,14 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
       uint32_t p[32];
       auto powers = [&](float off, auto with_mask) {
         float2 sum = make_float2(0.f, 0.f);
-        uint32_t x[2][32];
-        tmem_request32(s_at + 64 * h, x[0]);
-        tmem_request32(s_at + 64 * h + 32, x[1]);
-        tmem_wait_load();
-        tmem_arrived32(x[0]);
-        tmem_arrived32(x[1]);
+        uint32_t x[64];
+        tmem_load64(s_at + 64 * h, x);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          shape(64 * h + 32 * k, x[k], with_mask);
+          shape(64 * h + 32 * k, x + 32 * k, with_mask);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float2 y = ffma2(make_float2(__uint_as_float(x[k][2 * e]), __uint_as_float(x[k][2 * e + 1])),
+            const float2 y = ffma2(make_float2(__uint_as_float(x[32 * k + 2 * e]), __uint_as_float(x[32 * k + 2 * e + 1])),
                                    make_float2(mul_now, mul_now), make_float2(-off, -off));
             const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             sum = fadd2(sum, z);
