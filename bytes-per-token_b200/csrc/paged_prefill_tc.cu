@@ -37,8 +37,9 @@ static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "
 constexpr int kFlagSteps = 16;     // steps whose bad-block flags are kept (the ring runs at most 5 steps ahead)
 constexpr float kMostSum = 32768.f;  // a step's sum of powers beyond which a row's maximum moves
 
-template <int D>
+template <int KIND, int D>
 struct TcShape {
+  static constexpr int kRowBytes = D * kElemBytes<KIND>;  // a key's row in its page
   static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kQ = 2 * kTileBytes;
@@ -177,29 +178,54 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
                                              int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
                                              uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
                                              uint64_t* started, const uint32_t* flags) {
-  using S = TcShape<D>;
+  using S = TcShape<KIND, D>;
   const int r = threadIdx.x & 127, warp = r >> 5, lane = threadIdx.x & 31;
+  float q_unit = 1.f;
   {
     // 32 / CPR rows per pass of the warp, a row's 16-byte chunks side by side
-    constexpr int CPR = D / 8;
+    constexpr int CPR = D / 8, RPP = 32 / CPR;
     uint8_t* tile = smem + i * S::kTileBytes;
     const int c = lane % CPR;
     uint4 x[CPR];
 #pragma unroll
     for (int k = 0; k < CPR; ++k) {
-      const int64_t at = __shfl_sync(0xffffffffu, row.q, 32 / CPR * k + lane / CPR);
+      const int64_t at = __shfl_sync(0xffffffffu, row.q, RPP * k + lane / CPR);
       x[k] = at >= 0 ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at)[c] : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if constexpr (!kIs16<KIND>) {
+      // f16 products of bf16 queries: a row is brought into [-1, 1] by a power of two (exact, but for parts 2^-24 below its
+      // largest); the score's factor takes it back
+      if (a.q_dtype == BPT_DTYPE_BF16) {
+#pragma unroll
+        for (int k = 0; k < CPR; ++k) {
+          const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          float2 f[4];
+          float amax = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e] = unpack2<BPT_KV_BF16>(u[e]);
+            amax = fmaxf(amax, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+          }
+#pragma unroll
+          for (int o = CPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const float2 unit = unit_range(amax);
+          x[k] = make_uint4(pack2<KIND>(f[0].x * unit.x, f[0].y * unit.x), pack2<KIND>(f[1].x * unit.x, f[1].y * unit.x),
+                            pack2<KIND>(f[2].x * unit.x, f[2].y * unit.x), pack2<KIND>(f[3].x * unit.x, f[3].y * unit.x));
+          const float back = __shfl_sync(0xffffffffu, unit.y, (lane % RPP) * CPR);  // of row RPP k + lane mod RPP
+          if (lane / RPP == k) q_unit = back;
+        }
+      }
     }
 #pragma unroll
     for (int k = 0; k < CPR; ++k) {
-      const int rr = 32 * warp + 32 / CPR * k + lane / CPR;
+      const int rr = 32 * warp + RPP * k + lane / CPR;
       *reinterpret_cast<uint4*>(tile + (c >> 3) * (kTileRows * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[k];
     }
     fence_proxy_async_shared();
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_full[i]);
   }
-  const float raw = a.sm_scale * a.src.k_scale;  // a product as a score
+  const float raw = a.sm_scale * a.src.k_scale * q_unit;  // a product as a score
   const float mul = CAP ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
   const float cap_out = a.softcap * kLog2e;
   const float mul_now = CAP || SLOPED ? 1.f : mul;  // what is left to multiply once a product has its shape
@@ -330,6 +356,11 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
   // Rows to memory through the warp's share of the tile's queries (which the last products have read), so that a row's
   // 16-byte chunks are stored side by side: 2 D bytes of 32 rows at a time, all of them in 16 bits or half of a part in fp32.
   constexpr int CPR = D / 8;
+  const bool bf16 = a.q_dtype == BPT_DTYPE_BF16;
+  auto pack_out = [&](float x, float y) {
+    if constexpr (kIs16<KIND>) return pack2<KIND>(x, y);
+    return bf16 ? pack2<BPT_KV_BF16>(x, y) : pack2<BPT_KV_F16>(x, y);
+  };
   uint8_t* stage = smem + i * S::kTileBytes + warp * (32 * 2 * D);
   const int c = lane % CPR;
 #pragma unroll 1
@@ -359,7 +390,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = pack2<KIND>(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
+              w[k] = pack_out(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
             *reinterpret_cast<uint4*>(stage + lane * (2 * D) + (((b + 4 * q + e) ^ (lane & 7)) << 4)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -390,7 +421,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
 // maximum of scores).
 template <int KIND, int D, bool CAP, bool SLOPED>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillArgs a) {
-  using S = TcShape<D>;
+  using S = TcShape<KIND, D>;
   constexpr int NS = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -484,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     // ---- producer: warp w brings rows 32 w .. 32 w + 31 of every stage, two groups of 16 keys
     const int w = warp & 3;
     const int32_t* table = a.src.block_table + int64_t(b) * a.src.bt_stride;
-    const int64_t row_bytes = int64_t(a.src.Hkv) * (2 * D), head_bytes = int64_t(hk) * (2 * D);
+    const int64_t row_bytes = int64_t(a.src.Hkv) * S::kRowBytes, head_bytes = int64_t(hk) * S::kRowBytes;
     const bool two = a.src.bs_log2 == 3;
     const int take_from = max(from, lo);
     int held = -1, held2 = -1;  // lane n: the block(s) of group n of the current 16 steps
@@ -497,6 +528,76 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       }
       return blk;
     };
+    auto hold = [&](int j) {
+      const int key = from + kKeys * (j + (lane >> 1)) + 32 * w + 16 * (lane & 1);
+      held = block_at(key);
+      if (two) held2 = block_at(key + 8);
+    };
+    // The blocks of group grp of step j (one twice where pages are longer than 8), and what the table names wrongly.
+    auto blocks_of = [&](int j, int grp, int& blk, int& blk2, uint32_t& bad) {
+      const int key0 = from + kKeys * j + 32 * w + 16 * grp;
+      blk = __shfl_sync(0xffffffffu, held, 2 * (j & 15) + grp);
+      blk2 = two ? __shfl_sync(0xffffffffu, held2, 2 * (j & 15) + grp) : blk;
+      bad |= (blk < 0 && key0 < to ? 1u : 0u) << (2 * grp) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u) << (2 * grp);
+    };
+    if constexpr (!kIs16<KIND>) {
+    // Codes go through registers: 16 codes a load, an f16 each into the stage. An item's loads are issued an item ahead.
+    constexpr int CPR = D / 16, RPP = 32 / CPR;  // 16-code chunks of a row; rows per pass of the warp
+    const int r0 = lane / CPR, c0 = lane % CPR;
+    uint4 codes[2][CPR];
+    bool ok = true;
+    Item<NS> in;
+    auto load = [&](int n, uint4 (&x)[CPR]) {
+      const int j = n >> 1;
+      if ((n & 1) == 0 && (j & 15) == 0) hold(j);
+      const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
+      uint32_t bad = 0;
+#pragma unroll
+      for (int grp = 0; grp < 2; ++grp) {
+        int blk, blk2;
+        blocks_of(j, grp, blk, blk2, bad);
+        const int key0 = from + kKeys * j + 32 * w + 16 * grp;
+        const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
+        const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
+#pragma unroll
+        for (int k = 0; k < 16 / RPP; ++k) {
+          const int r = RPP * k + r0;
+          const bool take = key0 + r >= take_from && key0 + r < to && (RPP * k < 8 ? blk : blk2) >= 0;
+          x[grp * (16 / RPP) + k] =
+              take ? __ldg(reinterpret_cast<const uint4*>(pool + ((RPP * k < 8 ? slot0 : slot1) + r) * row_bytes + head_bytes) + c0)
+                   : make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
+    };
+    auto store = [&](const uint4 (&x)[CPR]) {
+      uint8_t* dst = ring + in.stage * S::kTileBytes + ((2 * c0) >> 3) * (kKeys * 128);
+#pragma unroll
+      for (int k = 0; k < CPR; ++k) {
+        const int rr = 32 * w + RPP * k + r0;
+        const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<uint4*>(dst + rr * 128 + ((((2 * c0 + e) & 7) ^ (rr & 7)) << 4)) =
+              make_uint4(codes_to_f16<KIND>(u[2 * e] & 0xFFFFu), codes_to_f16<KIND>(u[2 * e] >> 16),
+                         codes_to_f16<KIND>(u[2 * e + 1] & 0xFFFFu), codes_to_f16<KIND>(u[2 * e + 1] >> 16));
+      }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[in.stage]);
+    };
+    if (steps > 0) load(0, codes[0]);
+    for (int n = 0; n < 2 * steps && ok; n += 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (n + h + 1 < 2 * steps) load(n + h + 1, codes[h ^ 1]);
+        if (n + h >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+        if (!ok) break;
+        store(codes[h]);
+        in.next();
+      }
+    }
+    } else {
     constexpr int CPR = D / 8;  // 16-byte chunks of a row
     constexpr int kLag = 2;     // items in flight before the oldest is announced
     Item<NS> in, out;
@@ -521,11 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
         }
       }
       if ((n & 1) == 0) {
-        if ((j & 15) == 0) {
-          const int key = from + kKeys * (j + (lane >> 1)) + 32 * w + 16 * (lane & 1);
-          held = block_at(key);
-          if (two) held2 = block_at(key + 8);
-        }
+        if ((j & 15) == 0) hold(j);
       }
       const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
       const uint32_t dst = smem_u32(ring + in.stage * S::kTileBytes);
@@ -536,9 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
 #pragma unroll
       for (int grp = 0; grp < 2; ++grp) {
         const int key0 = from + kKeys * j + 32 * w + 16 * grp;
-        const int blk = __shfl_sync(0xffffffffu, held, 2 * (j & 15) + grp);
-        const int blk2 = two ? __shfl_sync(0xffffffffu, held2, 2 * (j & 15) + grp) : blk;
-        bad |= (blk < 0 && key0 < to ? 1u : 0u) << (2 * grp) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u) << (2 * grp);
+        int blk, blk2;
+        blocks_of(j, grp, blk, blk2, bad);
         const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
         const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
         constexpr int STEP = 32 / CPR;  // rows per pass of the warp
@@ -566,6 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     }
     cp_async_wait<0>();
     while (ok && announced < 2 * steps) announce();
+    }
   } else if (wg == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp < 14) {
@@ -651,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
 
 template <int KIND, int D, bool CAP, bool SLOPED>
 int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
-  using S = TcShape<D>;
+  using S = TcShape<KIND, D>;
   const void* kernel = reinterpret_cast<const void*>(paged_prefill_tc_kernel<KIND, D, CAP, SLOPED>);
   static std::atomic<uint64_t> ready{0};
   if (ready.load(std::memory_order_relaxed) == 0) {
@@ -697,6 +794,8 @@ int take_prefill_tc_error() {
 }
 
 int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream) {
+  if (kind == BPT_KV_FP8)
+    return a.D == 64 ? launch_shape<BPT_KV_FP8, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_FP8, 128>(a, tiles, flags, stream);
   if (kind == BPT_KV_F16)
     return a.D == 64 ? launch_shape<BPT_KV_F16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_F16, 128>(a, tiles, flags, stream);
   return a.D == 64 ? launch_shape<BPT_KV_BF16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_BF16, 128>(a, tiles, flags, stream);
