@@ -87,6 +87,7 @@ __device__ __forceinline__ int sequence_length(const PrefillArgs& a, int b, bool
 
 struct RowAt {
   int64_t q, out;  // element offsets of its query and its output, -1 for a row past the sequence's end
+  int code;        // the same row counted from its tile's first token and head: tokens << 16 | heads, -1 for none
   int pos, lo, hi;
   float slope;  // minus the head's slope, in base 2
 };
@@ -94,10 +95,11 @@ struct RowAt {
 __device__ __forceinline__ RowAt row_at(const PrefillArgs& a, const TileAt& at, int r, int hk, int len) {
   RowAt x;
   const int t = r / a.rep, h = hk * a.rep + r - t * a.rep;
-  if (t >= at.tokens) return RowAt{-1, -1, 0, 0, 0, 0.f};
+  if (t >= at.tokens) return RowAt{-1, -1, -1, 0, 0, 0, 0.f};
   const int token = at.token0 + t;
   x.q = int64_t(token) * a.q_st + int64_t(h) * a.q_sh;
   x.out = (int64_t(token) * a.Hq + h) * a.D;
+  x.code = ((t - at.row0 / a.rep) << 16) | (r - t * a.rep);
   x.pos = a.positions ? min(max(a.positions[token], -1), 1 << 30) : len - at.tokens + t;
   x.lo = a.key_starts ? max(a.key_starts[token], 0) : 0;
   if (a.window > 0) x.lo = max(x.lo, x.pos - a.window + 1);

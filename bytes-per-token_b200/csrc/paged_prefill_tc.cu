@@ -174,7 +174,7 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
 // What a softmax warpgroup does for tile i: its queries into shared memory, then every step's maximum, probabilities and
 // sum, and at the end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
 template <int KIND, int D, bool CAP, bool SLOPED>
-__device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& row, int hk, int sp, int parts,
+__device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt& at, const RowAt& row, int hk, int sp, int parts,
                                              int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
                                              uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
                                              uint64_t* started, const uint32_t* flags) {
@@ -187,11 +187,18 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     uint8_t* tile = smem + i * S::kTileBytes;
     const int c = lane % CPR;
     uint4 x[CPR];
+    // (loads without conditions, so that all are in flight at once: rows that are none read the tile's first and become zeros)
+    const int64_t q0 = int64_t(at.token0 + at.row0 / a.rep) * a.q_st + int64_t(hk * a.rep) * a.q_sh + 8 * c;
 #pragma unroll
     for (int k = 0; k < CPR; ++k) {
-      const int64_t at = __shfl_sync(0xffffffffu, row.q, RPP * k + lane / CPR);
-      x[k] = at >= 0 ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at)[c] : make_uint4(0u, 0u, 0u, 0u);
+      const int code = max(__shfl_sync(0xffffffffu, row.code, RPP * k + lane / CPR), 0);
+      const int64_t from_q0 = int64_t(code >> 16) * a.q_st + (code & 0xFFFF) * a.q_sh;
+      x[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + q0 + from_q0));
     }
+    const uint32_t rows = __ballot_sync(0xffffffffu, row.code >= 0);
+#pragma unroll
+    for (int k = 0; k < CPR; ++k)
+      if (!(rows >> (RPP * k + lane / CPR) & 1u)) x[k] = make_uint4(0u, 0u, 0u, 0u);
     if constexpr (!kIs16<KIND>) {
       // f16 products of bf16 queries: a row is brought into [-1, 1] by a power of two (exact, but for parts 2^-24 below its
       // largest); the score's factor takes it back
@@ -241,6 +248,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     const int key0 = from + j * kKeys;
     ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i], n & 1u));
     if (!ok) break;
+    if (i == 0 && n == 0 && lane == 0) mbar_arrive(started);
     const uint4 bad = *reinterpret_cast<const uint4*>(flags + (j & (kFlagSteps - 1)) * 4);
     const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
     const bool masked = any_bad || key0 < all_lo || key0 + kKeys > all_hi;
@@ -344,7 +352,6 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
-      if (i == 0 && n == 0 && h == 0 && lane == 0) mbar_arrive(started);
     }
     if (!ok) break;
   }
@@ -363,6 +370,8 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
   };
   uint8_t* stage = smem + i * S::kTileBytes + warp * (32 * 2 * D);
   const int c = lane % CPR;
+  const int64_t out0 = (int64_t(at.token0 + at.row0 / a.rep) * a.Hq + hk * a.rep) * (2 * D);  // of the tile's first row, in bytes
+  const int64_t part0 = ((tile * a.n_splits + sp) * kRows + i * kTileRows + 32 * warp) * (4 * D);  // of the warp's first row
 #pragma unroll 1
   for (int half = 0; half < (parts > 1 ? 2 : 1); ++half) {
 #pragma unroll
@@ -402,18 +411,16 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const RowAt& 
     for (int k = 0; k < CPR; ++k) {
       const int rr = 32 / CPR * k + lane / CPR;
       const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * (2 * D) + ((c ^ (rr & 7)) << 4));
-      const int64_t to = __shfl_sync(0xffffffffu, row.out, rr);
-      if (!ok || to < 0) continue;
-      if (parts > 1) {
-        float* part = a.part_out + ((tile * a.n_splits + sp) * kRows + i * kTileRows + 32 * warp + rr) * D + half * (D / 2);
-        reinterpret_cast<uint4*>(part)[c] = x;
-      } else {
-        reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to)[c] = x;
+      const int code = __shfl_sync(0xffffffffu, row.code, rr);
+      if (code >= 0 && ok) {
+        uint8_t* dst = parts > 1 ? reinterpret_cast<uint8_t*>(a.part_out) + part0 + int64_t(rr) * (4 * D) + half * (2 * D)
+                                 : static_cast<uint8_t*>(a.out) + out0 + ((code >> 16) * a.Hq + (code & 0xFFFF)) * (2 * D);
+        *reinterpret_cast<uint4*>(dst + 16 * c) = x;
       }
     }
     __syncwarp();
   }
-  if (ok && parts > 1 && row.out >= 0)
+  if (ok && parts > 1 && row.code >= 0)
     a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
 }
 
@@ -434,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   uint64_t* p_full = s_full + 4;     // [2][2] a half of P is in tensor memory, O rescaled where needed
   uint64_t* o_done = p_full + 4;     // [2][2] that half's P V is in O
   uint64_t* drained = o_done + 4;    // all products are done
-  uint64_t* started = drained + 1;   // tile 0 has taken its first powers
+  uint64_t* started = drained + 1;   // tile 0 has its first scores
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
   int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
   uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   __syncthreads();
 
   // the tiles' rows: thread r of a softmax warpgroup holds row r
-  RowAt row{-1, -1, 0, 0, 0, 0.f};
+  RowAt row{-1, -1, -1, 0, 0, 0, 0.f};
   if (wg < 2) {
     row = row_at(a, at, at.row0 + wg * kTileRows + (tid & 127), hk, len);
     const bool any = row.hi > row.lo;
@@ -483,13 +490,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       atomicMin(&range[wg], lo);
       atomicMax(&range[2 + wg], hi);
     }
+  } else if (warp == 12) {  // all of tensor memory (one CTA per SM)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  auto free_tmem = [&]() {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  };
   const int lo = min(range[0], range[1]), hi = max(range[2], range[3]);
   const int base = lo == INT_MAX ? 0 : lo & ~15;
   const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
   if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = parts;
-  if (sp >= max(parts, 1)) return;
+  if (sp >= max(parts, 1)) {
+    if (warp == 12) free_tmem();
+    return;
+  }
   const int from = base + sp * a.split;
   const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
   const int steps = (to - from + kKeys - 1) / kKeys;
@@ -501,15 +520,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     first[i] = h > l ? (l - from) / kKeys : 0;
     last[i] = h > l ? (h - from + kKeys - 1) / kKeys : 0;
   }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *slot;
-
   if (wg == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // ---- producer: warp w brings rows 32 w .. 32 w + 31 of every stage, two groups of 16 keys
@@ -545,9 +555,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     constexpr int CPR = D / 16, RPP = 32 / CPR;  // 16-code chunks of a row; rows per pass of the warp
     const int r0 = lane / CPR, c0 = lane % CPR;
     uint4 codes[2][CPR];
+    uint32_t taken[2];
     bool ok = true;
     Item<NS> in;
-    auto load = [&](int n, uint4 (&x)[CPR]) {
+    // (loads without conditions, so that all are in flight at once; what is not taken reads the pool's start and is dropped)
+    auto load = [&](int n, uint4 (&x)[CPR], uint32_t& taken) {
+      taken = 0;
       const int j = n >> 1;
       if ((n & 1) == 0 && (j & 15) == 0) hold(j);
       const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
@@ -563,19 +576,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
         for (int k = 0; k < 16 / RPP; ++k) {
           const int r = RPP * k + r0;
           const bool take = key0 + r >= take_from && key0 + r < to && (RPP * k < 8 ? blk : blk2) >= 0;
-          x[grp * (16 / RPP) + k] =
-              take ? __ldg(reinterpret_cast<const uint4*>(pool + ((RPP * k < 8 ? slot0 : slot1) + r) * row_bytes + head_bytes) + c0)
-                   : make_uint4(0u, 0u, 0u, 0u);
+          const uint8_t* src = pool + (take ? ((RPP * k < 8 ? slot0 : slot1) + r) * row_bytes + head_bytes : 0);
+          x[grp * (16 / RPP) + k] = __ldg(reinterpret_cast<const uint4*>(src) + c0);
+          taken |= (take ? 1u : 0u) << (grp * (16 / RPP) + k);
         }
       }
       if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
     };
-    auto store = [&](const uint4 (&x)[CPR]) {
+    auto store = [&](const uint4 (&x)[CPR], uint32_t taken) {
       uint8_t* dst = ring + in.stage * S::kTileBytes + ((2 * c0) >> 3) * (kKeys * 128);
 #pragma unroll
       for (int k = 0; k < CPR; ++k) {
         const int rr = 32 * w + RPP * k + r0;
-        const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+        const uint32_t keep = taken >> k & 1u ? 0xFFFFFFFFu : 0u, u[4] = {x[k].x & keep, x[k].y & keep, x[k].z & keep, x[k].w & keep};
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<uint4*>(dst + rr * 128 + ((((2 * c0 + e) & 7) ^ (rr & 7)) << 4)) =
@@ -586,14 +599,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[in.stage]);
     };
-    if (steps > 0) load(0, codes[0]);
+    if (steps > 0) load(0, codes[0], taken[0]);
     for (int n = 0; n < 2 * steps && ok; n += 2) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (n + h + 1 < 2 * steps) load(n + h + 1, codes[h ^ 1]);
+        if (n + h + 1 < 2 * steps) load(n + h + 1, codes[h ^ 1], taken[h ^ 1]);
         if (n + h >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
         if (!ok) break;
-        store(codes[h]);
+        store(codes[h], taken[h]);
         in.next();
       }
     }
@@ -657,8 +670,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
       cp_async_commit();
       in.next();
-      cp_async_wait<kLag>();
-      if (announced + kLag <= n) announce();
+      if (n == 0) {  // the first keys are waited for by everyone
+        cp_async_wait<0>();
+        announce();
+      } else {
+        cp_async_wait<kLag>();
+        if (announced + kLag <= n) announce();
+      }
     }
     cp_async_wait<0>();
     while (ok && announced < 2 * steps) announce();
@@ -733,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_rows<KIND, D, CAP, SLOPED>(a, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
+    softmax_rows<KIND, D, CAP, SLOPED>(a, at, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
                           started, flags);
   }
   __syncwarp();
@@ -742,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (warp == 12) {
     (void)mbar_wait(drained, 0u);  // every product issued is complete before tensor memory is freed
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    free_tmem();
   }
 }
 
