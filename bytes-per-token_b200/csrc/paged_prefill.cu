@@ -8,8 +8,8 @@
 // rows (row = token * rep + head), so every key and value brought in serves all of them; a row carries its own interval
 // [lo, hi), and a tile of rows visits only the keys between its smallest lo and largest hi.
 //
-// Heads of 64 and 128 take csrc/paged_prefill_tc.cu, but for int8 pages. The kernel here serves those (a scale per key on the
-// scores and the values) and heads of 256. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. Where there
+// Every format but int8 takes csrc/paged_prefill_tc.cu. The kernel here serves int8 pages, whose scale per key goes on the
+// scores and on the probabilities. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. Where there
 // are few tiles, each takes several CTAs, with a part of its keys each; a second kernel, launched dependently, joins them.
 #include "paged_prefill.cuh"
 
@@ -368,12 +368,12 @@ struct Plan {
 
 Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int kind, int64_t tokens) {
   Plan p;
-  p.tc = kind != BPT_KV_INT8 && D <= 128;
+  p.tc = kind != BPT_KV_INT8;
   p.rows = p.tc ? kPrefillTcRows : kRows;
   p.tiles = T * (Hq / Hkv) / p.rows + B;
-  // Fewer CTAs than fill the GPU (one per SM on the tensor-core kernel, two of the other): each tile's keys in parts
-  // of at least 256 until there are.
-  const int64_t ctas = p.tiles * Hkv, want = (p.tc ? 1 : 2) * int64_t(num_sms());
+  // Fewer CTAs than fill the GPU (two per SM, one of heads of 256 on the tensor-core kernel): each tile's keys in parts of at
+  // least 256 until there are.
+  const int64_t ctas = p.tiles * Hkv, want = (p.tc && D == 256 ? 1 : 2) * int64_t(num_sms());
   p.n_splits = std::max<int64_t>(std::min(want / ctas, (tokens + 255) / 256), 1);
   p.split = ((tokens + p.n_splits - 1) / p.n_splits + 127) / 128 * 128;
   return p;

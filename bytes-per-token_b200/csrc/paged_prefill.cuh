@@ -29,7 +29,7 @@ struct PrefillArgs {
   float* part_lse;  // [tiles, Hkv, n_splits, rows], base 2
 };
 
-constexpr int kPrefillTcRows = 256;  // packed rows per CTA of the tensor-core kernel
+constexpr int kPrefillTcRows = 128;  // packed rows per CTA of the tensor-core kernel
 int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream);
 
 // A tile of packed rows (token * rep + head) of one sequence.

@@ -1,23 +1,30 @@
-// Prefill attention on the 5th-generation tensor cores (tcgen05, sm_100a only), for head dims 64 and 128: the same
-// operation, rows, intervals and parts as csrc/paged_prefill.cu.
+// Prefill attention on the 5th-generation tensor cores (tcgen05, sm_100a only): the same operation, rows, intervals and parts
+// as csrc/paged_prefill.cu.
 //
-// A CTA takes 256 packed rows (token * rep + head) of one KV head as two tiles of 128 and walks their keys 128 at a time:
-//   S = Q K^T    both operands in shared memory (128-byte swizzle), fp32 S in tensor memory;
-//   P = 2^(s - m) rounded to the pages' 16-bit type over S's own columns in tensor memory;
+// A CTA takes a tile of 128 packed rows (token * rep + head) of one KV head and walks their keys 64 at a time:
+//   S = Q K^T    both operands in shared memory (128-byte swizzle), fp32 S in tensor memory, two buffers of 64 columns;
+//   P = 2^(s - m) rounded to 16 bits, over the S that it came from;
 //   O += P V     P from tensor memory, V as it lies in its pages ([key][dim], the transposed operand form), fp32 O in tensor
 //                memory.
-// Four warpgroups: two do the softmax, each of one tile, a thread per row (so neither maximum nor sum crosses threads); one
-// brings pages into a ring of shared-memory stages, K and V of a step in stages of their own, by cp.async (rows of any page
-// size; keys that are not visible become zeros); of the last, one thread issues the XX
+// Two warpgroups. One does the softmax, a thread per row, so that neither maximum nor sum crosses threads. Of the other, one
+// warp issues the products and the rest bring pages into a ring of shared-memory stages (K and V of a step in stages of their
+// own): 16-bit pages as TMA boxes, one warp, a box per page and 64 dims, pages past the visible keys out of the map's range
+// and so zero; E4M3 pages through registers, where the codes become f16. While the softmax takes a step's powers, the tensor
+// cores take the products of the step before and the scores of the next. At heads of 64 and 128 two CTAs share an SM, so that
+// one's loads, waits and stores run under the other's powers.
 //
-// A row's m is the true maximum of its first 64 keys and moves only when the sum of 2^(s - m) over 64 keys passes 2^15: until then
-// every P is below 2^15, which both 16-bit types hold, and is divided by the sum of the same powers, so nothing is lost by
-// an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
+// A row's m is the true maximum of the first step that it sees and moves only when a step's sum of 2^(s - m) passes 2^15: until
+// then every P is below 2^15, which both 16-bit types hold, and is divided by the sum of the same powers, so nothing is lost
+// by an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
 // times per row, if at all.
 //
 // Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
 // and the CTA still awaits its copies and products, frees its tensor memory and returns.
 #define BPT_WHOLE_PROGRAM  // compiled without relocatable device code
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cstring>
 #include <type_traits>
 
 #include "paged_prefill.cuh"
@@ -25,28 +32,28 @@
 namespace bpt {
 namespace {
 
-constexpr int kThreads = 512;     // warpgroups: softmax of tile 0, softmax of tile 1, producer, matrix products
-constexpr int kTileRows = 128;
-constexpr int kRows = 2 * kTileRows;
+constexpr int kThreads = 256;  // warpgroups: softmax; producers (warps 4-6) and products (warp 7)
+constexpr int kRows = 128;
 static_assert(kRows == kPrefillTcRows, "the tiles that the caller counts");
-constexpr int kKeys = 128;        // per step
-constexpr int kSoftmaxRegs = 200;  // 2 x 128 x 200 + 2 x 128 x 56 = 512 x 128: the split of the registers at launch
-constexpr int kOtherRegs = 56;
+constexpr int kKeys = 64;  // per step
 constexpr int kLaunchRegs = 128;
-static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
-constexpr int kFlagSteps = 16;     // steps whose bad-block flags are kept (the ring runs at most 5 steps ahead)
+constexpr int kFlagSteps = 16;       // steps whose bad-block flags are kept (the ring runs at most 4 steps ahead)
 constexpr float kMostSum = 32768.f;  // a step's sum of powers beyond which a row's maximum moves
 
 template <int KIND, int D>
 struct TcShape {
   static constexpr int kRowBytes = D * kElemBytes<KIND>;  // a key's row in its page
-  static constexpr int kTileBytes = kTileRows * D * 2;  // a Q tile; a K or V stage
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kQ = 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 18;  // an even number: the flags behind them start on 16 bytes
-  static constexpr int kSmem = 1024 + kQ + kStages * kTileBytes + kBars * 8 + kFlagSteps * 16 + 64;
-  static constexpr uint32_t kO = 256;     // columns: S0, S1 at 0, 128; O0, O1 at 256, 256 + D
-  static_assert(256 + 2 * D <= 512, "tensor memory");
+  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kStage = kKeys * D * 2;
+  static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
+  static constexpr int kBars = 2 * kStages + 10;  // an even number: what follows them starts on 16 bytes
+  static constexpr int kSmem = kQ + kStages * kStage + kBars * 8 + kFlagSteps * 4 + 16;
+  static_assert(D == 256 || kSmem <= 113 * 1024, "two CTAs per SM");
+  static constexpr int kProducers = kIs16<KIND> ? 1 : 3;  // warps
+  // setmaxnreg: 128 threads x (softmax + other) = 256 x the launch's 128
+  static constexpr int kSoftmaxRegs = kIs16<KIND> ? 200 : 184, kOtherRegs = 256 - kSoftmaxRegs;
+  static constexpr uint32_t kO = 128;                             // columns: S at 0 and 64, O from 128
+  static constexpr uint32_t kColumns = D == 256 ? 512 : 256;  // of tensor memory
 };
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
@@ -146,7 +153,7 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       : "memory");
 }
 
-// Item n of the ring (K of step n / 2 where n is even, V where odd): its stage and the parity of the lap it fills.
+// A place in the ring: its stage and the parity of the lap that fills it.
 template <int STAGES>
 struct Item {
   int stage = 0;
@@ -158,6 +165,15 @@ struct Item {
     }
   }
 };
+
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int dim, int head, int token, int block,
+                                        uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(head), "r"(token), "r"(block), "r"(smem_u32(bar))
+      : "memory");
+}
 
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   float2 d;
@@ -171,20 +187,19 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   return d;
 }
 
-// What a softmax warpgroup does for tile i: its queries into shared memory, then every step's maximum, probabilities and
-// sum, and at the end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
+// What the softmax warpgroup does: the tile's queries into shared memory, then every step's probabilities and sum, and at the
+// end its rows of O (or of a part) to memory. Thread = row = lane of tensor memory.
 template <int KIND, int D, bool CAP, bool SLOPED>
 __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt& at, const RowAt& row, int hk, int sp, int parts,
-                                             int from, int first, int last, int i, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
-                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
-                                             uint64_t* started, const uint32_t* flags) {
+                                             int from, int steps, uint32_t tmem, uint8_t* smem, uint64_t* q_full,
+                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done, const uint32_t* flags) {
   using S = TcShape<KIND, D>;
-  const int r = threadIdx.x & 127, warp = r >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = threadIdx.x;
   float q_unit = 1.f;
   {
     // 32 / CPR rows per pass of the warp, a row's 16-byte chunks side by side
     constexpr int CPR = D / 8, RPP = 32 / CPR;
-    uint8_t* tile = smem + i * S::kTileBytes;
+    uint8_t* tile = smem;
     const int c = lane % CPR;
     uint4 x[CPR];
     // (loads without conditions, so that all are in flight at once: rows that are none read the tile's first and become zeros)
@@ -226,32 +241,30 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
 #pragma unroll
     for (int k = 0; k < CPR; ++k) {
       const int rr = 32 * warp + RPP * k + lane / CPR;
-      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kTileRows * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[k];
+      *reinterpret_cast<uint4*>(tile + (c >> 3) * (kRows * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[k];
     }
     fence_proxy_async_shared();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&q_full[i]);
+    if (lane == 0) mbar_arrive(q_full);
   }
   const float raw = a.sm_scale * a.src.k_scale * q_unit;  // a product as a score
   const float mul = CAP ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
   const float cap_out = a.softcap * kLog2e;
   const float mul_now = CAP || SLOPED ? 1.f : mul;  // what is left to multiply once a product has its shape
   const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
-  const uint32_t lanes = uint32_t(32 * warp) << 16;
-  const uint32_t s_at = tmem + lanes + i * 128, o_at = tmem + lanes + S::kO + i * D;
+  const uint32_t lanes = uint32_t(32 * warp) << 16, o_at = tmem + lanes + S::kO;
 
   float m = -INFINITY;  // the maximum in use
   float l = 0.f;
-  uint32_t n = 0;
   bool ok = true;
-  for (int j = first; j < last; ++j, ++n) {
+  for (int j = 0; j < steps; ++j) {
     const int key0 = from + j * kKeys;
-    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i], n & 1u));
+    const uint32_t s_at = tmem + lanes + 64 * (j & 1), phase = (j >> 1) & 1;
+    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], phase));
     if (!ok) break;
-    if (i == 0 && n == 0 && lane == 0) mbar_arrive(started);
-    const uint4 bad = *reinterpret_cast<const uint4*>(flags + (j & (kFlagSteps - 1)) * 4);
-    const bool any_bad = (bad.x | bad.y | bad.z | bad.w) != 0u;
-    const bool masked = any_bad || key0 < all_lo || key0 + kKeys > all_hi;
+    tc_fence_after();
+    const uint32_t bad = flags[j & (kFlagSteps - 1)];
+    const bool masked = bad != 0u || key0 < all_lo || key0 + kKeys > all_hi;
     // Columns c .. c + 31 of S, as scores but for the factor mul_now.
     auto shape = [&](int c, uint32_t* x, auto with_mask) {
       if constexpr (CAP) {
@@ -268,95 +281,86 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
       }
       if constexpr (decltype(with_mask)::value) {
         const int below = row.lo - key0 - c, above = row.hi - key0 - c;
-        const uint32_t w = c == 0 ? bad.x : c == 32 ? bad.y : c == 64 ? bad.z : bad.w;
+        const uint32_t w = bad >> (c >> 3);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           if (e < below || e >= above || (w >> (e >> 3) & 1u)) x[e] = 0xFF800000u;
       }
     };
-    // The step's keys in halves h: P = 2^(s - m), rounded to 16 bits (as any operand of these matrix instructions), and the
-    // fp32 sum of what was rounded. P V of the first half runs while the powers of the second are taken.
+    // P = 2^(s - m), rounded to 16 bits (as any operand of these matrix instructions), and the fp32 sum of what was rounded.
+    uint32_t p[32];
+    auto powers = [&](float off, auto with_mask) {
+      float2 sum = make_float2(0.f, 0.f);
+      uint32_t x[64];
+      tmem_load64(s_at, x);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * i + 1], n & 1u));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t p[32];
-      auto powers = [&](float off, auto with_mask) {
-        float2 sum = make_float2(0.f, 0.f);
-        uint32_t x[64];
-        tmem_load64(s_at + 64 * h, x);
+      for (int k = 0; k < 2; ++k) {
+        shape(32 * k, x + 32 * k, with_mask);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          shape(64 * h + 32 * k, x + 32 * k, with_mask);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 y = ffma2(make_float2(__uint_as_float(x[32 * k + 2 * e]), __uint_as_float(x[32 * k + 2 * e + 1])),
-                                   make_float2(mul_now, mul_now), make_float2(-off, -off));
-            const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-            sum = fadd2(sum, z);
-            p[16 * k + e] = pack2<KIND>(z.x, z.y);
-          }
+        for (int e = 0; e < 16; ++e) {
+          const float2 y = ffma2(make_float2(__uint_as_float(x[32 * k + 2 * e]), __uint_as_float(x[32 * k + 2 * e + 1])),
+                                 make_float2(mul_now, mul_now), make_float2(-off, -off));
+          const float2 z = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          sum = fadd2(sum, z);
+          p[16 * k + e] = pack2<KIND>(z.x, z.y);
         }
-        return sum.x + sum.y;
-      };
-      // a row that has met no key yet meets some in this half: its first maximum
-      const int half0 = key0 + 64 * h;
-      const bool fresh = m == -INFINITY && row.lo < half0 + 64 && row.hi > half0;
-      float sum = 0.f;
-      bool looked = false, known = !__all_sync(0xffffffffu, fresh);  // some row has a maximum to begin with
-      for (;;) {
-        // (two bodies: as one, its masks would be taken on every step)
-        if (known) {
-          const float off = m == -INFINITY ? 0.f : m;
-          sum = masked ? powers(off, std::true_type()) : powers(off, std::false_type());
-        }
-        const bool moves = fresh ? m == -INFINITY : !(sum <= kMostSum);
-        if (looked || !__any_sync(0xffffffffu, moves)) break;
-        // a first half-step, and a few later ones: the row's maximum is looked up and moves
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 64 * h; c < 64 * h + 64; c += 32) {
-          uint32_t x[32];
-          tmem_load32(s_at + c, x);
-          shape(c, x, std::true_type());
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
-        }
-        top *= mul_now;
-        float shrink = 1.f;
-        if (moves && top > m) {
-          shrink = exp2_approx(m - top);
-          m = top;
-          l *= shrink;
-        }
-        if (n > 0 || h > 0) {  // the half-step before this one is in O
-          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * i + (h ^ 1)], (h ? n : n - 1) & 1u));
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_load32(o_at + c, o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-            tmem_store32(o_at + c, o);
-          }
-        }
-        known = looked = true;
       }
-      if (!ok) break;
-      l += sum;
-      tmem_store32(s_at + 64 * h, p);
-      tmem_wait_store();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+      return sum.x + sum.y;
+    };
+    // a row that has met no key yet meets some in this step: its first maximum
+    const bool fresh = m == -INFINITY && row.lo < key0 + kKeys && row.hi > key0;
+    float sum = 0.f;
+    bool looked = false, known = !__all_sync(0xffffffffu, fresh);  // some row has a maximum to begin with
+    for (;;) {
+      // (two bodies: as one, its masks would be taken on every step)
+      if (known) {
+        const float off = m == -INFINITY ? 0.f : m;
+        sum = masked ? powers(off, std::true_type()) : powers(off, std::false_type());
+      }
+      const bool moves = fresh ? m == -INFINITY : !(sum <= kMostSum);
+      if (looked || !__any_sync(0xffffffffu, moves)) break;
+      // a first step, and a few later ones: the row's maximum is looked up and moves
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < kKeys; c += 32) {
+        uint32_t x[32];
+        tmem_load32(s_at + c, x);
+        shape(c, x, std::true_type());
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+      }
+      top *= mul_now;
+      float shrink = 1.f;
+      if (moves && top > m) {
+        shrink = exp2_approx(m - top);
+        m = top;
+        l *= shrink;
+      }
+      if (j > 0) {  // the step before this one is in O
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1u));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_load32(o_at + c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+          tmem_store32(o_at + c, o);
+        }
+      }
+      known = looked = true;
     }
     if (!ok) break;
+    l += sum;
+    tmem_store32(s_at, p);
+    tmem_wait_store();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&p_full[j & 1]);
   }
-  if (i == 0 && n == 0 && lane == 0) mbar_arrive(started);  // (a tile that sees no key)
-  if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[2 * i + 1], (n - 1) & 1u));
+  const int n = steps;
+  if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(n - 1) & 1], ((n - 1) >> 1) & 1u));
   tc_fence_after();
   const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
   const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
@@ -368,10 +372,10 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
     if constexpr (kIs16<KIND>) return pack2<KIND>(x, y);
     return bf16 ? pack2<BPT_KV_BF16>(x, y) : pack2<BPT_KV_F16>(x, y);
   };
-  uint8_t* stage = smem + i * S::kTileBytes + warp * (32 * 2 * D);
+  uint8_t* stage = smem + warp * (32 * 2 * D);
   const int c = lane % CPR;
   const int64_t out0 = (int64_t(at.token0 + at.row0 / a.rep) * a.Hq + hk * a.rep) * (2 * D);  // of the tile's first row, in bytes
-  const int64_t part0 = ((tile * a.n_splits + sp) * kRows + i * kTileRows + 32 * warp) * (4 * D);  // of the warp's first row
+  const int64_t part0 = ((tile * a.n_splits + sp) * kRows + 32 * warp) * (4 * D);  // of the warp's first row
 #pragma unroll 1
   for (int half = 0; half < (parts > 1 ? 2 : 1); ++half) {
 #pragma unroll
@@ -421,50 +425,53 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
     __syncwarp();
   }
   if (ok && parts > 1 && row.code >= 0)
-    a.part_lse[(tile * a.n_splits + sp) * kRows + i * kTileRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+    a.part_lse[(tile * a.n_splits + sp) * kRows + r] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
 }
 
 // CAP: scores are capped. SLOPED: they fall with distance, or their factor is not positive (a maximum of products is then no
 // maximum of scores).
 template <int KIND, int D, bool CAP, bool SLOPED>
-__global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillArgs a) {
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_prefill_tc_kernel(const PrefillArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using S = TcShape<KIND, D>;
   constexpr int NS = S::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + S::kQ;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * S::kTileBytes);
-  uint64_t* full = bars;             // [NS] a stage's rows have landed (one arrival per producer warp)
-  uint64_t* empty = full + NS;       // [NS] both tiles' products that read it are done
-  uint64_t* q_full = empty + NS;     // [2] a tile's queries are in shared memory
-  uint64_t* s_full = q_full + 2;     // [2][2] a tile's half-step of S is in tensor memory
-  uint64_t* p_full = s_full + 4;     // [2][2] a half of P is in tensor memory, O rescaled where needed
-  uint64_t* o_done = p_full + 4;     // [2][2] that half's P V is in O
-  uint64_t* drained = o_done + 4;    // all products are done
-  uint64_t* started = drained + 1;   // tile 0 has its first scores
-  uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps][4] bad blocks, a word per producer warp
-  int* range = reinterpret_cast<int*>(flags + kFlagSteps * 4);      // [2] lo, [2] hi of the tiles
-  uint32_t* slot = reinterpret_cast<uint32_t*>(range + 4);          // tensor-memory address
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * S::kStage);
+  uint64_t* full = bars;             // [NS] a stage's rows have landed (an arrival per producer warp)
+  uint64_t* empty = full + NS;       // [NS] the products that read it are done
+  uint64_t* q_full = empty + NS;     // the queries are in shared memory
+  uint64_t* s_full = q_full + 1;     // [2] S is in its buffer: the products' completion, and the issuing thread (which has
+                                     //     waited for the keys, and so seen their flags)
+  uint64_t* p_full = s_full + 2;     // [2] P is in its buffer, O rescaled where needed
+  uint64_t* o_done = p_full + 2;     // [2] that buffer's P V is in O
+  uint64_t* drained = o_done + 2;    // all products are done
+  uint64_t* edge = drained + 1;      // a stage whose rows are only partly visible has landed
+  uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps] a bit per 8 keys of a block out of range
+  int* range = reinterpret_cast<int*>(flags + kFlagSteps);          // the smallest lo, the largest hi
+  uint32_t* slot = reinterpret_cast<uint32_t*>(range + 2);          // tensor-memory address
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
   const int hk = blockIdx.y, sp = blockIdx.z;
 
+  if (smem_u32(smem) & 1023u) {  // (dynamic shared memory starts there: the kernel has no other)
+    if (tid == 0) record_error(kDevErrTimeout);
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 4);
-      mbar_init(&empty[i], 2);
+      mbar_init(&full[i], S::kProducers);
+      mbar_init(&empty[i], 1);
     }
+    mbar_init(q_full, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
-      for (int h = 0; h < 2; ++h) mbar_init(&s_full[2 * i + h], 2);  // the products' completion, and the issuing thread (whose own waits saw the flags)
-      mbar_init(&p_full[2 * i], 4);
-      mbar_init(&p_full[2 * i + 1], 4);
-      mbar_init(&o_done[2 * i], 1);
-      mbar_init(&o_done[2 * i + 1], 1);
-      range[i] = INT_MAX;
-      range[2 + i] = 0;
+      mbar_init(&s_full[i], 2);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
     }
-    mbar_init(drained, 2);
-    mbar_init(started, 4);
+    mbar_init(drained, 1);
+    mbar_init(edge, 1);
+    range[0] = INT_MAX;
+    range[1] = 0;
     fence_mbar_init();
   }
   pdl_launch_dependents();
@@ -479,19 +486,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   const int len = sequence_length(a, b, tid == 0 && hk == 0 && sp == 0);
   __syncthreads();
 
-  // the tiles' rows: thread r of a softmax warpgroup holds row r
+  // the tile's rows: thread r of the softmax warpgroup holds row r
   RowAt row{-1, -1, -1, 0, 0, 0, 0.f};
-  if (wg < 2) {
-    row = row_at(a, at, at.row0 + wg * kTileRows + (tid & 127), hk, len);
+  if (wg == 0) {
+    row = row_at(a, at, at.row0 + tid, hk, len);
     const bool any = row.hi > row.lo;
     const int lo = __reduce_min_sync(0xffffffffu, any ? row.lo : INT_MAX);
     const int hi = __reduce_max_sync(0xffffffffu, any ? row.hi : 0);
     if (lane == 0 && hi > 0) {
-      atomicMin(&range[wg], lo);
-      atomicMax(&range[2 + wg], hi);
+      atomicMin(&range[0], lo);
+      atomicMax(&range[1], hi);
     }
-  } else if (warp == 12) {  // all of tensor memory (one CTA per SM)
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+  } else if (warp == 7) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(S::kColumns)
+                 : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -499,265 +507,237 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   tc_fence_after();
   const uint32_t tmem = *slot;
   auto free_tmem = [&]() {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
   };
-  const int lo = min(range[0], range[1]), hi = max(range[2], range[3]);
-  const int base = lo == INT_MAX ? 0 : lo & ~15;
+  const int lo = range[0], hi = range[1];
+  const int base = lo == INT_MAX ? 0 : lo & ~(kKeys - 1);
   const int parts = hi > base ? min(a.n_splits, (hi - base + a.split - 1) / a.split) : 0;
   if (a.n_splits > 1 && sp == 0 && tid == 0) a.part_count[tile] = parts;
   if (sp >= max(parts, 1)) {
-    if (warp == 12) free_tmem();
+    if (warp == 7) free_tmem();
     return;
   }
   const int from = base + sp * a.split;
   const int to = parts == 0 ? from : sp == parts - 1 ? hi : from + a.split;
   const int steps = (to - from + kKeys - 1) / kKeys;
-  // the steps that tile i has keys in: first[i] <= j < last[i]
-  int first[2], last[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int l = max(range[i], from), h = min(range[2 + i], to);
-    first[i] = h > l ? (l - from) / kKeys : 0;
-    last[i] = h > l ? (h - from + kKeys - 1) / kKeys : 0;
-  }
-  if (wg == 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    // ---- producer: warp w brings rows 32 w .. 32 w + 31 of every stage, two groups of 16 keys
-    const int w = warp & 3;
-    const int32_t* table = a.src.block_table + int64_t(b) * a.src.bt_stride;
-    const int64_t row_bytes = int64_t(a.src.Hkv) * S::kRowBytes, head_bytes = int64_t(hk) * S::kRowBytes;
-    const bool two = a.src.bs_log2 == 3;
-    const int take_from = max(from, lo);
-    int held = -1, held2 = -1;  // lane n: the block(s) of group n of the current 16 steps
-    auto block_at = [&](int key) -> int {
-      if (key >= to) return -1;
-      const int blk = table[key >> a.src.bs_log2];
-      if (blk < 0 || blk >= a.src.num_blocks) {
-        record_error(kDevErrBlockIndex);
-        return -1;
-      }
-      return blk;
-    };
-    auto hold = [&](int j) {
-      const int key = from + kKeys * (j + (lane >> 1)) + 32 * w + 16 * (lane & 1);
-      held = block_at(key);
-      if (two) held2 = block_at(key + 8);
-    };
-    // The blocks of group grp of step j (one twice where pages are longer than 8), and what the table names wrongly.
-    auto blocks_of = [&](int j, int grp, int& blk, int& blk2, uint32_t& bad) {
-      const int key0 = from + kKeys * j + 32 * w + 16 * grp;
-      blk = __shfl_sync(0xffffffffu, held, 2 * (j & 15) + grp);
-      blk2 = two ? __shfl_sync(0xffffffffu, held2, 2 * (j & 15) + grp) : blk;
-      bad |= (blk < 0 && key0 < to ? 1u : 0u) << (2 * grp) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u) << (2 * grp);
-    };
-    if constexpr (!kIs16<KIND>) {
-    // Codes go through registers: 16 codes a load, an f16 each into the stage. An item's loads are issued an item ahead.
-    constexpr int CPR = D / 16, RPP = 32 / CPR;  // 16-code chunks of a row; rows per pass of the warp
-    const int r0 = lane / CPR, c0 = lane % CPR;
-    uint4 codes[2][CPR];
-    uint32_t taken[2];
-    bool ok = true;
-    Item<NS> in;
-    // (loads without conditions, so that all are in flight at once; what is not taken reads the pool's start and is dropped)
-    auto load = [&](int n, uint4 (&x)[CPR], uint32_t& taken) {
-      taken = 0;
-      const int j = n >> 1;
-      if ((n & 1) == 0 && (j & 15) == 0) hold(j);
-      const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
-      uint32_t bad = 0;
-#pragma unroll
-      for (int grp = 0; grp < 2; ++grp) {
-        int blk, blk2;
-        blocks_of(j, grp, blk, blk2, bad);
-        const int key0 = from + kKeys * j + 32 * w + 16 * grp;
-        const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
-        const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
-#pragma unroll
-        for (int k = 0; k < 16 / RPP; ++k) {
-          const int r = RPP * k + r0;
-          const bool take = key0 + r >= take_from && key0 + r < to && (RPP * k < 8 ? blk : blk2) >= 0;
-          const uint8_t* src = pool + (take ? ((RPP * k < 8 ? slot0 : slot1) + r) * row_bytes + head_bytes : 0);
-          x[grp * (16 / RPP) + k] = __ldg(reinterpret_cast<const uint4*>(src) + c0);
-          taken |= (take ? 1u : 0u) << (grp * (16 / RPP) + k);
+  // Ring items in the order that the products take them: K 0, K 1, then V j, K j + 2 for every step j.
+  const int items = 2 * steps;
+  auto step_of = [&](int n) { return n < 2 ? n : n & 1 ? (n + 1) >> 1 : (n - 2) >> 1; };  // (n odd from 3 on: K)
+  auto is_v = [&](int n) { return n >= 2 && (n & 1) == 0; };
+
+  if (wg == 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
+    if (warp < 4 + S::kProducers) {
+      // ---- producers
+      const int w = warp - 4;
+      const int32_t* table = a.src.block_table + int64_t(b) * a.src.bt_stride;
+      const int take_from = max(from, lo);
+      auto block_at = [&](int key) -> int {  // -1: none is visible there, -2: the table names one out of range
+        if (key >= to) return -1;
+        const int blk = table[key >> a.src.bs_log2];
+        if (blk < 0 || blk >= a.src.num_blocks) {
+          record_error(kDevErrBlockIndex);
+          return -2;
         }
-      }
-      if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
-    };
-    auto store = [&](const uint4 (&x)[CPR], uint32_t taken) {
-      uint8_t* dst = ring + in.stage * S::kTileBytes + ((2 * c0) >> 3) * (kKeys * 128);
-#pragma unroll
-      for (int k = 0; k < CPR; ++k) {
-        const int rr = 32 * w + RPP * k + r0;
-        const uint32_t keep = taken >> k & 1u ? 0xFFFFFFFFu : 0u, u[4] = {x[k].x & keep, x[k].y & keep, x[k].z & keep, x[k].w & keep};
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<uint4*>(dst + rr * 128 + ((((2 * c0 + e) & 7) ^ (rr & 7)) << 4)) =
-              make_uint4(codes_to_f16<KIND>(u[2 * e] & 0xFFFFu), codes_to_f16<KIND>(u[2 * e] >> 16),
-                         codes_to_f16<KIND>(u[2 * e + 1] & 0xFFFFu), codes_to_f16<KIND>(u[2 * e + 1] >> 16));
-      }
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[in.stage]);
-    };
-    if (steps > 0) load(0, codes[0], taken[0]);
-    for (int n = 0; n < 2 * steps && ok; n += 2) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (n + h + 1 < 2 * steps) load(n + h + 1, codes[h ^ 1], taken[h ^ 1]);
-        if (n + h >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
-        if (!ok) break;
-        store(codes[h], taken[h]);
-        in.next();
-      }
-    }
-    } else {
-    constexpr int CPR = D / 8;  // 16-byte chunks of a row
-    constexpr int kLag = 2;     // items in flight before the oldest is announced
-    Item<NS> in, out;
-    bool ok = true;
-    int announced = 0;
-    auto announce = [&]() {  // the oldest item's copies of this warp have landed: make them the tensor cores' to read
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[out.stage]);
-      out.next();
-      ++announced;
-    };
-    for (int n = 0; n < 2 * steps && ok; ++n) {
-      const int j = n >> 1;
-      if (n >= NS) {
-        // before waiting for a stage, announce what is in flight: the products that free it may need just that
-        if (!__all_sync(0xffffffffu, mbar_test(&empty[in.stage], in.lap ^ 1u))) {
-          cp_async_wait<0>();
-          while (announced < n) announce();
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
-          if (!ok) break;
-        }
-      }
-      if ((n & 1) == 0) {
-        if ((j & 15) == 0) hold(j);
-      }
-      const uint8_t* pool = (n & 1) ? a.src.v_pool : a.src.k_pool;
-      const uint32_t dst = smem_u32(ring + in.stage * S::kTileBytes);
-      uint32_t bad = 0;
-      // this lane's chunk of the first rows of each group, and its place: rows 32 / CPR further on are constants away
-      const int r0 = lane / CPR, c0 = lane % CPR;
-      const uint32_t dst0 = dst + (c0 >> 3) * (kKeys * 128) + (32 * w + r0) * 128, x0 = uint32_t((c0 & 7) ^ r0);
-#pragma unroll
-      for (int grp = 0; grp < 2; ++grp) {
-        const int key0 = from + kKeys * j + 32 * w + 16 * grp;
-        int blk, blk2;
-        blocks_of(j, grp, blk, blk2, bad);
-        const int64_t slot0 = (int64_t(max(blk, 0)) << a.src.bs_log2) + (key0 & ((1 << a.src.bs_log2) - 1));
-        const int64_t slot1 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot0;
-        constexpr int STEP = 32 / CPR;  // rows per pass of the warp
-        const uint8_t* src0 = pool + (slot0 + r0) * row_bytes + head_bytes + c0 * 16;
-        const uint8_t* src1 = pool + (slot1 + r0) * row_bytes + head_bytes + c0 * 16;
-        const bool whole = key0 >= take_from && key0 + 16 <= to && blk >= 0 && blk2 >= 0;
-#pragma unroll
-        for (int k = 0; k < 16 / STEP; ++k) {
-          const uint32_t d = dst0 + (16 * grp + STEP * k) * 128 + ((x0 ^ uint32_t((STEP * k) & 7)) << 4);
-          const uint8_t* src = (STEP * k < 8 ? src0 : src1) + STEP * k * row_bytes;
-          if (whole) {
-            cp_async16(d, src);
+        return blk;
+      };
+      // A step's pages: 64 / page size of them (one where pages are longer). Lane i of a window holds page i mod per_step of
+      // step first + i / per_step; the next window is loaded while this one is in use.
+      const int page_log2 = min(a.src.bs_log2, 6), per_log2 = 6 - page_log2, window_log2 = 5 - per_log2;
+      auto window = [&](int first) {
+        return block_at(from + ((first + (lane >> per_log2)) << 6) + ((lane & ((1 << per_log2) - 1)) << page_log2));
+      };
+      int k_held = window(0), k_next = window(1 << window_log2), v_held = k_held, v_next = k_next;
+      // this lane's page (lane < pages) of step j
+      auto page_of = [&](int j, bool v) {
+        const int in = j & ((1 << window_log2) - 1);
+        if (in == 0 && j > 0) {
+          if (v) {
+            v_held = v_next;
+            v_next = window(j + (1 << window_log2));
           } else {
-            const int key = key0 + STEP * k + r0;
-            const bool take = key >= take_from && key < to && (STEP * k < 8 ? blk : blk2) >= 0;
-            cp_async16(d, take ? src : pool, take);
+            k_held = k_next;
+            k_next = window(j + (1 << window_log2));
           }
         }
-      }
-      if ((n & 1) == 0 && lane == 0) flags[(j & (kFlagSteps - 1)) * 4 + w] = bad;
-      cp_async_commit();
-      in.next();
-      if (n == 0) {  // the first keys are waited for by everyone
-        cp_async_wait<0>();
-        announce();
-      } else {
-        cp_async_wait<kLag>();
-        if (announced + kLag <= n) announce();
-      }
-    }
-    cp_async_wait<0>();
-    while (ok && announced < 2 * steps) announce();
-    }
-  } else if (wg == 3) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp < 14) {
-      // ---- matrix products: a warp per tile; the whole warp waits, one of its threads issues. A step's keys go in halves:
-      // S of the next step's half overwrites the columns of this step's half as soon as its P V has been issued.
-      constexpr uint32_t id_s = tc_idesc<KIND>(kTileRows, kKeys / 2, false), id_o = tc_idesc<KIND>(kTileRows, D, true);
-      const int i = warp - 12, begin = i ? first[1] : first[0], end = i ? last[1] : last[0];
-      const uint64_t q_desc = desc_along(smem_u32(smem + i * S::kTileBytes)), k_desc = desc_along(smem_u32(ring)),
-                     v_desc = desc_across(smem_u32(ring), kKeys * 128);
-      const uint32_t s_at = tmem + i * 128, o_at = tmem + S::kO + i * D;
-      Item<NS> item;  // the ring's next item: K of step j on entering step j = 0, else V of step j - 1, then K of step j
-      uint32_t n = 0;  // steps whose Q K^T has been issued
+        return __shfl_sync(0xffffffffu, v ? v_held : k_held, (in << per_log2) + (lane & ((1 << per_log2) - 1)));
+      };
+      // the bits of a step's 8-key units whose block is out of range
+      auto flag = [&](int j, int blk) {
+        const uint32_t wrong = __ballot_sync(0xffffffffu, blk == -2) & ((1u << (1 << per_log2)) - 1u);
+        uint32_t bits = 0;
+        if (wrong)
+          for (int u = 0; u < 8; ++u) bits |= (wrong >> (u >> (page_log2 - 3)) & 1u) << u;
+        if (lane == 0) flags[j & (kFlagSteps - 1)] = bits;
+      };
+      Item<NS> in;
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
-      if (end > begin) wait(&q_full[i], 0u);
-      // Tile 1 starts half a step late, and stays so: in step, both tiles would take powers at once and then wait at once.
-      if (i == 1 && ok && end > begin) wait(started, 0u);
-      for (int j = 0; j <= steps && ok; ++j) {
-        const int v_stage = item.stage;
-        if (j > 0) {
-          wait(&full[v_stage], item.lap);
+      if constexpr (kIs16<KIND>) {
+        uint32_t edges = 0;
+        const int pages = 1 << per_log2, page = lane & (pages - 1), part = lane >> per_log2;  // a box: a page's 64 dims
+        const int head_dim0 = 64 * part, box_rows = 1 << page_log2;
+        const bool boxed = part < D / 64;
+        for (int n = 0; n < items; ++n) {
+          if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
           if (!ok) break;
-          item.next();
-        }
-        const int k_stage = item.stage;
-        if (j < steps) {
-          wait(&full[k_stage], item.lap);
-          if (!ok) break;
-          item.next();
-        }
-        const bool pv = j > begin && j <= end, qk = j >= begin && j < end;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (pv) wait(&p_full[2 * i + h], (n - 1) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            if (pv) {  // P V of step j - 1
-              const uint64_t vd = v_desc + uint32_t(v_stage * (S::kTileBytes >> 4) + h * (kKeys / 2 * 128 >> 4));
-#pragma unroll
-              for (int k = 0; k < kKeys / 32; ++k)
-                tc_mma_ts(o_at, s_at + 64 * h + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || h > 0 || j - 1 > begin ? 1u : 0u);
-              tc_commit(&o_done[2 * i + h]);
+          // (the last steps have no K after their V: items past steps - 1 are skipped by the order's tail)
+          const bool v = is_v(n) || n >= 2 * steps - 1;
+          const int j = n >= 2 * steps - 1 ? steps - 1 : step_of(n);
+          const int blk = page_of(j, v);
+          if (!v) flag(j, blk);
+          const int key0 = from + kKeys * j;
+          const bool partly = v && (key0 < take_from || key0 + kKeys > to);
+          uint64_t* bar = partly ? edge : &full[in.stage];
+          const uint32_t dst = smem_u32(ring + in.stage * S::kStage);
+          if (lane == 0) mbar_arrive_expect_tx(bar, S::kStage);
+          __syncwarp();
+          if (boxed)  // a page that is not there lies behind the pool: the box becomes zeros
+            tma_box(dst + part * (kKeys * 128) + page * (box_rows * 128), v ? &tm_v : &tm_k, head_dim0, hk,
+                    key0 & ((1 << a.src.bs_log2) - 1) & ~(box_rows - 1), blk >= 0 ? blk : int(a.src.num_blocks), bar);
+          if (partly) {  // values next to the visible ones may be anything: their rows become zeros, as P's columns are there
+            ok = __all_sync(0xffffffffu, mbar_wait(edge, edges & 1u));
+            ++edges;
+            if (!ok) break;
+            for (int i = lane; i < kKeys * (D / 8); i += 32) {
+              const int r = i / (D / 8), c = i % (D / 8);
+              if (key0 + r < take_from || key0 + r >= to)
+                *reinterpret_cast<uint4*>(ring + in.stage * S::kStage + (c >> 3) * (kKeys * 128) + r * 128 + (c & 7) * 16) =
+                    make_uint4(0u, 0u, 0u, 0u);
             }
-            if (qk) {  // Q K^T of step j
-              const uint64_t kd = k_desc + uint32_t(k_stage * (S::kTileBytes >> 4) + h * (kKeys / 2 * 128 >> 4));
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[in.stage]);
+          }
+          in.next();
+        }
+      } else {
+        // Codes go through registers: 16 codes a load, an f16 each into the stage. Warp w takes the slabs of 8 rows w, w + 3, ...;
+        // an item's loads are issued an item ahead, without conditions, so that all are in flight at once (what is not taken
+        // reads the pool's start and is dropped).
+        constexpr int CPR = D / 16, PER = CPR * 8 / 32, SLABS = 3;  // chunks of a row; a lane's chunks of a slab
+        const int64_t row_bytes = int64_t(a.src.Hkv) * S::kRowBytes, head_bytes = int64_t(hk) * S::kRowBytes;
+        uint4 codes[2][SLABS * PER];
+        uint32_t taken[2];
+        auto order = [&](int n, int& j, bool& v) {
+          v = is_v(n) || n >= 2 * steps - 1;
+          j = n >= 2 * steps - 1 ? steps - 1 : step_of(n);
+        };
+        auto load = [&](int n, uint4 (&x)[SLABS * PER], uint32_t& got) {
+          int j;
+          bool v;
+          order(n, j, v);
+          const int blk = page_of(j, v);
+          if (!v && w == 0) flag(j, blk);
+          const uint8_t* pool = v ? a.src.v_pool : a.src.k_pool;
+          const int key0 = from + kKeys * j;
+          got = 0;
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t at_k = (k & 3) * (32 >> 4), at_q = (k >> 2) * (kTileRows * 128 >> 4) + at_k;
-                tc_mma_ss(s_at + 64 * h, q_desc + at_q, kd + (k >> 2) * (kKeys * 128 >> 4) + at_k, id_s, k > 0 ? 1u : 0u);
-              }
-              tc_commit(&s_full[2 * i + h]);
-              mbar_arrive(&s_full[2 * i + h]);
+          for (int i = 0; i < SLABS; ++i) {
+            const int slab = w + 3 * i;
+            const int blk8 = __shfl_sync(0xffffffffu, blk, (slab & 7) >> (page_log2 - 3));
+            const int64_t slot0 = (int64_t(max(blk8, 0)) << a.src.bs_log2) + ((key0 + 8 * (slab & 7)) & ((1 << a.src.bs_log2) - 1));
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+              const int r = (lane + 32 * e) / CPR, c = (lane + 32 * e) % CPR, key = key0 + 8 * slab + r;
+              const bool take = slab < 8 && key >= take_from && key < to && blk8 >= 0;
+              const uint8_t* src = pool + (take ? (slot0 + r) * row_bytes + head_bytes : 0);
+              x[i * PER + e] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+              got |= (take ? 1u : 0u) << (i * PER + e);
             }
           }
+        };
+        auto store = [&](const uint4 (&x)[SLABS * PER], uint32_t got) {
+#pragma unroll
+          for (int i = 0; i < SLABS; ++i) {
+            if (w + 3 * i >= 8) break;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+              const int rr = 8 * (w + 3 * i) + (lane + 32 * e) / CPR, c = (lane + 32 * e) % CPR;
+              const uint4 v4 = x[i * PER + e];
+              const uint32_t keep = got >> (i * PER + e) & 1u ? 0xFFFFFFFFu : 0u;
+              const uint32_t u[4] = {v4.x & keep, v4.y & keep, v4.z & keep, v4.w & keep};
+              uint8_t* dst = ring + in.stage * S::kStage + ((2 * c) >> 3) * (kKeys * 128) + rr * 128;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ (rr & 7)) << 4)) =
+                    make_uint4(codes_to_f16<KIND>(u[2 * h] & 0xFFFFu), codes_to_f16<KIND>(u[2 * h] >> 16),
+                               codes_to_f16<KIND>(u[2 * h + 1] & 0xFFFFu), codes_to_f16<KIND>(u[2 * h + 1] >> 16));
+            }
+          }
+          fence_proxy_async_shared();
           __syncwarp();
+          if (lane == 0) mbar_arrive(&full[in.stage]);
+        };
+        if (items > 0) load(0, codes[0], taken[0]);
+        for (int n = 0; n < items && ok; n += 2) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (n + h + 1 < items) load(n + h + 1, codes[h ^ 1], taken[h ^ 1]);
+            if (n + h >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+            if (!ok) break;
+            store(codes[h], taken[h]);
+            in.next();
+          }
         }
-        if (!ok) break;
-        if (qk) ++n;
+      }
+    } else if (warp == 7) {
+      // ---- matrix products: the whole warp waits, one of its threads issues
+      constexpr uint32_t id_s = tc_idesc<KIND>(kRows, kKeys, false), id_o = tc_idesc<KIND>(kRows, D, true);
+      const uint64_t q_desc = desc_along(smem_u32(smem)), k_desc = desc_along(smem_u32(ring)),
+                     v_desc = desc_across(smem_u32(ring), kKeys * 128);
+      Item<NS> item;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      auto scores = [&](int j) {  // S = Q K^T of step j
+        wait(&full[item.stage], item.lap);
+        if (!ok) return;
+        tc_fence_after();
         if (elect_one()) {
-          if (j > 0) tc_commit(&empty[v_stage]);
-          if (j < steps) tc_commit(&empty[k_stage]);
+          const uint64_t kd = k_desc + uint32_t(item.stage * (S::kStage >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at_k = (k & 3) * (32 >> 4);
+            tc_mma_ss(tmem + 64 * (j & 1), q_desc + (k >> 2) * (kRows * 128 >> 4) + at_k, kd + (k >> 2) * (kKeys * 128 >> 4) + at_k,
+                      id_s, k > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[j & 1]);
+          mbar_arrive(&s_full[j & 1]);
+          tc_commit(&empty[item.stage]);
         }
         __syncwarp();
+        item.next();
+      };
+      if (steps > 0) wait(q_full, 0u);
+      if (steps > 0 && ok) scores(0);
+      if (steps > 1 && ok) scores(1);
+      for (int j = 0; j < steps && ok; ++j) {  // O += P V of step j, then S of step j + 2 over the P that it took
+        wait(&full[item.stage], item.lap);
+        wait(&p_full[j & 1], (j >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = v_desc + uint32_t(item.stage * (S::kStage >> 4));
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            tc_mma_ts(tmem + S::kO, tmem + 64 * (j & 1) + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || j > 0 ? 1u : 0u);
+          tc_commit(&o_done[j & 1]);
+          tc_commit(&empty[item.stage]);
+        }
+        __syncwarp();
+        item.next();
+        if (j + 2 < steps) scores(j + 2);
       }
       if (elect_one()) tc_commit(drained);
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_rows<KIND, D, CAP, SLOPED>(a, at, row, hk, sp, parts, from, first[wg], last[wg], wg, tmem, smem, q_full, s_full, p_full, o_done,
-                          started, flags);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+    softmax_rows<KIND, D, CAP, SLOPED>(a, at, row, hk, sp, parts, from, steps, tmem, smem, q_full, s_full, p_full, o_done, flags);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 7) {
     (void)mbar_wait(drained, 0u);  // every product issued is complete before tensor memory is freed
     tc_fence_after();
     free_tmem();
@@ -779,6 +759,24 @@ int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t strea
   }
   const int st = set_max_smem_once(kernel, S::kSmem, ready);
   if (st) return st;
+  CUtensorMap tm_k, tm_v;
+  memset(&tm_k, 0, sizeof(tm_k));
+  memset(&tm_v, 0, sizeof(tm_v));
+  if constexpr (kIs16<KIND>) {
+    auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+    if (!encode) return set_error(BPT_ERR_UNSUPPORTED, "paged prefill: the driver has no tensor-map encoder");
+    const cuuint64_t row = cuuint64_t(S::kRowBytes), token = row * a.src.Hkv, bs = cuuint64_t(1) << a.src.bs_log2;
+    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(a.src.Hkv), bs, cuuint64_t(a.src.num_blocks)};
+    const cuuint64_t strides[3] = {row, token, token * bs};
+    const cuuint32_t box[4] = {64, 1, cuuint32_t(std::min<cuuint64_t>(bs, kKeys)), 1}, ones[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = KIND == BPT_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; ++i) {
+      const CUresult res = encode(i ? &tm_v : &tm_k, type, 4, const_cast<uint8_t*>(i ? a.src.v_pool : a.src.k_pool), dims, strides,
+                                  box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (res != CUDA_SUCCESS) return set_error(BPT_ERR_INVALID, "paged prefill: tensor map: error %d", int(res));
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
   cfg.blockDim = dim3(kThreads);
@@ -789,7 +787,7 @@ int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t strea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_tc_kernel<KIND, D, CAP, SLOPED>, a);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_tc_kernel<KIND, D, CAP, SLOPED>, a, tm_k, tm_v);
   if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
   return BPT_OK;
 }
@@ -812,11 +810,15 @@ int take_prefill_tc_error() {
 }
 
 int prefill_tc(const PrefillArgs& a, int kind, int64_t tiles, int flags, cudaStream_t stream) {
-  if (kind == BPT_KV_FP8)
-    return a.D == 64 ? launch_shape<BPT_KV_FP8, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_FP8, 128>(a, tiles, flags, stream);
-  if (kind == BPT_KV_F16)
-    return a.D == 64 ? launch_shape<BPT_KV_F16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_F16, 128>(a, tiles, flags, stream);
-  return a.D == 64 ? launch_shape<BPT_KV_BF16, 64>(a, tiles, flags, stream) : launch_shape<BPT_KV_BF16, 128>(a, tiles, flags, stream);
+  auto of = [&](auto k) {
+    constexpr int K = decltype(k)::value;
+    if (a.D == 64) return launch_shape<K, 64>(a, tiles, flags, stream);
+    if (a.D == 128) return launch_shape<K, 128>(a, tiles, flags, stream);
+    return launch_shape<K, 256>(a, tiles, flags, stream);
+  };
+  if (kind == BPT_KV_FP8) return of(std::integral_constant<int, BPT_KV_FP8>());
+  if (kind == BPT_KV_F16) return of(std::integral_constant<int, BPT_KV_F16>());
+  return of(std::integral_constant<int, BPT_KV_BF16>());
 }
 
 }  // namespace bpt
