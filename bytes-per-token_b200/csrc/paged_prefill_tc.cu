@@ -8,7 +8,7 @@
 //                memory.
 // Two warpgroups. One does the softmax, a thread per row, so that neither maximum nor sum crosses threads. Of the other, one
 // warp issues the products and the rest bring pages into a ring of shared-memory stages (K and V of a step in stages of their
-// own): 16-bit pages as TMA boxes, one warp, a box per page and 64 dims, pages past the visible keys out of the map's range
+// own): 16-bit pages as TMA boxes, one warp, a box per page, pages past the visible keys out of the map's range
 // and so zero; E4M3 pages through registers, where the codes become f16. While the softmax takes a step's powers, the tensor
 // cores take the products of the step before and the scores of the next. At heads of 64 and 128 two CTAs share an SM, so that
 // one's loads, waits and stores run under the other's powers.
@@ -44,7 +44,8 @@ template <int KIND, int D>
 struct TcShape {
   static constexpr int kRowBytes = D * kElemBytes<KIND>;  // a key's row in its page
   static constexpr int kQ = kRows * D * 2;
-  static constexpr int kStage = kKeys * D * 2;
+  static constexpr int kStage = kKeys * D * 2;  // [group of 8 keys][part of 64 dims][8][128 bytes, swizzled]
+  static constexpr int kGroup = 8 * D * 2;
   static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
   static constexpr int kBars = 2 * kStages + 10;  // an even number: what follows them starts on 16 bytes
   static constexpr int kSmem = kQ + kStages * kStage + kBars * 8 + kFlagSteps * 4 + 16;
@@ -106,15 +107,15 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                : "memory");
 }
 
-// Shared-memory descriptors of 128-byte-swizzled tiles whose rows are 128 bytes, in atoms of 8 rows (1024 bytes). With the
-// contraction along the row (Q, K): the next 8 rows 1024 bytes on. With the contraction across rows (V): the next 8 keys
-// 1024 bytes on, the next 64 dims `half` bytes on.
-__device__ __forceinline__ uint64_t desc_along(uint32_t addr) {
-  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+// Shared-memory descriptors of 128-byte-swizzled tiles, whose rows of 64 values are 128 bytes, in atoms of 8 rows (1024
+// bytes). With the contraction along the row (Q, K): the next 8 rows `rows8` bytes on. With the contraction across rows
+// (V): the next 8 keys `rows8` bytes on, the next 64 dims `dims64` bytes on.
+__device__ __forceinline__ uint64_t desc_along(uint32_t addr, uint32_t rows8) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(rows8 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
-__device__ __forceinline__ uint64_t desc_across(uint32_t addr, uint32_t half) {
-  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(half >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+__device__ __forceinline__ uint64_t desc_across(uint32_t addr, uint32_t rows8, uint32_t dims64) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(dims64 >> 4) << 16) | (uint64_t(rows8 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
 // Instruction descriptor, kind::f16: D f32 (bits 4-5 = 1), A and B f16 or bf16 (bits 7-9, 10-12 = 0 or 1), B's rows across
@@ -166,12 +167,13 @@ struct Item {
   }
 };
 
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int dim, int head, int token, int block,
-                                        uint64_t* bar) {
+// One page's keys (64 of a longer one) of a head, by groups of 8: the map's dims are 64 dims of a row, 8 rows, the row's
+// D / 64 parts, heads, and groups of 8 tokens of the pool.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int head, int group, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(head), "r"(token), "r"(block), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(group), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -574,9 +576,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       bool ok = true;
       if constexpr (kIs16<KIND>) {
         uint32_t edges = 0;
-        const int pages = 1 << per_log2, page = lane & (pages - 1), part = lane >> per_log2;  // a box: a page's 64 dims
-        const int head_dim0 = 64 * part, box_rows = 1 << page_log2;
-        const bool boxed = part < D / 64;
+        const int pages = 1 << per_log2, nowhere = int(a.src.num_blocks << (a.src.bs_log2 - 3));  // a group behind the pool
         for (int n = 0; n < items; ++n) {
           if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
           if (!ok) break;
@@ -591,9 +591,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           const uint32_t dst = smem_u32(ring + in.stage * S::kStage);
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kStage);
           __syncwarp();
-          if (boxed)  // a page that is not there lies behind the pool: the box becomes zeros
-            tma_box(dst + part * (kKeys * 128) + page * (box_rows * 128), v ? &tm_v : &tm_k, head_dim0, hk,
-                    key0 & ((1 << a.src.bs_log2) - 1) & ~(box_rows - 1), blk >= 0 ? blk : int(a.src.num_blocks), bar);
+          if (lane < pages)  // (a page that is not there lies behind the pool: its box becomes zeros)
+            tma_box(dst + (lane << (page_log2 - 3)) * S::kGroup, v ? &tm_v : &tm_k, hk,
+                    blk >= 0 ? (blk << (a.src.bs_log2 - 3)) + ((key0 & ((1 << a.src.bs_log2) - 1)) >> 6 << 3) : nowhere, bar);
           if (partly) {  // values next to the visible ones may be anything: their rows become zeros, as P's columns are there
             ok = __all_sync(0xffffffffu, mbar_wait(edge, edges & 1u));
             ++edges;
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int i = lane; i < kKeys * (D / 8); i += 32) {
               const int r = i / (D / 8), c = i % (D / 8);
               if (key0 + r < take_from || key0 + r >= to)
-                *reinterpret_cast<uint4*>(ring + in.stage * S::kStage + (c >> 3) * (kKeys * 128) + r * 128 + (c & 7) * 16) =
+                *reinterpret_cast<uint4*>(ring + in.stage * S::kStage + (r >> 3) * S::kGroup + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) =
                     make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_shared();
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               const uint4 v4 = x[i * PER + e];
               const uint32_t keep = got >> (i * PER + e) & 1u ? 0xFFFFFFFFu : 0u;
               const uint32_t u[4] = {v4.x & keep, v4.y & keep, v4.z & keep, v4.w & keep};
-              uint8_t* dst = ring + in.stage * S::kStage + ((2 * c) >> 3) * (kKeys * 128) + rr * 128;
+              uint8_t* dst = ring + in.stage * S::kStage + (rr >> 3) * S::kGroup + ((2 * c) >> 3) * 1024 + (rr & 7) * 128;
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ (rr & 7)) << 4)) =
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else if (warp == 7) {
       // ---- matrix products: the whole warp waits, one of its threads issues
       constexpr uint32_t id_s = tc_idesc<KIND>(kRows, kKeys, false), id_o = tc_idesc<KIND>(kRows, D, true);
-      const uint64_t q_desc = desc_along(smem_u32(smem)), k_desc = desc_along(smem_u32(ring)),
-                     v_desc = desc_across(smem_u32(ring), kKeys * 128);
+      const uint64_t q_desc = desc_along(smem_u32(smem), 1024), k_desc = desc_along(smem_u32(ring), S::kGroup),
+                     v_desc = desc_across(smem_u32(ring), S::kGroup, 1024);
       Item<NS> item;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at_k = (k & 3) * (32 >> 4);
-            tc_mma_ss(tmem + 64 * (j & 1), q_desc + (k >> 2) * (kRows * 128 >> 4) + at_k, kd + (k >> 2) * (kKeys * 128 >> 4) + at_k,
+            tc_mma_ss(tmem + 64 * (j & 1), q_desc + (k >> 2) * (kRows * 128 >> 4) + at_k, kd + (k >> 2) * (1024 >> 4) + at_k,
                       id_s, k > 0 ? 1u : 0u);
           }
           tc_commit(&s_full[j & 1]);
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const uint64_t vd = v_desc + uint32_t(item.stage * (S::kStage >> 4));
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            tc_mma_ts(tmem + S::kO, tmem + 64 * (j & 1) + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || j > 0 ? 1u : 0u);
+            tc_mma_ts(tmem + S::kO, tmem + 64 * (j & 1) + 8 * k, vd + k * (2 * S::kGroup >> 4), id_o, k > 0 || j > 0 ? 1u : 0u);
           tc_commit(&o_done[j & 1]);
           tc_commit(&empty[item.stage]);
         }
@@ -765,13 +765,15 @@ int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t strea
   if constexpr (kIs16<KIND>) {
     auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
     if (!encode) return set_error(BPT_ERR_UNSUPPORTED, "paged prefill: the driver has no tensor-map encoder");
-    const cuuint64_t row = cuuint64_t(S::kRowBytes), token = row * a.src.Hkv, bs = cuuint64_t(1) << a.src.bs_log2;
-    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(a.src.Hkv), bs, cuuint64_t(a.src.num_blocks)};
-    const cuuint64_t strides[3] = {row, token, token * bs};
-    const cuuint32_t box[4] = {64, 1, cuuint32_t(std::min<cuuint64_t>(bs, kKeys)), 1}, ones[4] = {1, 1, 1, 1};
+    const int64_t groups = a.src.num_blocks << (a.src.bs_log2 - 3);
+    BPT_REQUIRE(groups < (1ll << 31) - 1, BPT_ERR_UNSUPPORTED, "paged prefill: a pool of %lld tokens", (long long)groups * 8);
+    const cuuint64_t row = cuuint64_t(S::kRowBytes), token = row * a.src.Hkv;
+    const cuuint64_t dims[5] = {64, 8, D / 64, cuuint64_t(a.src.Hkv), cuuint64_t(groups)};
+    const cuuint64_t strides[4] = {token, 128, row, 8 * token};
+    const cuuint32_t box[5] = {64, 8, D / 64, 1, 1u << (std::min(a.src.bs_log2, 6) - 3)}, ones[5] = {1, 1, 1, 1, 1};
     const CUtensorMapDataType type = KIND == BPT_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     for (int i = 0; i < 2; ++i) {
-      const CUresult res = encode(i ? &tm_v : &tm_k, type, 4, const_cast<uint8_t*>(i ? a.src.v_pool : a.src.k_pool), dims, strides,
+      const CUresult res = encode(i ? &tm_v : &tm_k, type, 5, const_cast<uint8_t*>(i ? a.src.v_pool : a.src.k_pool), dims, strides,
                                   box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
       if (res != CUDA_SUCCESS) return set_error(BPT_ERR_INVALID, "paged prefill: tensor map: error %d", int(res));
