@@ -50,7 +50,7 @@ struct TcShape {
   static constexpr int kBars = 2 * kStages + 10;  // an even number: what follows them starts on 16 bytes
   static constexpr int kSmem = kQ + kStages * kStage + kBars * 8 + kFlagSteps * 4 + 16;
   static_assert(D == 256 || kSmem <= 113 * 1024, "two CTAs per SM");
-  static constexpr int kProducers = kIs16<KIND> ? 1 : 3;  // warps
+  static constexpr int kProducers = kIs16<KIND> ? 2 : 3;  // warps
   // setmaxnreg: 128 threads x (softmax + other) = 256 x the launch's 128
   static constexpr int kSoftmaxRegs = kIs16<KIND> ? 200 : 184, kOtherRegs = 256 - kSoftmaxRegs;
   static constexpr uint32_t kO = 128;                             // columns: S at 0 and 64, O from 128
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + S::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * S::kStage);
-  uint64_t* full = bars;             // [NS] a stage's rows have landed (an arrival per producer warp)
+  uint64_t* full = bars;             // [NS] a stage's rows have landed
   uint64_t* empty = full + NS;       // [NS] the products that read it are done
   uint64_t* q_full = empty + NS;     // the queries are in shared memory
   uint64_t* s_full = q_full + 1;     // [2] S is in its buffer: the products' completion, and the issuing thread (which has
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], S::kProducers);
+      mbar_init(&full[i], kIs16<KIND> ? 1 : S::kProducers);
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, 4);
@@ -575,25 +575,28 @@ __global__ void __launch_bounds__(kThreads, 2)
       Item<NS> in;
       bool ok = true;
       if constexpr (kIs16<KIND>) {
-        uint32_t edges = 0;
+        // warp 4 brings K, warp 5 V: every second item of the ring
+        const bool v = w == 1;
         const int pages = 1 << per_log2, nowhere = int(a.src.num_blocks << (a.src.bs_log2 - 3));  // a group behind the pool
-        for (int n = 0; n < items; ++n) {
-          if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
-          if (!ok) break;
-          // (the last steps have no K after their V: items past steps - 1 are skipped by the order's tail)
-          const bool v = is_v(n) || n >= 2 * steps - 1;
-          const int j = n >= 2 * steps - 1 ? steps - 1 : step_of(n);
+        const CUtensorMap* map = v ? &tm_v : &tm_k;
+        uint32_t edges = 0;
+        int n = v ? min(2, steps) : 0;  // the item of step j
+        for (int i = 0; i < n; ++i) in.next();
+        for (int j = 0; j < steps; ++j) {
           const int blk = page_of(j, v);
           if (!v) flag(j, blk);
           const int key0 = from + kKeys * j;
+          const int group =
+              blk >= 0 ? (blk << (a.src.bs_log2 - 3)) + ((key0 & ((1 << a.src.bs_log2) - 1)) >> 6 << 3) : nowhere;
           const bool partly = v && (key0 < take_from || key0 + kKeys > to);
           uint64_t* bar = partly ? edge : &full[in.stage];
           const uint32_t dst = smem_u32(ring + in.stage * S::kStage);
+          if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+          if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kStage);
           __syncwarp();
           if (lane < pages)  // (a page that is not there lies behind the pool: its box becomes zeros)
-            tma_box(dst + (lane << (page_log2 - 3)) * S::kGroup, v ? &tm_v : &tm_k, hk,
-                    blk >= 0 ? (blk << (a.src.bs_log2 - 3)) + ((key0 & ((1 << a.src.bs_log2) - 1)) >> 6 << 3) : nowhere, bar);
+            tma_box(dst + (lane << (page_log2 - 3)) * S::kGroup, map, hk, group, bar);
           if (partly) {  // values next to the visible ones may be anything: their rows become zeros, as P's columns are there
             ok = __all_sync(0xffffffffu, mbar_wait(edge, edges & 1u));
             ++edges;
@@ -608,7 +611,10 @@ __global__ void __launch_bounds__(kThreads, 2)
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[in.stage]);
           }
+          const int ahead = v ? (j == steps - 2 ? 1 : 2) : (j == 0 ? 1 : 2);
+          n += ahead;
           in.next();
+          if (ahead == 2) in.next();
         }
       } else {
         // Codes go through registers: 16 codes a load, an f16 each into the stage. Warp w takes the slabs of 8 rows w, w + 3, ...;
