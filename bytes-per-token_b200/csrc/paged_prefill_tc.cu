@@ -13,6 +13,8 @@
 // cores take the products of the step before and the scores of the next. At heads of 64 and 128 two CTAs share an SM, so that
 // one's loads, waits and stores run under the other's powers.
 //
+// Keys go from the last to the first: a row's nearest come first, which a bias by distance favours.
+//
 // A row's m is the true maximum of the first step that it sees and moves only when a step's sum of 2^(s - m) passes 2^15: until
 // then every P is below 2^15, which both 16-bit types hold, and is divided by the sum of the same powers, so nothing is lost
 // by an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
@@ -52,7 +54,7 @@ struct TcShape {
   static_assert(D == 256 || kSmem <= 113 * 1024, "two CTAs per SM");
   static constexpr int kProducers = kIs16<KIND> ? 2 : 3;  // warps
   // setmaxnreg: 128 threads x (softmax + other) = 256 x the launch's 128
-  static constexpr int kSoftmaxRegs = kIs16<KIND> ? 200 : 184, kOtherRegs = 256 - kSoftmaxRegs;
+  static constexpr int kSoftmaxRegs = kIs16<KIND> ? 200 : 168, kOtherRegs = 256 - kSoftmaxRegs;
   static constexpr uint32_t kO = 128;                             // columns: S at 0 and 64, O from 128
   static constexpr uint32_t kColumns = D == 256 ? 512 : 256;  // of tensor memory
 };
@@ -260,7 +262,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
   float l = 0.f;
   bool ok = true;
   for (int j = 0; j < steps; ++j) {
-    const int key0 = from + j * kKeys;
+    const int key0 = from + (steps - 1 - j) * kKeys;
     const uint32_t s_at = tmem + lanes + 64 * (j & 1), phase = (j >> 1) & 1;
     ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], phase));
     if (!ok) break;
@@ -547,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       // step first + i / per_step; the next window is loaded while this one is in use.
       const int page_log2 = min(a.src.bs_log2, 6), per_log2 = 6 - page_log2, window_log2 = 5 - per_log2;
       auto window = [&](int first) {
-        return block_at(from + ((first + (lane >> per_log2)) << 6) + ((lane & ((1 << per_log2) - 1)) << page_log2));
+        const int back = steps - 1 - first - (lane >> per_log2);  // steps go from the last keys to the first
+        return back < 0 ? -1 : block_at(from + (back << 6) + ((lane & ((1 << per_log2) - 1)) << page_log2));
       };
       int k_held = window(0), k_next = window(1 << window_log2), v_held = k_held, v_next = k_next;
       // this lane's page (lane < pages) of step j
@@ -585,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int j = 0; j < steps; ++j) {
           const int blk = page_of(j, v);
           if (!v) flag(j, blk);
-          const int key0 = from + kKeys * j;
+          const int key0 = from + kKeys * (steps - 1 - j);
           const int group =
               blk >= 0 ? (blk << (a.src.bs_log2 - 3)) + ((key0 & ((1 << a.src.bs_log2) - 1)) >> 6 << 3) : nowhere;
           const bool partly = v && (key0 < take_from || key0 + kKeys > to);
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int blk = page_of(j, v);
           if (!v && w == 0) flag(j, blk);
           const uint8_t* pool = v ? a.src.v_pool : a.src.k_pool;
-          const int key0 = from + kKeys * j;
+          const int key0 = from + kKeys * (steps - 1 - j);
           got = 0;
 #pragma unroll
           for (int i = 0; i < SLABS; ++i) {
