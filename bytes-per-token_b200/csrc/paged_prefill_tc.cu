@@ -667,10 +667,10 @@ __global__ void __launch_bounds__(kThreads, 2)
               const uint32_t u[4] = {v4.x & keep, v4.y & keep, v4.z & keep, v4.w & keep};
               uint8_t* dst = ring + in.stage * S::kStage + (rr >> 3) * S::kGroup + ((2 * c) >> 3) * 1024 + (rr & 7) * 128;
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ (rr & 7)) << 4)) =
-                    make_uint4(codes_to_f16<KIND>(u[2 * h] & 0xFFFFu), codes_to_f16<KIND>(u[2 * h] >> 16),
-                               codes_to_f16<KIND>(u[2 * h + 1] & 0xFFFFu), codes_to_f16<KIND>(u[2 * h + 1] >> 16));
+              for (int h = 0; h < 2; ++h) {
+                const uint2 x0 = codes_to_f16<KIND>(u[2 * h]), x1 = codes_to_f16<KIND>(u[2 * h + 1]);
+                *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ (rr & 7)) << 4)) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+              }
             }
           }
           fence_proxy_async_shared();

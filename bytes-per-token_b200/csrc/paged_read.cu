@@ -4,8 +4,8 @@
 //   s_j = cap tanh(scale q.k_j / cap) - slope |p - j|,  out = sum_j softmax(s)_j v_j  over  max(0, start, p - window + 1) <= j
 //   <= p, p = length - 1; no visible key gives 0.
 //
-// Bound by memory: each visible key and value is read once. Work is cut into equal shares, one per warp of a full GPU (8 warps
-// per SM): a warp takes a contiguous range of groups of 16 keys, of one KV head (and eight of its query heads), across the
+// Bound by memory: each visible key and value is read once. Work is cut into equal shares, one per warp of a full GPU (8
+// warps per SM): a warp takes a contiguous range of groups of 16 keys, of one KV head (and eight of its query heads), across the
 // sequences of the batch, so that ragged lengths leave no SM idle; the warps of a CTA hold the heads of one range, whose rows
 // lie next to each other in the pages. A warp never waits for another: it has its own ring of cp.async stages, running on
 // into its next sequence, and its own running maximum and sum. A group's rows arrive whole (D elements of one head); rows
@@ -16,7 +16,7 @@
 // are added in fp32. Products are thus good to 16 (bf16) or 22 bits at no cost.
 //
 // A sequence inside one range goes straight to out. One that crosses ranges leaves a part per range, and a second kernel,
-// launched dependently, joins them: a CTA per range, whose sequence starts there.
+// launched dependently, joins them.
 #include <algorithm>
 
 #include "paged_read.cuh"
@@ -26,8 +26,8 @@ namespace bpt {
 namespace {
 
 constexpr int kWarps = 4;          // per CTA, at most
-constexpr int kStartCost = 4;      // what a sequence's start costs a range, in groups of 16 keys
-constexpr int kLeastShare = 4;     // groups; a smaller share would be all start and join
+constexpr int kStartCost = 2;      // what a sequence's start costs a range, in groups of 16 keys
+constexpr int kLeastShare = 2;     // groups; a smaller share would be all start and join
 
 struct ReadArgs {
   PagedSource src;
@@ -44,10 +44,13 @@ struct ReadArgs {
   void* out;
   int out_dtype;
   // merged: parts[ranges][heads][2] (0: of the sequence that a range continues, 1: of the one it leaves unfinished), each
-  // o [8][D] and base-2 log-sum-exps [8]; meta[ranges][heads]: the unfinished sequence and its last range (sequence -1: none)
+  // o [8][D] and base-2 log-sum-exps [8]; meta[places][heads]: a sequence in several ranges as (itself, its first range, its
+  // last), (-1, ., .) for none. A place is a sequence where there are no more of them than ranges, else the range that it
+  // starts in: the second kernel has a CTA per place and head.
   float* ws_out;
   float* ws_lse;
-  int2* ws_meta;
+  int4* ws_meta;
+  int by_sequence;
   // partials: out [B, Hq, n_splits, D], lse [B, Hq, n_splits] (natural logarithm) of `split` keys each
   float* part_out;
   float* part_lse;
@@ -113,8 +116,8 @@ struct ReadShape {
   // Stages per warp: what keeps the memory busy. 16-bit heads of 128: 3 stages x 8 KB x 4 warps = 96 KB, two CTAs per SM.
   static constexpr int kStages = RB >= 512 ? 3 : RB == 256 ? 3 : 4;
   static constexpr int kPerWarp = kStages * kStage;
-  static constexpr int kSmem = kWarps * kPerWarp;  // two CTAs per SM, one at 16-bit heads of 256
-  static constexpr int kWarpsPerSm = RB >= 512 ? 4 : 8;  // the warps that share the work
+  static constexpr int kSmem = kWarps * kPerWarp;
+  static constexpr int kCtas = RB >= 512 ? 1 : 2;  // per SM
 };
 
 // The visible keys of a sequence, cut to the pages that its table has.
@@ -155,7 +158,7 @@ struct Walk {
 };
 
 template <int KIND, int D, bool MERGE>
-__global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_read_kernel(const ReadArgs a) {
   using S = ReadShape<KIND, D>;
   constexpr int RB = S::RB, NST = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs 
     share = max((total + a.ranges - 1) / a.ranges, int64_t(kStartCost + kLeastShare));
     begin = range * share;
     end = min(begin + share, total);
-    if (a.ranges > 1 && lane == 0) a.ws_meta[id] = make_int2(-1, 0);
+    if (a.ranges > 1 && !a.by_sequence && lane == 0) a.ws_meta[id] = make_int4(-1, 0, 0, 0);
     if (begin >= total) return;
     int64_t before = 0;  // the sequence that holds cost `begin`
     for (int b0 = 0;; b0 += 32) {
@@ -272,7 +275,9 @@ __global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs 
   int st = 0, st_in = NST - 1;
 
   for (;;) {  // the range's sequences
-    if (MERGE && use.g1 == use.g0 && use.v.groups == 0 && use.at >= begin && lane < D / 8) {  // nothing visible: zeros
+    if (MERGE && use.v.groups == 0 && use.at >= begin && a.by_sequence && a.ranges > 1 && lane == 0)
+      a.ws_meta[int64_t(use.b) * a.heads + ht] = make_int4(-1, 0, 0, 0);
+    if (MERGE && use.v.groups == 0 && use.at >= begin && lane < D / 8) {  // nothing visible: zeros
       for (int r = 0; r < heads; ++r)
 #pragma unroll
         for (int i = 0; i < 8; ++i) store_any(a.out, a.out_dtype, (int64_t(use.b) * a.Hq + h0 + r) * D + lane * 8 + i, 0.f);
@@ -368,9 +373,10 @@ __global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs 
       const int64_t part = id * 2 + (starts ? 1 : 0);
       dst = a.ws_out + (part * 8 + g) * D;
       if (t == 0) a.ws_lse[part * 8 + g] = lse;
-      if (starts && lane == 0)
-        a.ws_meta[id] = make_int2(use.b, int((use.at + kStartCost + use.v.groups - 1) / share));
     }
+    if (starts && lane == 0 && a.ranges > 1 && (a.by_sequence || !ends))
+      a.ws_meta[a.by_sequence ? int64_t(use.b) * a.heads + ht : id] =
+          make_int4(ends ? -1 : use.b, range, int((use.at + kStartCost + use.v.groups - 1) / share), 0);
   } else if (g < heads) {
     dst = a.part_out + (row * a.n_splits + sp) * D;
     if (t == 0) a.part_lse[row * a.n_splits + sp] = lse / kLog2e;
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_read_kernel(const ReadArgs 
   cp_async_wait<0>();
 }
 
-// Joins the parts of the sequence that range x of a head leaves unfinished. Eight warps: as many per row as fit.
+// Joins the parts of a place's sequence for one of its heads. Eight warps: as many per row as fit.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const ReadArgs a) {
   __shared__ float s_sum[8], s_top[8];
@@ -410,15 +416,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ReadArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int64_t id = blockIdx.x;
-  const int2 meta = a.ws_meta[id];
+  const int4 meta = a.ws_meta[id];
   if (meta.x < 0) return;
-  const int range = int(id / a.heads), ht = int(id - int64_t(range) * a.heads), hk = ht / a.tiles, tile = ht - hk * a.tiles;
+  const int range = meta.y, ht = int(id % a.heads), hk = ht / a.tiles, tile = ht - hk * a.tiles;
   const int h0 = hk * a.rep + tile * 8, heads = min(8, a.rep - tile * 8), rows = gridDim.y == 1 ? heads : 1;
   if (int(blockIdx.y) >= heads) return;
   const int per_row = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = warp / per_row, first = warp % per_row;
   const int row = rows == 1 ? int(blockIdx.y) : r;
-  const int parts = meta.y - range + 1;
+  const int parts = meta.z - range + 1;
   constexpr int V = D / 32;
   float top = -INFINITY, sum = 0.f, acc[V];
 #pragma unroll
@@ -481,10 +487,11 @@ int launch(const void* kernel, dim3 grid, int threads, int smem, bool dependent,
   return BPT_OK;
 }
 
-// The most ranges of a merged read: as many as give every warp of a full GPU one head of one range.
+// The most ranges of a merged read: as many as give every warp of a full GPU one head of one range (two CTAs per SM, one at
+// 16-bit heads of 256; three CTAs of 8-bit heads of 128 measured 37 us where two take 35).
 int64_t read_ranges(int64_t heads, int64_t D, int kind) {
   const bool wide = D == 256 && (kind == BPT_KV_F16 || kind == BPT_KV_BF16);
-  return std::max<int64_t>(int64_t(num_sms()) * (wide ? ReadShape<BPT_KV_F16, 256>::kWarpsPerSm : 8) / heads, 1);
+  return std::max<int64_t>(int64_t(num_sms()) * (wide ? 1 : 2) * kWarps / heads, 1);
 }
 
 template <int KIND, int D, bool MERGE>
@@ -503,7 +510,8 @@ int launch_read(const ReadArgs& a, int flags, cudaStream_t stream) {
   if (st || !MERGE || a.ranges == 1) return st;
   // many ranges per sequence: a CTA per row, so that no warp reads a long row of parts
   const unsigned rows = a.ranges >= 16 * int64_t(a.B) ? unsigned(std::min(a.rep, 8)) : 1u;
-  return launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(unsigned(warps), rows), 256, 0, true, a, stream);
+  const int64_t places = (a.by_sequence ? a.B : a.ranges) * int64_t(a.heads);
+  return launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(unsigned(places), rows), 256, 0, true, a, stream);
 }
 
 template <int KIND>
@@ -524,7 +532,7 @@ struct ReadWorkspace {
 ReadWorkspace read_workspace(int64_t Hq, int64_t Hkv, int64_t D, int kind) {
   const int64_t heads = Hkv * ((Hq / Hkv + 7) / 8), warps = read_ranges(heads, D, kind) * heads;
   ReadWorkspace w;
-  w.meta = (warps * 8 + 255) / 256 * 256;
+  w.meta = (warps * 16 + 255) / 256 * 256;
   w.lse = w.meta + (warps * 2 * 8 * 4 + 255) / 256 * 256;
   w.total = w.lse + warps * 2 * 8 * D * 4;
   return w;
@@ -652,6 +660,7 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
   a.split = a.n_splits = a.ranges = 1;
   a.ws_out = a.ws_lse = nullptr;
   a.ws_meta = nullptr;
+  a.by_sequence = 0;
   if (merge) {
     BPT_REQUIRE(out, BPT_ERR_INVALID, "%s: null output", who);
     BPT_REQUIRE(out_dtype == BPT_DTYPE_F32 || out_dtype == BPT_DTYPE_F16 || out_dtype == BPT_DTYPE_BF16, BPT_ERR_INVALID,
@@ -660,6 +669,7 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
     const int64_t keys = a.window > 0 ? std::min<int64_t>(tokens, int64_t(a.window) + 15) : tokens;
     const int64_t cost = (std::min<int64_t>(keys, 1 << 30) + 15) / 16 + kStartCost;
     a.ranges = int(std::min(read_ranges(a.heads, D, kind), std::max<int64_t>(B * cost / (kStartCost + kLeastShare), 1)));
+    a.by_sequence = B <= a.ranges;
     if (a.ranges > 1) {
       const ReadWorkspace w = read_workspace(Hq, Hkv, D, kind);
       BPT_REQUIRE(workspace, BPT_ERR_WORKSPACE, "%s: no workspace", who);
@@ -667,7 +677,7 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
       BPT_REQUIRE(workspace_bytes >= w.total, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
                   (long long)workspace_bytes, (long long)w.total);
       uint8_t* ws = static_cast<uint8_t*>(workspace);
-      a.ws_meta = reinterpret_cast<int2*>(ws);
+      a.ws_meta = reinterpret_cast<int4*>(ws);
       a.ws_lse = reinterpret_cast<float*>(ws + w.meta);
       a.ws_out = reinterpret_cast<float*>(ws + w.lse);
     }

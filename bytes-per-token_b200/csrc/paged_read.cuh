@@ -98,16 +98,23 @@ __device__ __forceinline__ int q_dim(int j, int t, int i) {
   return 64 * (j >> 2) + 16 * t + 4 * (j & 3) + i;
 }
 
-// Two codes (the low two bytes of `two`) as an f16 pair.
+// Four codes as two f16 pairs: bytes 0, 1 and bytes 2, 3.
 template <int KIND>
-__device__ __forceinline__ uint32_t codes_to_f16(uint32_t two) {
-  uint32_t h;
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t four) {
+  uint2 h;
   if constexpr (KIND == BPT_KV_FP8) {
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(two)));
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "mov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(h.x), "=r"(h.y)
+        : "r"(four));
   } else {  // 1024 + (code + 128) as f16 bits, less 1152
-    const uint32_t m = __byte_perm(two ^ 0x8080u, 0x64646464u, 0x4140);
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1152.f, 1152.f));
-    h = *reinterpret_cast<const uint32_t*>(&v);
+    const uint32_t u = four ^ 0x80808080u, m0 = __byte_perm(u, 0x64646464u, 0x4140), m1 = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+    const __half2 v0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), off), v1 = __hsub2(*reinterpret_cast<const __half2*>(&m1), off);
+    h.x = *reinterpret_cast<const uint32_t*>(&v0);
+    h.y = *reinterpret_cast<const uint32_t*>(&v1);
   }
   return h;
 }
@@ -162,8 +169,9 @@ __device__ __forceinline__ void scores16(uint32_t tile, int lane, const Q& q, fl
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const MmaRows qj = q(4 * j4 + i);
-        mma_16816<KIND>(i & 1 ? t0 : s0, qj.v, codes_to_f16<KIND>(xs[i] & 0xFFFFu), codes_to_f16<KIND>(xs[i] >> 16));
-        mma_16816<KIND>(i & 1 ? t1 : s1, qj.v, codes_to_f16<KIND>(ys[i] & 0xFFFFu), codes_to_f16<KIND>(ys[i] >> 16));
+        const uint2 x2 = codes_to_f16<KIND>(xs[i]), y2 = codes_to_f16<KIND>(ys[i]);
+        mma_16816<KIND>(i & 1 ? t0 : s0, qj.v, x2.x, x2.y);
+        mma_16816<KIND>(i & 1 ? t1 : s1, qj.v, y2.x, y2.y);
       }
     }
   }
@@ -214,11 +222,12 @@ __device__ __forceinline__ void values16(uint32_t tile, int lane, const uint32_t
         // bytes j of rows 2t and 2t + 1 next to each other (and of rows 2t + 8, 2t + 9), two j per word
         const uint32_t a0 = __byte_perm(w[0][i], w[1][i], 0x5140), a1 = __byte_perm(w[0][i], w[1][i], 0x7362);
         const uint32_t c0 = __byte_perm(w[2][i], w[3][i], 0x5140), c1 = __byte_perm(w[2][i], w[3][i], 0x7362);
+        const uint2 x0 = codes_to_f16<KIND>(a0), x1 = codes_to_f16<KIND>(a1), y0 = codes_to_f16<KIND>(c0), y1 = codes_to_f16<KIND>(c1);
         const int n = 4 * W * pass + 4 * i;
-        mma_16816<KIND>(o[n], p, codes_to_f16<KIND>(a0 & 0xFFFFu), codes_to_f16<KIND>(c0 & 0xFFFFu));
-        mma_16816<KIND>(o[n + 1], p, codes_to_f16<KIND>(a0 >> 16), codes_to_f16<KIND>(c0 >> 16));
-        mma_16816<KIND>(o[n + 2], p, codes_to_f16<KIND>(a1 & 0xFFFFu), codes_to_f16<KIND>(c1 & 0xFFFFu));
-        mma_16816<KIND>(o[n + 3], p, codes_to_f16<KIND>(a1 >> 16), codes_to_f16<KIND>(c1 >> 16));
+        mma_16816<KIND>(o[n], p, x0.x, y0.x);
+        mma_16816<KIND>(o[n + 1], p, x0.y, y0.y);
+        mma_16816<KIND>(o[n + 2], p, x1.x, y1.x);
+        mma_16816<KIND>(o[n + 3], p, x1.y, y1.y);
       }
     }
   }
@@ -276,14 +285,28 @@ struct GroupLoader {
     const int64_t at = slot * row_bytes + head_bytes, at2 = slot2 * row_bytes + head_bytes;
     if (lane == 0) *flag = (blk < 0 && key0 < to ? 1u : 0u) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u);
     constexpr int CPR = RB / 16;
+    const int r0 = lane / CPR, c0 = lane % CPR;  // this lane's chunk of the first rows; a pass of the warp takes STEP rows
+    constexpr int STEP = CPR >= 32 ? 1 : 32 / CPR;
+    if (key0 >= from && key0 + 16 <= to && blk >= 0 && blk2 >= 0) {  // all of it
+      const int64_t mine = r0 * row_bytes + c0 * 16;
+      const uint8_t *k0 = src.k_pool + at + mine, *k1 = src.k_pool + at2 + mine, *v0 = src.v_pool + at + mine, *v1 = src.v_pool + at2 + mine;
 #pragma unroll
-    for (int n = 0; n < 16 * CPR / 32; ++n) {
-      const int idx = lane + 32 * n, r = idx / CPR, c = idx % CPR;
-      const bool take = key0 + r >= from && key0 + r < to && (r < 8 ? blk : blk2) >= 0;
-      const int64_t off = take ? (r < 8 ? at : at2) + r * row_bytes + c * 16 : 0;
-      const uint32_t d = r * RB + swizzled<KIND, D>(r, c) * 16;
-      cp_async16(k_dst + d, src.k_pool + off, take);
-      cp_async16(v_dst + d, src.v_pool + off, take);
+      for (int n = 0; n < 16 / STEP; ++n) {
+        const uint32_t d = (STEP * n + r0) * RB + swizzled<KIND, D>(STEP * n + r0, c0) * 16;
+        const int64_t down = STEP * n * row_bytes;
+        cp_async16(k_dst + d, (STEP * n < 8 ? k0 : k1) + down);
+        cp_async16(v_dst + d, (STEP * n < 8 ? v0 : v1) + down);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 16 / STEP; ++n) {
+        const int r = STEP * n + r0;
+        const bool take = key0 + r >= from && key0 + r < to && (STEP * n < 8 ? blk : blk2) >= 0;
+        const int64_t off = take ? (STEP * n < 8 ? at : at2) + r * row_bytes + c0 * 16 : 0;
+        const uint32_t d = r * RB + swizzled<KIND, D>(r, c0) * 16;
+        cp_async16(k_dst + d, src.k_pool + off, take);
+        cp_async16(v_dst + d, src.v_pool + off, take);
+      }
     }
     if constexpr (KIND == BPT_KV_INT8) {  // lanes 0-15 the group's K scales, 16-31 its V scales; stored by place()
       const int r = lane & 15;
