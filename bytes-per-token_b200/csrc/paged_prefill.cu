@@ -9,8 +9,11 @@
 // [lo, hi), and a tile of rows visits only the keys between its smallest lo and largest hi.
 //
 // Every format but int8 takes csrc/paged_prefill_tc.cu. The kernel here serves int8 pages, whose scale per key goes on the
-// scores and on the probabilities. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. Where there
-// are few tiles, each takes several CTAs, with a part of its keys each; a second kernel, launched dependently, joins them.
+// scores (a factor per column of S) and on the probabilities (a factor per column of P), so that the codes themselves are the
+// operands. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. It is bound by
+// the legacy matrix path and the conversion of the codes: the same design over bf16 pages took 467 us for twelve ragged prompts
+// where the tcgen05 kernel takes 120. This file also holds, for both kernels, the plan and the join: where there
+// are few tiles, each takes several CTAs, with a part of its keys each, and a second kernel, launched dependently, joins them.
 #include "paged_prefill.cuh"
 
 namespace bpt {
@@ -21,19 +24,21 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16 * kWarps;
 constexpr int kKeys = 64;
 
-template <int KIND, int D>
+constexpr int KIND = BPT_KV_INT8;
+
+template <int D>
 struct PrefillShape {
   static constexpr int RB = D * kElemBytes<KIND>;
-  static constexpr int kScaleBytes = KIND == BPT_KV_INT8 ? kKeys * 4 : 0;  // 16 K then 16 V scales (fp16) per 16 keys
-  static constexpr int kStage = 2 * kKeys * RB + kScaleBytes + 16;          // keys, values, scales, a flag per 16 keys
-  static constexpr int kQ = kWarps * (D / 16) * 32 * 16;                    // the q fragments
+  static constexpr int kScaleBytes = kKeys * 4;                     // 16 K then 16 V scales (fp16) per 16 keys
+  static constexpr int kStage = 2 * kKeys * RB + kScaleBytes + 16;  // keys, values, scales, a flag per 16 keys
+  static constexpr int kQ = kWarps * (D / 16) * 32 * 16;            // the q fragments
   static constexpr int kStages = 2;
   static constexpr int kSmem = kStages * kStage + kQ;
 };
 
-template <int KIND, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillArgs a) {
-  using S = PrefillShape<KIND, D>;
+  using S = PrefillShape<D>;
   constexpr int RB = S::RB;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_range[2][kWarps];
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   float unit[2];
   {
     float amax[2] = {0.f, 0.f};
-    if (KIND != BPT_KV_BF16 && a.q_dtype == BPT_DTYPE_BF16) {
+    if (a.q_dtype == BPT_DTYPE_BF16) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (row[i].q >= 0)
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
 
   for (int i = 0; i < steps; ++i) {
     const int st = i & 1, key0 = from + i * kKeys;
-    if constexpr (KIND == BPT_KV_INT8) loader.place(scales_of(st, warp));
+    loader.place(scales_of(st, warp));
     __syncthreads();  // everyone is done with the stage refilled next
     request(i + 1, st ^ 1);
     cp_async_wait<1>();
@@ -185,8 +190,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
       for (int e = 0; e < 4; ++e) {
         const int i2 = e >> 1, key = key0 + 8 * n + 2 * t + (e & 1);
         float x = s[n][e];
-        if constexpr (KIND == BPT_KV_INT8) x *= __half2float(reinterpret_cast<const __half*>(scales_of(st, n >> 1))[8 * (n & 1) + 2 * t + (e & 1)]);
-        x *= mul[i2];
+        x *= __half2float(reinterpret_cast<const __half*>(scales_of(st, n >> 1))[8 * (n & 1) + 2 * t + (e & 1)]) * mul[i2];
         if (cap) x = capped(x, cap_out);
         if (a.slopes) x = fmaf(row[i2].slope, fabsf(float(key - row[i2].pos)), x);
         if (masked && (key < row[i2].lo || key >= row[i2].hi)) x = -INFINITY;
@@ -225,11 +229,9 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
         for (int i2 = 0; i2 < 2; ++i2) {
           float x = exp2_approx(s[2 * n + k][2 * i2] - off[i2]), y = exp2_approx(s[2 * n + k][2 * i2 + 1] - off[i2]);
           l[i2] += x + y;
-          if constexpr (KIND == BPT_KV_INT8) {
-            const __half* vs = reinterpret_cast<const __half*>(scales_of(st, n)) + 16 + 8 * k + 2 * t;
-            x *= __half2float(vs[0]);
-            y *= __half2float(vs[1]);
-          }
+          const __half* vs = reinterpret_cast<const __half*>(scales_of(st, n)) + 16 + 8 * k + 2 * t;
+          x *= __half2float(vs[0]);
+          y *= __half2float(vs[1]);
           p[2 * k + i2] = pack2<KIND>(x, y);
         }
       values16<KIND, D>(stage(st) + (kKeys + n * 16) * RB, lane, p, o);
@@ -251,12 +253,8 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
       for (int n = 0; n < D / 8; ++n) {
         const float x = o[n][2 * i] * inv[i], y = o[n][2 * i + 1] * inv[i];
         const int64_t dst = row[i].out + v_dim<KIND, D>(n, t, 0);
-        if constexpr (kIs16<KIND>) {
-          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + dst) = pack2<KIND>(x, y);
-        } else {
-          store_16(a.out, a.q_dtype, dst, x);
-          store_16(a.out, a.q_dtype, row[i].out + v_dim<KIND, D>(n, t, 1), y);
-        }
+        store_16(a.out, a.q_dtype, dst, x);
+        store_16(a.out, a.q_dtype, row[i].out + v_dim<KIND, D>(n, t, 1), y);
       }
     }
     return;
@@ -330,11 +328,11 @@ int launch_join(const PrefillArgs& a, int64_t tiles, int rows, cudaStream_t stre
   return BPT_OK;
 }
 
-template <int KIND, int D>
+template <int D>
 int launch_prefill(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
-  using S = PrefillShape<KIND, D>;
+  using S = PrefillShape<D>;
   static std::atomic<uint64_t> ready{0};
-  const int st = set_max_smem_once(reinterpret_cast<const void*>(paged_prefill_kernel<KIND, D>), S::kSmem, ready);
+  const int st = set_max_smem_once(reinterpret_cast<const void*>(paged_prefill_kernel<D>), S::kSmem, ready);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
@@ -346,16 +344,15 @@ int launch_prefill(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & BPT_FLAG_PDL) ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<KIND, D>, a);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D>, a);
   if (err != cudaSuccess) return set_error(BPT_ERR_CUDA, "paged prefill launch: %s", cudaGetErrorString(err));
   return BPT_OK;
 }
 
-template <int KIND>
-int prefill_dim(const PrefillArgs& a, int64_t D, int64_t tiles, int flags, cudaStream_t stream) {
-  if (D == 64) return launch_prefill<KIND, 64>(a, tiles, flags, stream);
-  if (D == 128) return launch_prefill<KIND, 128>(a, tiles, flags, stream);
-  return launch_prefill<KIND, 256>(a, tiles, flags, stream);
+int prefill_int8(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t stream) {
+  if (a.D == 64) return launch_prefill<64>(a, tiles, flags, stream);
+  if (a.D == 128) return launch_prefill<128>(a, tiles, flags, stream);
+  return launch_prefill<256>(a, tiles, flags, stream);
 }
 
 // How a call is cut: which kernel, rows per tile, the most tiles that the rows can make, keys per part and parts.
@@ -491,10 +488,6 @@ extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
     a.part_out = reinterpret_cast<float*>(ws + count_bytes(p, Hkv) + lse_bytes(p, Hkv));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int st = p.tc                  ? prefill_tc(a, kind, p.tiles, flags, s)
-                 : kind == BPT_KV_FP8  ? prefill_dim<BPT_KV_FP8>(a, D, p.tiles, flags, s)
-                 : kind == BPT_KV_INT8 ? prefill_dim<BPT_KV_INT8>(a, D, p.tiles, flags, s)
-                 : kind == BPT_KV_F16  ? prefill_dim<BPT_KV_F16>(a, D, p.tiles, flags, s)
-                                       : prefill_dim<BPT_KV_BF16>(a, D, p.tiles, flags, s);
+  const int st = p.tc ? prefill_tc(a, kind, p.tiles, flags, s) : prefill_int8(a, p.tiles, flags, s);
   return st || p.n_splits == 1 ? st : launch_join(a, p.tiles, p.rows, s);
 }
