@@ -13,9 +13,11 @@ then the final norm, the tied LM head and a greedy pick. The hot-path pieces run
 With `fused=True` (the default) the small ops around them are two fused kernels per use (`decode_fused.py`):
 the residual adds with the following RMSNorm (`engine/model.py:24-36, 109-111`), and q_norm / k_norm, RoPE and
 the FP8 cache write of the new token in one pass; `fused=False` runs them as the reference's PyTorch ops (plus
-`quantize_kv_paged`). The embedding and the LM head stay in PyTorch. Weights are random (no checkpoints here): N(0, 0.02), quantized to INT4 g128
-by `quantize_w4a16`; the LM head stays bf16 and tied to the embedding (`quant/model.py:3-4`). The KV pools hold
-random finite E4M3 codes for the existing context. All buffers are allocated up front, so `step` can be
+`quantize_kv_paged`). With `kv_kind="bf16"` the cache holds bf16 pages: `rope_kv_append` normalises, rotates and
+stores the new token, and the any-format decode read attends. The embedding and the LM head stay in PyTorch. Weights
+are random (no checkpoints here): N(0, 0.02), quantized to INT4 g128 by `quantize_w4a16`; the LM head stays bf16 and
+tied to the embedding (`quant/model.py:3-4`). The KV pools hold random finite E4M3 codes (or N(0, 1) values) for the
+existing context. All buffers are allocated up front, so `step` can be
 captured in a CUDA graph (`capture`).
 """
 
@@ -28,7 +30,7 @@ import torch
 
 from bpt_b200.kernels.decode_fused import qk_norm_rope_kv_write, rms_norm_residual
 from bpt_b200.kernels.kv_attention import PagedQuantKV, attend, attend_workspace, paged_split
-from bpt_b200.kernels.kv_write import quantize_kv_paged
+from bpt_b200.kernels.kv_write import quantize_kv_paged, rope_kv_append, rope_table
 from bpt_b200.kernels.w4a16 import interleave_rows, quantize_w4a16, w4a16_gate_up_silu, w4a16_linear
 
 
@@ -92,14 +94,17 @@ class Layer:
 
 
 class Qwen3Decoder:
-    """Random-weight Qwen3 with a paged FP8 cache, stepping `batch` sequences one token at a time.
+    """Random-weight Qwen3 with a paged FP8 (or bf16) cache, stepping `batch` sequences one token at a time.
 
     `lengths` are the tokens already in each sequence's cache; each step writes one more and attends over
     length + 1. `capacity` is how many steps the block table leaves room for.
     """
 
     def __init__(self, dims: Qwen3Dims, lengths: torch.Tensor, *, device="cuda", seed: int = 0, capacity: int = 64,
-                 kv_scale: float = 1.0 / 64, keep_dense: bool = False, fused: bool = True):
+                 kv_scale: float = 1.0 / 64, keep_dense: bool = False, fused: bool = True, kv_kind: str = "fp8"):
+        if kv_kind not in ("fp8", "bf16") or (kv_kind == "bf16" and not fused):
+            raise ValueError(f"kv_kind must be 'fp8' or, with fused=True, 'bf16', got {kv_kind!r}")
+        self.kv_kind = kv_kind
         self.dims, self.device, self.fused = dims, torch.device(device), fused
         d, dev = dims, self.device
         g = torch.Generator(device=dev).manual_seed(seed)
@@ -133,9 +138,13 @@ class Qwen3Decoder:
             wo, wg, wu, wd = w(d.hidden, qd), w(d.intermediate, d.hidden), w(d.intermediate, d.hidden), w(d.hidden, d.intermediate)
             qg, qu = quantize_w4a16(wg, d.group), quantize_w4a16(wu, d.group)
             gate_up = tuple(interleave_rows(x, y) for x, y in zip(qg, qu, strict=True))
-            kpool = random_e4m3_codes((pages, 16, d.kv_heads, d.head_dim), g, dev)
-            vpool = random_e4m3_codes((pages, 16, d.kv_heads, d.head_dim), g, dev)
-            kv = PagedQuantKV("fp8", kpool, vpool, self.block_table, 16, kv_scale, kv_scale)
+            pool = (pages, 16, d.kv_heads, d.head_dim)
+            if kv_kind == "bf16":
+                kpool, vpool = (torch.randn(pool, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+                kv = PagedQuantKV("bf16", kpool, vpool, self.block_table, 16)
+            else:
+                kpool, vpool = random_e4m3_codes(pool, g, dev), random_e4m3_codes(pool, g, dev)
+                kv = PagedQuantKV("fp8", kpool, vpool, self.block_table, 16, kv_scale, kv_scale)
             layer = Layer(quantize_w4a16(torch.cat([wq, wk, wv]), d.group), quantize_w4a16(wo, d.group), gate_up,
                           quantize_w4a16(wd, d.group), norm(d.hidden), norm(d.hidden), norm(d.head_dim),
                           norm(d.head_dim), kv)
@@ -159,6 +168,7 @@ class Qwen3Decoder:
         self.split = split
         self.workspace = attend_workspace(b, d.q_heads, d.head_dim, -(-self.max_tokens // split), dev).clone()
         self.scale = 1.0 / math.sqrt(d.head_dim)
+        self.rope = rope_table(self.max_tokens, d.head_dim, d.rope_theta, dev) if kv_kind == "bf16" else None
         self.graph = None
 
     # ---- one step ----------------------------------------------------------------------------------------------
@@ -193,10 +203,16 @@ class Qwen3Decoder:
         rms_norm_residual(self.h, self.layers[0].input_norm, d.eps, x_out=self.x, pdl=True)
         for i, layer in enumerate(self.layers):
             w4a16_linear(self.x, *layer.qkv, group=d.group, out=self.qkv, pdl=True)
-            qk_norm_rope_kv_write(self.qkv, d.q_heads, d.kv_heads, layer.q_norm, layer.k_norm, cos, sin, d.eps,
-                                  layer.kv, write_blocks, write_offsets, q_out=self.q, pdl=True)
-            attend(self.q, layer.kv, lengths_after, self.scale, out=self.attn, workspace=self.workspace,
-                   tokens=self.max_tokens, split=self.split, pdl=True)
+            if self.kv_kind == "bf16":
+                q, k, v = (t.view(b, -1, d.head_dim) for t in self.qkv.split([qd, *[d.kv_heads * d.head_dim] * 2], dim=1))
+                rope_kv_append(q, k, v, layer.kv, self.lengths, *self.rope, write_blocks, write_offsets,
+                               q_norm=layer.q_norm, k_norm=layer.k_norm, eps=d.eps, q_out=self.q, pdl=True)
+                attend(self.q, layer.kv, lengths_after, self.scale, out=self.attn, tokens=self.max_tokens, pdl=True)
+            else:
+                qk_norm_rope_kv_write(self.qkv, d.q_heads, d.kv_heads, layer.q_norm, layer.k_norm, cos, sin, d.eps,
+                                      layer.kv, write_blocks, write_offsets, q_out=self.q, pdl=True)
+                attend(self.q, layer.kv, lengths_after, self.scale, out=self.attn, workspace=self.workspace,
+                       tokens=self.max_tokens, split=self.split, pdl=True)
             w4a16_linear(self.attn.view(b, qd), *layer.o, group=d.group, out=self.proj, pdl=True)
             rms_norm_residual(self.h, layer.post_norm, d.eps, delta=self.proj, h_out=self.h2, x_out=self.x, pdl=True)
             w4a16_gate_up_silu(self.x, *layer.gate_up, group=d.group, out=self.act, pdl=True)
@@ -209,7 +225,8 @@ class Qwen3Decoder:
         """Embed self.tokens, run every layer, pick the next tokens (greedy), advance the lengths."""
         d = self.dims
         pos = self.lengths.to(torch.int64)
-        cos, sin = rope_cos_sin(pos, d.head_dim, d.rope_theta, torch.bfloat16)
+        # (bf16 pages read the fp32 table of every position instead: `rope_kv_append`)
+        cos, sin = (None, None) if self.rope else rope_cos_sin(pos, d.head_dim, d.rope_theta, torch.bfloat16)
         write_blocks = torch.gather(self.block_table, 1, (pos // self.block_size)[:, None]).to(torch.int32)
         write_offsets = (pos % self.block_size).to(torch.int32)[:, None]
         lengths_after = self.lengths + 1
@@ -251,7 +268,7 @@ class Qwen3Decoder:
         """KV bytes one step reads: every layer, every sequence's visible tokens, K and V."""
         d = self.dims
         tokens = int(self.lengths.sum().item()) + self.batch
-        return d.layers * tokens * 2 * d.kv_heads * d.head_dim
+        return d.layers * tokens * 2 * d.kv_heads * d.head_dim * (2 if self.kv_kind == "bf16" else 1)
 
     def weight_bytes_per_step(self) -> int:
         """INT4 weights (codes + fp16 scales + 4-bit zeros) of every layer, plus the bf16 LM head."""

@@ -1,4 +1,5 @@
-"""A paged KV cache for nanoserve that stores FP8 or INT8 codes and attends over them with this package's kernels.
+"""A paged KV cache for nanoserve that stores FP8 or INT8 codes, or 16-bit values, and attends over them with this package's
+kernels.
 
 The reference has two caches that meet at this seam:
 
@@ -20,9 +21,12 @@ it unchanged:
   through the block table. By default one fused launch (`kv_attention.attend`: split-K with the merge in the same
   kernel); with `decode=` a `DecodeFn` such as `kv_attention.decode_attention` returns per-split partials that
   `merge_partials` joins, as the reference's cache does.
-- **prefill read** (several new tokens): the unfused path, as in the reference (`integration/kv_cache.py:187-192`):
-  the pages are gathered and dequantized, then a causal GQA attention runs in PyTorch. The decode kernel is a
-  decode kernel; prefill is compute-bound and not where the cache's bytes matter.
+- **prefill read** (several new tokens) of `attend` over FP8 / INT8 pages: the unfused path, as in the reference
+  (`integration/kv_cache.py:187-192`): the pages are gathered and dequantized, then a causal GQA attention runs in
+  PyTorch. Over 16-bit pages ("bf16", "f16") it is `prefill_attend`, which reads the pages in place.
+- **`rotate_and_attend`** takes q, k, v as the projections give them, for pages of any kind: `rope_kv_append` normalises and
+  rotates q and k and stores k and v in one launch, then the decode or the prefill kernel reads the pages in place, with
+  the score caps, windows and biases that the model uses.
 
 Every tensor lives on one CUDA device; there is no CPU path.
 """
@@ -39,10 +43,14 @@ import torch
 
 from bpt_b200._lib import require_cuda
 from bpt_b200.kernels.kv_attention import PagedQuantKV, attend, merge_partials
-from bpt_b200.kernels.kv_write import quantize_kv_paged
+from bpt_b200.kernels.kv_write import quantize_kv_paged, rope_kv_append
+from bpt_b200.kernels.prefill_attention import prefill_attend
 
 # (q [B, Hq, D], kv, lengths [B], scale, tokens) -> (out [B, Hq, S, D], lse [B, Hq, S]), integration/kv_cache.py:38-39
 DecodeFn = Callable[..., tuple[torch.Tensor, torch.Tensor]]
+
+
+_SIXTEEN = {"bf16": torch.bfloat16, "f16": torch.float16}
 
 
 class OutOfBlocksError(RuntimeError):
@@ -63,18 +71,18 @@ class PagedQuantMeta:
 
 
 class PagedQuantizedKVCache:
-    """Paged FP8 / INT8 KV cache with the `attend` seam of the reference's quantized cache.
+    """Paged FP8 / INT8 / 16-bit KV cache with the `attend` seam of the reference's quantized cache.
 
     cfg: anything with `num_layers`, `num_kv_heads` and `head_dim` (the reference's `ModelConfig`,
     `engine/config.py:15-27`). kind "fp8": `k_scale` / `v_scale` are the per-tensor scales (x / scale is stored);
-    kind "int8": the scales are per (token, KV head) and computed on write.
+    kind "int8": the scales are per (token, KV head) and computed on write; kind "bf16" / "f16": the values themselves.
     """
 
     def __init__(self, cfg: Any, *, num_blocks: int, block_size: int = 16, kind: str = "fp8",
                  k_scale: float = 1.0, v_scale: float = 1.0, device: torch.device | str = "cuda",
                  decode: DecodeFn | None = None):
-        if kind not in ("fp8", "int8"):
-            raise ValueError(f"kind must be 'fp8' or 'int8', got {kind!r}")
+        if kind not in ("fp8", "int8", "bf16", "f16"):
+            raise ValueError(f"kind must be 'fp8', 'int8', 'bf16' or 'f16', got {kind!r}")
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise ValueError("PagedQuantizedKVCache lives on a CUDA device: its kernels have no CPU path")
@@ -87,6 +95,9 @@ class PagedQuantizedKVCache:
                 return PagedQuantKV("fp8", torch.zeros(shape, dtype=torch.uint8, device=self.device),
                                     torch.zeros(shape, dtype=torch.uint8, device=self.device), empty_table, block_size,
                                     float(k_scale), float(v_scale))
+            if kind in _SIXTEEN:
+                return PagedQuantKV(kind, torch.zeros(shape, dtype=_SIXTEEN[kind], device=self.device),
+                                    torch.zeros(shape, dtype=_SIXTEEN[kind], device=self.device), empty_table, block_size)
             return PagedQuantKV("int8", torch.zeros(shape, dtype=torch.int8, device=self.device),
                                 torch.zeros(shape, dtype=torch.int8, device=self.device), empty_table, block_size,
                                 torch.ones(shape[:3], dtype=torch.float16, device=self.device),
@@ -157,7 +168,13 @@ class PagedQuantizedKVCache:
         raise NotImplementedError("a quantized cache never returns float keys and values: use attend()")
 
     def _append(self, layer: int, k: torch.Tensor, v: torch.Tensor, meta: PagedQuantMeta) -> None:
-        """Quantize k, v [B, Hkv, Q, D] into the layer's pools at the metadata's slots (one launch)."""
+        """Quantize k, v [B, Hkv, Q, D] into the layer's pools at the metadata's slots (one launch; 16-bit pools: a scatter)."""
+        kv = self.layers[layer]
+        if self.kind in _SIXTEEN:
+            at = (meta.write_blocks.long(), meta.write_offsets.long())
+            kv.k_pool[at] = k.transpose(1, 2).to(kv.k_pool.dtype)
+            kv.v_pool[at] = v.transpose(1, 2).to(kv.v_pool.dtype)
+            return
         quantize_kv_paged(k, v, self.layers[layer], meta.write_blocks, meta.write_offsets)
 
     def layer_view(self, layer: int, meta: PagedQuantMeta) -> PagedQuantKV:
@@ -180,6 +197,8 @@ class PagedQuantizedKVCache:
                 return attend(query, kv, meta.lengths, scale, tokens=meta.kv_len)[:, :, None].to(q.dtype)
             out, lse = self.decode(query, kv, meta.lengths, scale, tokens=meta.kv_len)
             return merge_partials(out, lse)[:, :, None].to(q.dtype)
+        if self.kind in _SIXTEEN and q.dtype == _SIXTEEN[self.kind]:
+            return self._prefill(layer, q.transpose(1, 2).flatten(0, 1), meta, scale)
         # prefill: the unfused path (gather, dequantize, causal GQA attention)
         keys, values = self.dequantized(layer, meta)
         slots = torch.arange(meta.kv_len, device=q.device)
@@ -188,6 +207,33 @@ class PagedQuantizedKVCache:
         keys = keys.to(q.dtype).repeat_interleave(rep, dim=1)
         values = values.to(q.dtype).repeat_interleave(rep, dim=1)
         return torch.nn.functional.scaled_dot_product_attention(q, keys, values, attn_mask=mask, scale=scale)
+
+    def _prefill(self, layer: int, q: torch.Tensor, meta: PagedQuantMeta, scale: float, **scores) -> torch.Tensor:
+        """q [B * Q, Hq, D] over the pages, every token at its own position -> [B, Hq, Q, D]."""
+        b, q_len = meta.positions.shape
+        cu = torch.arange(0, b * q_len + 1, q_len, dtype=torch.int32, device=q.device)
+        out = prefill_attend(q, self.layer_view(layer, meta), cu, meta.lengths, scale, positions=meta.positions.flatten(),
+                             tokens=meta.kv_len, **scores)
+        return out.view(b, q_len, *out.shape[1:]).transpose(1, 2)
+
+    def rotate_and_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: PagedQuantMeta,
+                          scale: float, cos: torch.Tensor, sin: torch.Tensor, *, q_norm: torch.Tensor | None = None,
+                          k_norm: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                          softcap: float = 0.0, window: int = 0, alibi_slopes: torch.Tensor | None = None) -> torch.Tensor:
+        """The projections' q [B, Hq, Q, D], k and v [B, Hkv, Q, D] (f16 or bf16), not rotated: store this step, then attend.
+
+        cos, sin: fp32 tables [positions, R / 2] (`kv_write.rope_table`), read at the metadata's positions. Norm weights,
+        rotation and the scores' options are those of `rope_kv_append`, `attend` and `prefill_attend`; 16-bit pages take
+        queries of their own dtype where several tokens come at once. Returns [B, Hq, Q, D] in q's dtype.
+        """
+        kv = self.layer_view(layer, meta)
+        tokens = [x.transpose(1, 2).flatten(0, 1) for x in (q, k, v)]  # [B * Q, H, D]
+        turned = rope_kv_append(*tokens, kv, meta.positions, cos, sin, meta.write_blocks, meta.write_offsets, q_norm=q_norm,
+                                k_norm=k_norm, eps=eps, interleaved=interleaved)
+        scores = {"softcap": softcap, "window": window, "alibi_slopes": alibi_slopes}
+        if meta.q_len > 1:
+            return self._prefill(layer, turned, meta, scale, **scores)
+        return attend(turned, kv, meta.lengths, scale, tokens=meta.kv_len, out=torch.empty_like(turned), **scores)[:, :, None]
 
     def dequantized(self, layer: int, meta: PagedQuantMeta) -> tuple[torch.Tensor, torch.Tensor]:
         """Every row's first kv_len tokens, gathered through the block table and dequantized to fp32:
@@ -198,7 +244,9 @@ class PagedQuantizedKVCache:
 
         def gather(pool, scales):
             blocks = pool[idx]  # [B, n_blocks, block_size, Hkv, D]
-            if kv.kind == "fp8":
+            if kv.kind in _SIXTEEN:
+                vals = blocks.float()
+            elif kv.kind == "fp8":
                 vals = blocks.view(torch.float8_e4m3fn).float() * float(scales)
             else:
                 vals = blocks.float() * scales[idx].float()[..., None]
