@@ -8,8 +8,8 @@
 //                memory.
 // Two warpgroups. One does the softmax, a thread per row, so that neither maximum nor sum crosses threads. Of the other, one
 // warp issues the products and the rest bring pages into a ring of shared-memory stages (K and V of a step in stages of their
-// own): 16-bit pages as TMA boxes, one warp, a box per page, pages past the visible keys out of the map's range
-// and so zero; E4M3 pages through registers, where the codes become f16. While the softmax takes a step's powers, the tensor
+// own) as TMA boxes, pages past the visible keys out of the map's range and so zero: 16-bit pages as the products take them, a
+// box per page, a warp for K and one for V; E4M3 codes by one warp, and through the registers of two to f16. While the softmax takes a step's powers, the tensor
 // cores take the products of the step before and the scores of the next. At heads of 64 and 128 two CTAs share an SM, so that
 // one's loads, waits and stores run under the other's powers.
 //
@@ -26,7 +26,6 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <cstring>
 #include <type_traits>
 
 #include "paged_prefill.cuh"
@@ -49,7 +48,7 @@ struct TcShape {
   static constexpr int kStage = kKeys * D * 2;  // [group of 8 keys][part of 64 dims][8][128 bytes, swizzled]
   static constexpr int kGroup = 8 * D * 2;
   static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
-  static constexpr int kBars = 2 * kStages + 10;  // an even number: what follows them starts on 16 bytes
+  static constexpr int kBars = ((kIs16<KIND> ? 2 : 3) * kStages + 12) / 2 * 2;  // (even: what follows starts on 16 bytes)
   static constexpr int kSmem = kQ + kStages * kStage + kBars * 8 + kFlagSteps * 4 + 16;
   static_assert(D == 256 || kSmem <= 113 * 1024, "two CTAs per SM");
   static constexpr int kProducers = kIs16<KIND> ? 2 : 3;  // warps
@@ -451,6 +450,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* o_done = p_full + 2;     // [2] that buffer's P V is in O
   uint64_t* drained = o_done + 2;    // all products are done
   uint64_t* edge = drained + 1;      // a stage whose rows are only partly visible has landed
+  uint64_t* raw = edge + 1;          // [NS] a stage's codes have landed (E4M3)
   uint32_t* flags = reinterpret_cast<uint32_t*>(bars + S::kBars);  // [kFlagSteps] a bit per 8 keys of a block out of range
   int* range = reinterpret_cast<int*>(flags + kFlagSteps);          // the smallest lo, the largest hi
   uint32_t* slot = reinterpret_cast<uint32_t*>(range + 2);          // tensor-memory address
@@ -461,10 +461,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (tid == 0) record_error(kDevErrTimeout);
     return;
   }
+  if (tid == 32 || tid == 64)  // (a first box waits for its map)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tid == 32 ? &tm_k : &tm_v)) : "memory");
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], kIs16<KIND> ? 1 : S::kProducers);
+      mbar_init(&full[i], kIs16<KIND> ? 1 : 2);
       mbar_init(&empty[i], 1);
+      if constexpr (!kIs16<KIND>) mbar_init(&raw[i], 1);
     }
     mbar_init(q_full, 4);
     for (int i = 0; i < 2; ++i) {
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool v = w == 1;
         const int pages = 1 << per_log2, nowhere = int(a.src.num_blocks << (a.src.bs_log2 - 3));  // a group behind the pool
         const CUtensorMap* map = v ? &tm_v : &tm_k;
-        uint32_t edges = 0;
+        uint32_t edges = 0, asked = 0, laps = 0;  // bits of stages: a copy was asked for, the lap of the last
         int n = v ? min(2, steps) : 0;  // the item of step j
         for (int i = 0; i < n; ++i) in.next();
         for (int j = 0; j < steps; ++j) {
@@ -614,77 +617,97 @@ __global__ void __launch_bounds__(kThreads, 2)
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[in.stage]);
           }
+          asked |= 1u << in.stage;
+          laps = (laps & ~(1u << in.stage)) | in.lap << in.stage;
           const int ahead = v ? (j == steps - 2 ? 1 : 2) : (j == 0 ? 1 : 2);
           n += ahead;
           in.next();
           if (ahead == 2) in.next();
         }
+        // (a wait ran out: the copies asked for land before the CTA ends)
+        if (!ok)
+          for (int i = 0; i < NS; ++i)
+            if (asked >> i & 1u) (void)mbar_wait(&full[i], laps >> i & 1u);
       } else {
-        // Codes go through registers: 16 codes a load, an f16 each into the stage. Warp w takes the slabs of 8 rows w, w + 3, ...;
-        // an item's loads are issued an item ahead, without conditions, so that all are in flight at once (what is not taken
-        // reads the pool's start and is dropped).
-        constexpr int CPR = D / 16, PER = CPR * 8 / 32, SLABS = 3;  // chunks of a row; a lane's chunks of a slab
-        const int64_t row_bytes = int64_t(a.src.Hkv) * S::kRowBytes, head_bytes = int64_t(hk) * S::kRowBytes;
-        uint4 codes[2][SLABS * PER];
-        uint32_t taken[2];
+        // Warp 6 brings the codes, 8 keys a TMA box, a lane a box, into the second half of the place that their f16 values
+        // take; warps 4 and 5 then take four of the eight places each, two at a time: codes into registers, f16 back. (One
+        // warp that both brought and converted left the ring empty while it waited: two chunks of about 1,800 tokens 357 us, not 236.)
+        constexpr int CPR = D / 16, PER = CPR * 8 / 32;  // 16-byte chunks of a key's codes; a lane's of 8 keys
         auto order = [&](int n, int& j, bool& v) {
           v = is_v(n) || n >= 2 * steps - 1;
           j = n >= 2 * steps - 1 ? steps - 1 : step_of(n);
         };
-        auto load = [&](int n, uint4 (&x)[SLABS * PER], uint32_t& got) {
-          int j;
-          bool v;
-          order(n, j, v);
-          const int blk = page_of(j, v);
-          if (!v && w == 0) flag(j, blk);
-          const uint8_t* pool = v ? a.src.v_pool : a.src.k_pool;
-          const int key0 = from + kKeys * (steps - 1 - j);
-          got = 0;
-#pragma unroll
-          for (int i = 0; i < SLABS; ++i) {
-            const int slab = w + 3 * i;
-            const int blk8 = __shfl_sync(0xffffffffu, blk, (slab & 7) >> (page_log2 - 3));
-            const int64_t slot0 = (int64_t(max(blk8, 0)) << a.src.bs_log2) + ((key0 + 8 * (slab & 7)) & ((1 << a.src.bs_log2) - 1));
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-              const int r = (lane + 32 * e) / CPR, c = (lane + 32 * e) % CPR, key = key0 + 8 * slab + r;
-              const bool take = slab < 8 && key >= take_from && key < to && blk8 >= 0;
-              const uint8_t* src = pool + (take ? (slot0 + r) * row_bytes + head_bytes : 0);
-              x[i * PER + e] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-              got |= (take ? 1u : 0u) << (i * PER + e);
-            }
-          }
-        };
-        auto store = [&](const uint4 (&x)[SLABS * PER], uint32_t got) {
-#pragma unroll
-          for (int i = 0; i < SLABS; ++i) {
-            if (w + 3 * i >= 8) break;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-              const int rr = 8 * (w + 3 * i) + (lane + 32 * e) / CPR, c = (lane + 32 * e) % CPR;
-              const uint4 v4 = x[i * PER + e];
-              const uint32_t keep = got >> (i * PER + e) & 1u ? 0xFFFFFFFFu : 0u;
-              const uint32_t u[4] = {v4.x & keep, v4.y & keep, v4.z & keep, v4.w & keep};
-              uint8_t* dst = ring + in.stage * S::kStage + (rr >> 3) * S::kGroup + ((2 * c) >> 3) * 1024 + (rr & 7) * 128;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint2 x0 = codes_to_f16<KIND>(u[2 * h]), x1 = codes_to_f16<KIND>(u[2 * h + 1]);
-                *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ (rr & 7)) << 4)) = make_uint4(x0.x, x0.y, x1.x, x1.y);
-              }
-            }
-          }
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[in.stage]);
-        };
-        if (items > 0) load(0, codes[0], taken[0]);
-        for (int n = 0; n < items && ok; n += 2) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (n + h + 1 < items) load(n + h + 1, codes[h ^ 1], taken[h ^ 1]);
-            if (n + h >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
+        if (w == 2) {
+          const int nowhere = int(a.src.num_blocks << (a.src.bs_log2 - 3));  // a group behind the pool
+          int n = 0;
+          for (; n < items; ++n) {
+            int j;
+            bool v;
+            order(n, j, v);
+            const int blk = page_of(j, v);
+            if (!v) flag(j, blk);
+            const int key = from + kKeys * (steps - 1 - j) + 8 * (lane & 7);
+            const int blk8 = __shfl_sync(0xffffffffu, blk, (lane & 7) >> (page_log2 - 3));
+            const int group =
+                blk8 >= 0 ? (blk8 << (a.src.bs_log2 - 3)) + ((key & ((1 << a.src.bs_log2) - 1)) >> 3) : nowhere;
+            if (n >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[in.stage], in.lap ^ 1u));
             if (!ok) break;
-            store(codes[h], taken[h]);
+            if (lane == 0) mbar_arrive_expect_tx(&raw[in.stage], kKeys * D);
+            __syncwarp();
+            if (lane < 8)
+              tma_box(smem_u32(ring + in.stage * S::kStage) + lane * S::kGroup + 8 * D, v ? &tm_v : &tm_k, hk, group,
+                      &raw[in.stage]);
+            in.next();
+          }
+          // (a wait ran out: the copies asked for land before the CTA ends)
+          if (!ok)
+            for (int i = 0; i < NS; ++i)
+              if (i < n) (void)mbar_wait(&raw[i], i < in.stage ? in.lap : in.lap ^ 1u);
+        } else {
+          for (int n = 0; n < items; ++n) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&raw[in.stage], in.lap));
+            if (!ok) break;
+            int j;
+            bool v;
+            order(n, j, v);
+            const int key0 = from + kKeys * (steps - 1 - j);
+            const bool partly = v && (key0 < take_from || key0 + kKeys > to);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              uint8_t* const rows = ring + in.stage * S::kStage + (4 * w + i) * S::kGroup;
+              uint4 x[2][PER];
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                  x[k][e] = *reinterpret_cast<const uint4*>(rows + k * S::kGroup + 8 * D + (lane + 32 * e) * 16);
+              if (partly) {  // values next to the visible ones may be anything: zeros
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int e = 0; e < PER; ++e) {
+                    const int key = key0 + 8 * (4 * w + i + k) + (lane + 32 * e) / CPR;
+                    if (key < take_from || key >= to) x[k][e] = make_uint4(0u, 0u, 0u, 0u);
+                  }
+              }
+              __syncwarp();  // the warp has these codes: their places may be written
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                  const int r = (lane + 32 * e) / CPR, c = (lane + 32 * e) % CPR;
+                  const uint32_t u[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
+                  uint8_t* dst = rows + k * S::kGroup + ((2 * c) >> 3) * 1024 + r * 128;
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const uint2 x0 = codes_to_f16<KIND>(u[2 * h]), x1 = codes_to_f16<KIND>(u[2 * h + 1]);
+                    *reinterpret_cast<uint4*>(dst + ((((2 * c + h) & 7) ^ r) << 4)) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+                  }
+                }
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[in.stage]);
             in.next();
           }
         }
@@ -769,24 +792,26 @@ int launch_tc(const PrefillArgs& a, int64_t tiles, int flags, cudaStream_t strea
   const int st = set_max_smem_once(kernel, S::kSmem, ready);
   if (st) return st;
   CUtensorMap tm_k, tm_v;
-  memset(&tm_k, 0, sizeof(tm_k));
-  memset(&tm_v, 0, sizeof(tm_v));
-  if constexpr (kIs16<KIND>) {
-    auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
-    if (!encode) return set_error(BPT_ERR_UNSUPPORTED, "paged prefill: the driver has no tensor-map encoder");
-    const int64_t groups = a.src.num_blocks << (a.src.bs_log2 - 3);
-    BPT_REQUIRE(groups < (1ll << 31) - 1, BPT_ERR_UNSUPPORTED, "paged prefill: a pool of %lld tokens", (long long)groups * 8);
-    const cuuint64_t row = cuuint64_t(S::kRowBytes), token = row * a.src.Hkv;
-    const cuuint64_t dims[5] = {64, 8, D / 64, cuuint64_t(a.src.Hkv), cuuint64_t(groups)};
-    const cuuint64_t strides[4] = {token, 128, row, 8 * token};
-    const cuuint32_t box[5] = {64, 8, D / 64, 1, 1u << (std::min(a.src.bs_log2, 6) - 3)}, ones[5] = {1, 1, 1, 1, 1};
-    const CUtensorMapDataType type = KIND == BPT_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    for (int i = 0; i < 2; ++i) {
-      const CUresult res = encode(i ? &tm_v : &tm_k, type, 5, const_cast<uint8_t*>(i ? a.src.v_pool : a.src.k_pool), dims, strides,
-                                  box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-      if (res != CUDA_SUCCESS) return set_error(BPT_ERR_INVALID, "paged prefill: tensor map: error %d", int(res));
-    }
+  auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+  if (!encode) return set_error(BPT_ERR_UNSUPPORTED, "paged prefill: the driver has no tensor-map encoder");
+  const int64_t groups = a.src.num_blocks << (a.src.bs_log2 - 3);
+  BPT_REQUIRE(groups < (1ll << 31) - 1, BPT_ERR_UNSUPPORTED, "paged prefill: a pool of %lld tokens", (long long)groups * 8);
+  // 16-bit pages: a box has a row's parts of 64 dims one after another, swizzled; codes: rows as they are, 8 a box
+  constexpr bool k16 = kIs16<KIND>;
+  const cuuint64_t row = cuuint64_t(S::kRowBytes), token = row * a.src.Hkv;
+  const cuuint64_t dims[5] = {k16 ? 64 : D, 8, k16 ? D / 64 : 1, cuuint64_t(a.src.Hkv), cuuint64_t(groups)};
+  const cuuint64_t strides[4] = {token, k16 ? 128 : row, row, 8 * token};
+  const cuuint32_t box[5] = {k16 ? 64 : D, 8, k16 ? D / 64 : 1, 1, k16 ? 1u << (std::min(a.src.bs_log2, 6) - 3) : 1u};
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  const CUtensorMapDataType type = KIND == BPT_KV_FP8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : KIND == BPT_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int i = 0; i < 2; ++i) {
+    const CUresult res = encode(i ? &tm_v : &tm_k, type, 5, const_cast<uint8_t*>(i ? a.src.v_pool : a.src.k_pool), dims, strides,
+                                box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                k16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (res != CUDA_SUCCESS) return set_error(BPT_ERR_INVALID, "paged prefill: tensor map: error %d", int(res));
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles), unsigned(a.src.Hkv), unsigned(a.n_splits));
