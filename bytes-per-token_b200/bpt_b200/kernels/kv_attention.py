@@ -9,7 +9,7 @@ Mirrors `src/fastserve/kernels/kv_attention.py` (ish-codes-magic/bytes-per-token
 
 `kv` is either the reference's contiguous KIVI cache (any object with QuantKV's fields: bits, group, k_codes,
 v_codes, k_scale, k_zero, v_scale, v_zero; `QuantKV` below has them) or a `PagedQuantKV`: the paged FP8 / INT8
-pool this build adds, in the reference's paged layout [num_blocks, block_size, Hkv, D]
+pool this package adds (and a bf16 / f16 one), in the reference's paged layout [num_blocks, block_size, Hkv, D]
 (`src/fastserve/engine/kv_cache.py:108`). The same functions serve both, so the cache that calls them
 (`QuantizedKVCache.attend`, `integration/kv_cache.py:160-185`) does not change.
 

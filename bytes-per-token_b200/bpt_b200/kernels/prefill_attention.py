@@ -30,7 +30,8 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
     - `softcap` c > 0: scores become c * tanh(score / c); `alibi_slopes` [Hq]: they fall by slope * |p - j|.
 
     A token that sees no key gets zeros; rows of q that belong to no sequence leave `out` as it is. q is f16 or bf16, of the
-    pages' own dtype where they are 16-bit. `tokens` bounds the longest length (no host sync on lengths.max()).
+    pages' own dtype where they are 16-bit. A value that is NaN or infinite reaches every token of its sequence that shares a
+    tile of rows with one that sees it; where no token sees it, it reaches none. `tokens` bounds the longest length (no host sync on lengths.max()).
     """
     device = require_cuda(q, kv.k_pool, kv.v_pool, kv.block_table, cu_seqlens, lengths, positions, alibi_slopes, key_starts,
                           prefix_lens, out, workspace)

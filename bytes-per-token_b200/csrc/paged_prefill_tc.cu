@@ -20,6 +20,14 @@
 // by an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
 // times per row, if at all.
 //
+// Measured (B200: 1,646 TFLOP/s bf16 by library product, 6,558 GB/s copy): a prompt of 8,192 tokens, 32 + 8 heads of 128,
+// bf16: 486 us back to back, 1,131 TFLOP/s. There the exponentials (16 a clock per SM) and the products ask for about the same
+// time, and each step's chain S -> P -> O has to hide behind the other CTA's. Ragged batches are bound by what is not the loop:
+// about 9 us per CTA for its map, first pages, queries and rows out. 256 rows in one CTA per SM took 713 us for that
+// prompt, pages by cp.async warps 1,128, a box per 64 dims 687, K and V by one warp 565; a polynomial in place of a
+// quarter of the exponentials 576 against 572. E4M3: two chunks of about 1,800 tokens over 4,500, 16 + 4 heads of 128, 236 us
+// (bf16 157): the two converting warps.
+//
 // Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
 // and the CTA still awaits its copies and products, frees its tensor memory and returns.
 #define BPT_WHOLE_PROGRAM  // compiled without relocatable device code

@@ -4,8 +4,8 @@
 //   s_j = cap tanh(scale q.k_j / cap) - slope |p - j|,  out = sum_j softmax(s)_j v_j  over  max(0, start, p - window + 1) <= j
 //   <= p, p = length - 1; no visible key gives 0.
 //
-// Bound by memory: each visible key and value is read once. Work is cut into equal shares, one per warp of a full GPU (8
-// warps per SM): a warp takes a contiguous range of groups of 16 keys, of one KV head (and eight of its query heads), across the
+// Bound by memory: each visible key and value is read once. Work is cut into equal shares, one per warp of a full GPU (two
+// CTAs of four warps an SM; one CTA where rows of 512 bytes leave no room): a warp takes a contiguous range of groups of 16 keys, of one KV head (and eight of its query heads), across the
 // sequences of the batch, so that ragged lengths leave no SM idle; the warps of a CTA hold the heads of one range, whose rows
 // lie next to each other in the pages. A warp never waits for another: it has its own ring of cp.async stages, running on
 // into its next sequence, and its own running maximum and sum. A group's rows arrive whole (D elements of one head); rows
@@ -17,6 +17,11 @@
 //
 // A sequence inside one range goes straight to out. One that crosses ranges leaves a part per range, and a second kernel,
 // launched dependently, joins them.
+//
+// Measured (B200, 6,558 GB/s copy): f16, 8 sequences of 32,768, 32 query and 8 KV heads of 128, capped: 186 us, 5.8 TB/s;
+// bf16, 32 sequences of 512 to 4,096: 63 us, 4.8 TB/s (start and join); E4M3 in a window of 4,096, 17 sequences: 33 us, bound
+// by the codes' conversion; one sequence of 1,000: 15 us, two launches and a dependent chain of loads. A ring of six stages
+// with one CTA an SM took 73 us for the batch of 32, twelve warps an SM 37 for the E4M3 one.
 #include <algorithm>
 
 #include "paged_read.cuh"
@@ -26,7 +31,8 @@ namespace bpt {
 namespace {
 
 constexpr int kWarps = 4;          // per CTA, at most
-constexpr int kStartCost = 2;      // what a sequence's start costs a range, in groups of 16 keys
+// What a sequence's start costs a range, in groups of 16 keys. (8: one sequence of 1,000 takes 20.6 us instead of 14.7.)
+constexpr int kStartCost = 2;
 constexpr int kLeastShare = 2;     // groups; a smaller share would be all start and join
 
 struct ReadArgs {
