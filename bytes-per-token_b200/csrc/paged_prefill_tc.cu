@@ -429,7 +429,7 @@ __device__ __forceinline__ void softmax_rows(const PrefillArgs& a, const TileAt&
       const int code = __shfl_sync(0xffffffffu, row.code, rr);
       if (code >= 0 && ok) {
         uint8_t* dst = parts > 1 ? reinterpret_cast<uint8_t*>(a.part_out) + part0 + int64_t(rr) * (4 * D) + half * (2 * D)
-                                 : static_cast<uint8_t*>(a.out) + out0 + ((code >> 16) * a.Hq + (code & 0xFFFF)) * (2 * D);
+                                 : static_cast<uint8_t*>(a.out) + out0 + int64_t((code >> 16) * a.Hq + (code & 0xFFFF)) * (2 * D);
         *reinterpret_cast<uint4*>(dst + 16 * c) = x;
       }
     }
