@@ -299,7 +299,7 @@ def decode_attention(
     `key_starts` (paged caches only): see `attend`.
     """
     del num_warps
-    if _any_format(kv, softcap, window, alibi_slopes, key_starts):
+    if _any_format(q, kv, softcap, window, alibi_slopes, key_starts):
         return _paged_read(q, kv, lengths, scale, tokens=tokens, split=split, softcap=softcap, window=window,
                            alibi_slopes=alibi_slopes, key_starts=key_starts, partials=True)
     device = require_cuda(q, lengths, kv.k_codes if not isinstance(kv, PagedQuantKV) else kv.k_pool)
@@ -403,14 +403,20 @@ def _read_scratch_bytes(hq: int, hkv: int, d: int, code: int, device: torch.devi
     return int(lib().bpt_paged_read_workspace_bytes(hq, hkv, d, code))
 
 
-def _any_format(kv, softcap, window, alibi_slopes, key_starts) -> bool:
-    """Whether a call takes the any-format read: 16-bit pages, or a score option over pages of any kind."""
+def _any_format(q, kv, softcap, window, alibi_slopes, key_starts) -> bool:
+    """Whether a call takes the any-format read: 16-bit pages, or over pages of any kind a score option, pages of other than 16
+    tokens, or numbers of heads that the kernels for 8-bit codes alone do not take."""
     options = bool(softcap) or bool(window) or alibi_slopes is not None or key_starts is not None
     if not isinstance(kv, PagedQuantKV):
         if options:
             raise ValueError("softcap, window, alibi_slopes and key_starts need a paged cache")
         return False
-    return options or kv.kind in ("bf16", "f16")
+    if options or kv.kind in ("bf16", "f16"):
+        return True
+    if q.dim() != 3 or kv.k_pool.dim() != 4 or not kv.k_pool.shape[2] or q.shape[1] % kv.k_pool.shape[2]:
+        return False
+    block_size, heads = kv.k_pool.shape[1:3]
+    return block_size != 16 or heads > 16 or q.shape[1] // heads not in (1, 2, 4, 8)
 
 
 def attend(
@@ -434,12 +440,13 @@ def attend(
     launch; `kv_ready=True` adds the promise that the lengths, block table and pools are not written by the
     kernel this call follows, so the persistent kernel starts copying pages before it waits on that kernel.
 
-    Paged caches of any kind take, and 16-bit pages ("bf16", "f16") always run, the any-format kernel with: `softcap` c > 0
+    Paged caches of any kind take, and 16-bit pages ("bf16", "f16") or pages of other than 16 tokens always run, the any-format
+    kernel with: `softcap` c > 0
     (scores c * tanh(score / c)), `window` w > 0 (only the last w keys are seen), `alibi_slopes` fp32 [Hq] (a score falls
     by slope * distance) and `key_starts` int32 [B] (the first key each sequence sees). A sequence that sees no key
     gives zeros.
     """
-    if _any_format(kv, softcap, window, alibi_slopes, key_starts):
+    if _any_format(q, kv, softcap, window, alibi_slopes, key_starts):
         return _paged_read(q, kv, lengths, scale, tokens=launch.get("tokens"), split=launch.get("split"), softcap=softcap,
                            window=window, alibi_slopes=alibi_slopes, key_starts=key_starts, out=out, workspace=workspace,
                            flags=_lib.FLAG_PDL if launch.get("pdl") else 0)

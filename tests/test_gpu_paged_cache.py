@@ -10,7 +10,8 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from tests.paged_reference import DTYPES, KINDS, assert_within, attention_row, visible
+from tests.paged_reference import DTYPES, KINDS, assert_within, attention_row, page_table, visible
+from tests.paged_reference import make_cache as filled_cache
 
 HQ, HKV, D = 4, 2, 128
 
@@ -164,6 +165,57 @@ def test_decode_step_over_bf16_pages_replays():
     assert torch.equal(eager.hidden, graphed.hidden)
     for a, b in zip(eager.layers, graphed.layers, strict=True):
         assert torch.equal(a.kv.k_pool, b.kv.k_pool) and torch.equal(a.kv.v_pool, b.kv.v_pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bs,d", [(128, 128), (1024, 64), (256, 256)])
+def test_pages_longer_than_a_step(kind, bs, d):
+    """Pages that a kernel reads in several steps, the last one of each sequence filled in part."""
+    from bpt_b200.kernels.kv_attention import attend
+    from bpt_b200.kernels.prefill_attention import prefill_attend
+
+    g = torch.Generator().manual_seed(bs)
+    seqs = [(300, 40), (0, 130), (1100, 3)]  # cached, new
+    lengths = [c + n for c, n in seqs]
+    table, blocks = page_table(lengths, bs, g)
+    kv, keys, values = filled_cache(kind, blocks, bs, HKV, d, table, g)
+    dtype, scale, vmax = DTYPES.get(kind, torch.bfloat16), 1 / math.sqrt(d), values.abs().max()
+    q = torch.randn(sum(n for _, n in seqs), HQ, d, generator=g).to(dtype)
+    cu = torch.tensor([0] + [n for _, n in seqs]).cumsum(0).to(torch.int32)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+
+    def row(b, x, pos, window):
+        pages = table[b, : -(-lengths[b] // bs)].long()
+        k, v = (y[pages].flatten(0, 1) for y in (keys, values))
+        lo, hi = visible(pos, lengths[b], window=window)
+        return attention_row(x.double(), k, v, pos, lo, hi, scale)
+
+    for window in (0, 90):
+        got = prefill_attend(q.cuda(), kv, cu.cuda(), n, scale, window=window)
+        want = torch.stack([row(b, q[int(cu[b]) + i], c + i, window) for b, (c, new) in enumerate(seqs) for i in range(new)])
+        assert_within(got, want, dtype, vmax, 8 if kind == "bf16" else 11)
+        last = q[cu[1:].long() - 1]
+        got = attend(last.cuda(), kv, n, scale, window=window)
+        want = torch.stack([row(b, last[b], lengths[b] - 1, window) for b in range(len(seqs))])
+        assert_within(got, want, torch.float32, vmax, 8 if kind == "bf16" else 11)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("hq,hkv", [(7, 1), (6, 2), (20, 20)])
+def test_numbers_of_heads_that_the_8_bit_kernels_leave(kind, hq, hkv):
+    from bpt_b200.kernels.kv_attention import attend, decode_attention, merge_partials
+
+    g = torch.Generator().manual_seed(hq)
+    lengths = [70, 0, 33]
+    table, blocks = page_table(lengths, 16, g)
+    kv, keys, values = filled_cache(kind, blocks, 16, hkv, D, table, g)
+    q, n = torch.randn(3, hq, D, generator=g), torch.tensor(lengths, dtype=torch.int32).cuda()
+    k, v = ([x[table[b, : max(1, -(-m // 16))].long()].flatten(0, 1) for b, m in enumerate(lengths)] for x in (keys, values))
+    want = torch.stack([attention_row(q[b].double(), k[b], v[b], m - 1, 0, m, 1 / math.sqrt(D)) for b, m in enumerate(lengths)])
+    for got in (attend(q.cuda(), kv, n, 1 / math.sqrt(D)), merge_partials(*decode_attention(q.cuda(), kv, n, 1 / math.sqrt(D)))):
+        assert_within(got, want, torch.float32, values.abs().max(), 11)
 
 
 def test_refusals_need_no_gpu():
