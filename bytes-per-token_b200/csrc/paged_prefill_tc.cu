@@ -489,7 +489,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     range[1] = 0;
     fence_mbar_init();
   }
-  pdl_launch_dependents();
   pdl_wait();
   const TileAt at = find_tile(a, kRows, int(blockIdx.x));
   const int64_t tile = int64_t(blockIdx.x) * a.src.Hkv + hk;
@@ -521,6 +520,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
+  // Every CTA of this grid holds its tensor memory (or has left) before any dependent CTA can start: one that allocated
+  // columns which a CTA here still needs would wait for this grid's end, and this grid for the columns.
+  pdl_launch_dependents();
   auto free_tmem = [&]() {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
   };
