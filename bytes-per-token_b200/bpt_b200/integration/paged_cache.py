@@ -43,7 +43,7 @@ import torch
 
 from bpt_b200._lib import require_cuda
 from bpt_b200.kernels.kv_attention import PagedQuantKV, attend, merge_partials
-from bpt_b200.kernels.kv_write import quantize_kv_paged, rope_kv_append
+from bpt_b200.kernels.kv_write import quantize_kv_paged, rope_kv_append, store_kv_paged
 from bpt_b200.kernels.prefill_attention import prefill_attend
 
 # (q [B, Hq, D], kv, lengths [B], scale, tokens) -> (out [B, Hq, S, D], lse [B, Hq, S]), integration/kv_cache.py:38-39
@@ -168,14 +168,9 @@ class PagedQuantizedKVCache:
         raise NotImplementedError("a quantized cache never returns float keys and values: use attend()")
 
     def _append(self, layer: int, k: torch.Tensor, v: torch.Tensor, meta: PagedQuantMeta) -> None:
-        """Quantize k, v [B, Hkv, Q, D] into the layer's pools at the metadata's slots (one launch; 16-bit pools: a scatter)."""
-        kv = self.layers[layer]
-        if self.kind in _SIXTEEN:
-            at = (meta.write_blocks.long(), meta.write_offsets.long())
-            kv.k_pool[at] = k.transpose(1, 2).to(kv.k_pool.dtype)
-            kv.v_pool[at] = v.transpose(1, 2).to(kv.v_pool.dtype)
-            return
-        quantize_kv_paged(k, v, self.layers[layer], meta.write_blocks, meta.write_offsets)
+        """Quantize (or round) k, v [B, Hkv, Q, D] into the layer's pools at the metadata's slots, in one launch."""
+        store = store_kv_paged if self.kind in _SIXTEEN else quantize_kv_paged
+        store(k, v, self.layers[layer], meta.write_blocks, meta.write_offsets)
 
     def layer_view(self, layer: int, meta: PagedQuantMeta) -> PagedQuantKV:
         """The layer's pools with this forward's block table: what the attention kernels read."""

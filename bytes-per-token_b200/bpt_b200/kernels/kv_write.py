@@ -4,6 +4,8 @@
   [B, Hkv, Q, D] to FP8 or INT8 and scatter them into a `PagedQuantKV` pool. The write of
   `PagedKVCache.update` (`src/fastserve/engine/kv_cache.py:150-161`) with the store of `kv/quant.py:40-48`
   in front of it.
+- `rope_kv_append` and `store_kv_paged`: the same slots of a paged cache of any kind, with rotation (and QK-norm) on the way
+  or as the keys and values come.
 - `quantize_kv(k, v, bits, group)`: the reference's `kernels/reference.py:132-160` (KIVI codes and grids) on
   the GPU, returning a `QuantKV`; `quantize_kv_into` writes whole groups into an existing cache, as
   `QuantizedKVCache._append` does (`integration/kv_cache.py:139-158`).
@@ -119,6 +121,34 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: PagedQ
             FLAG_PDL if pdl else 0, stream_of(device))
     check(st, "rope_kv_append")
     return q_out
+
+
+def store_kv_paged(k: torch.Tensor, v: torch.Tensor, kv: PagedQuantKV, write_blocks: torch.Tensor,
+                   write_offsets: torch.Tensor) -> None:
+    """Store k, v [B, Hkv, Q, D] (fp32, f16 or bf16) as they come at the slots write_blocks / write_offsets [B, Q] of a paged
+    cache, rounded once: the store of `rope_kv_append` alone, for pages that `quantize_kv_paged` does not write (16-bit ones).
+
+    A token with write_blocks -1 is padding and is not stored; a slot outside the pool is not written and is recorded.
+    """
+    device = require_cuda(k, v, kv.k_pool, kv.v_pool, write_blocks, write_offsets)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k and v must both be [B, Hkv, Q, D] of one dtype, got {tuple(k.shape)} in {k.dtype} and "
+                         f"{tuple(v.shape)} in {v.dtype}")
+    b, hkv, q, d = k.shape
+    code, ks, vs, kss, vss, nb, bs, pool_heads, pool_dim = pool_format(kv)
+    if hkv != pool_heads or d != pool_dim:
+        raise ValueError(f"k has {hkv} heads of {d}, the pool {pool_heads} of {pool_dim}")
+    if write_blocks.shape != (b, q) or write_offsets.shape != (b, q):
+        raise ValueError(f"write_blocks / write_offsets must be [{b}, {q}]")
+    with on_device(device):
+        k, k_stride = _aligned_rows(k.transpose(1, 2).flatten(0, 1))  # [B * Q, Hkv, D]
+        v, v_stride = _aligned_rows(v.transpose(1, 2).flatten(0, 1))
+        wb, wo = as_int32(write_blocks), as_int32(write_offsets)
+        st = _lib.rope_kv_append(
+            0, k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), 0, 0, k_stride[0], k_stride[1], v_stride[0], v_stride[1], b * q,
+            0, hkv, d, 0, 0, 0, 0, 0, False, 0, 0, 0.0, 0, wb.data_ptr(), wo.data_ptr(), kv.k_pool.data_ptr(),
+            kv.v_pool.data_ptr(), code, ks, vs, addr(kss), addr(vss), bs, nb, 0, stream_of(device))
+    check(st, "store_kv_paged")
 
 
 def empty_quant_kv(batch: int, kv_heads: int, tokens: int, head_dim: int, bits: int, group: int, device,

@@ -9,6 +9,8 @@
 // int8 codes under an fp16 scale per (token, KV head). Everything between the load and that one rounding is fp32: the
 // quantized codes are taken from the fp32 rotation, not from a 16-bit copy of it.
 //
+// Without queries (Hq 0) nothing rotates and positions are not read: keys and values are stored as they come.
+//
 // Bound by memory at many tokens and by launch and load latency at few: 16-byte loads and stores only. A lane owns 16 values
 // of a head, 8 and the 8 that rotate with them, so the rotation needs no shuffle; D / 16 lanes hold a head (4, 8 or 16 at D
 // 64, 128, 256) and a warp 32 / (D / 16) heads of one token at a time. A warp takes `per_warp` such groups of one
@@ -109,9 +111,9 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const AppendArgs a) {
   if (item >= uint32_t(a.T) * uint32_t(a.chunks)) return;  // whole warps leave together
   const int lane = threadIdx.x & 31, l = lane % LPH;
   const int t = int(item / uint32_t(a.chunks)), chunk = int(item - uint32_t(t) * uint32_t(a.chunks));
-  const int blk = a.blocks[t], off = a.offsets[t], pos = a.positions[t];
+  const int blk = a.blocks[t], off = a.offsets[t], pos = a.positions ? a.positions[t] : 0;
   if (blk == -1) return;  // a padding token
-  if (pos < 0 || pos >= a.table_rows) {
+  if (a.positions && (pos < 0 || pos >= a.table_rows)) {
     if (lane == 0) record_error(kDevErrPosition);
     return;
   }
@@ -324,7 +326,8 @@ extern "C" int bpt_rope_kv_append(const bpt_rope_kv_append_args* args) {
   void* const stream = args->stream;
   BPT_REQUIRE(T >= 0 && T < (1ll << 31), BPT_ERR_INVALID, "rope_kv_append: T=%lld", (long long)T);
   if (T == 0) return BPT_OK;
-  BPT_REQUIRE(q && k && v && positions && cos && sin && q_out && write_blocks && write_offsets && k_pool && v_pool,
+  const bool store_only = Hq == 0;
+  BPT_REQUIRE((store_only || (q && positions && cos && sin && q_out)) && k && v && write_blocks && write_offsets && k_pool && v_pool,
               BPT_ERR_INVALID, "rope_kv_append: null pointer argument");
   BPT_REQUIRE(dtype == BPT_DTYPE_F32 || dtype == BPT_DTYPE_F16 || dtype == BPT_DTYPE_BF16, BPT_ERR_INVALID,
               "rope_kv_append: dtype %d", dtype);
@@ -332,11 +335,13 @@ extern "C" int bpt_rope_kv_append(const bpt_rope_kv_append_args* args) {
               "rope_kv_append: kind %d", kind);
   BPT_REQUIRE(D == 64 || D == 128 || D == 256, BPT_ERR_UNSUPPORTED, "rope_kv_append: D=%lld (64, 128 or 256)",
               (long long)D);
-  BPT_REQUIRE(rotary >= 16 && rotary <= D && rotary % 16 == 0, BPT_ERR_UNSUPPORTED,
+  BPT_REQUIRE(!store_only || (rotary == 0 && !positions && !q_norm && !k_norm), BPT_ERR_INVALID,
+              "rope_kv_append: without queries nothing rotates (rotary 0, no positions, no norms)");
+  BPT_REQUIRE(store_only || (rotary >= 16 && rotary <= D && rotary % 16 == 0), BPT_ERR_UNSUPPORTED,
               "rope_kv_append: rotary=%lld must be a multiple of 16 from 16 to D", (long long)rotary);
-  BPT_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq < (1ll << 16) && Hkv < (1ll << 16), BPT_ERR_INVALID,
+  BPT_REQUIRE(Hq >= 0 && Hkv >= 1 && Hq < (1ll << 16) && Hkv < (1ll << 16), BPT_ERR_INVALID,
               "rope_kv_append: Hq=%lld Hkv=%lld", (long long)Hq, (long long)Hkv);
-  BPT_REQUIRE(table_rows >= 1, BPT_ERR_INVALID, "rope_kv_append: empty cos / sin table");
+  BPT_REQUIRE(store_only || table_rows >= 1, BPT_ERR_INVALID, "rope_kv_append: empty cos / sin table");
   BPT_REQUIRE(block_size >= 1 && block_size < (1ll << 31) && num_blocks >= 1 && num_blocks < (1ll << 31), BPT_ERR_INVALID,
               "rope_kv_append: bad pool shape");
   if (kind == BPT_KV_FP8)

@@ -323,7 +323,8 @@ int bpt_qk_norm_rope_kv_write(const void* qkv, int64_t ld, int64_t B, int64_t Hq
  * the fp32 rotation). A token whose write_blocks entry is -1 is padding: nothing of it is read or written. A position
  * outside the table (device error 4) skips the token; a block or offset out of range (2, 3) stores no k and v. Slots of
  * one call must be distinct. D in {64, 128, 256}, rotary a multiple of 16 from 16 to D; rows of q, k, v start
- * on 16 bytes. Replaces: rope.apply (engine/rope.py:31-43), q_norm / k_norm (engine/model.py:63-70) and the cache write
+ * on 16 bytes. Hq 0 stores k and v as they come: rotary 0, and positions, q_norm and k_norm NULL (q, q_out, cos and sin are
+ * not read). Replaces: rope.apply (engine/rope.py:31-43), q_norm / k_norm (engine/model.py:63-70) and the cache write
  * (engine/kv_cache.py:150-161) for any number of tokens and any of the cache's formats. */
 typedef struct {
   const void *q, *k, *v;
