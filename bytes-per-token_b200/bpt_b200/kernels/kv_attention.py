@@ -368,13 +368,15 @@ _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
 
 def attend_workspace(batch: int, q_heads: int, head_dim: int, n_splits: int, device: torch.device) -> torch.Tensor:
-    """A zeroed workspace for the fused split merge, cached per device and stream, grown on demand.
+    """A zeroed workspace for `attend` over a paged cache, cached per device and stream, grown on demand.
 
-    Each call of the fused kernel leaves the workspace's counters at zero again, so the buffer is reused as is.
+    It serves the fused split merge of these sizes and the any-format read of as many query heads (whose parts go behind the
+    merge's counters), in any order: each call leaves the counters at zero again, so the buffer is reused as is.
     Calls that overlap on the GPU (different streams) need different workspaces: the cache is keyed by stream.
     Under CUDA graph capture, size it before capturing (or pass `workspace=` to `attend`).
     """
     need = int(lib().bpt_paged_attend_workspace_bytes(batch, q_heads, head_dim, n_splits))
+    need = max(need, _most_read_scratch_bytes(q_heads, head_dim, device))
     key = (device.index or 0, stream_of(device))
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < need:
@@ -401,6 +403,13 @@ def _scratch(need: int, device: torch.device) -> torch.Tensor:
 @functools.cache
 def _read_scratch_bytes(hq: int, hkv: int, d: int, code: int, device: torch.device) -> int:
     return int(lib().bpt_paged_read_workspace_bytes(hq, hkv, d, code))
+
+
+@functools.cache
+def _most_read_scratch_bytes(hq: int, d: int, device: torch.device) -> int:
+    """The most that the any-format read of `hq` query heads takes, whatever the KV heads and the format: 8-bit pages, and the
+    fewest heads (as many ranges as the GPU has warps) or the most (a range's warps)."""
+    return max(_read_scratch_bytes(h, h, d, _lib.KV_FP8, device) for h in (1, hq))
 
 
 def _any_format(q, kv, softcap, window, alibi_slopes, key_starts) -> bool:
@@ -439,6 +448,8 @@ def attend(
     KIVI caches run the split kernel, then the merge kernel. `pdl=True` launches with programmatic dependent
     launch; `kv_ready=True` adds the promise that the lengths, block table and pools are not written by the
     kernel this call follows, so the persistent kernel starts copying pages before it waits on that kernel.
+    `workspace` (`attend_workspace`, of the batch's query heads and head dim; paged caches only) is the call's alone while it
+    runs; without one the device's and stream's is used.
 
     Paged caches of any kind take, and 16-bit pages ("bf16", "f16") or pages of other than 16 tokens always run, the any-format
     kernel with: `softcap` c > 0

@@ -32,6 +32,8 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
     A token that sees no key gets zeros; rows of q that belong to no sequence leave `out` as it is. q is f16 or bf16, of the
     pages' own dtype where they are 16-bit. A value that is NaN or infinite reaches every token of its sequence that shares a
     tile of rows with one that sees it; where no token sees it, it reaches none. `tokens` bounds the longest length (no host sync on lengths.max()).
+    `workspace`: `bpt_paged_prefill_workspace_bytes` bytes of any content (a workspace of `attend`'s that is large enough serves
+    too: its first 256 KiB, where `attend` keeps counters, are left alone).
     """
     device = require_cuda(q, kv.k_pool, kv.v_pool, kv.block_table, cu_seqlens, lengths, positions, alibi_slopes, key_starts,
                           prefix_lens, out, workspace)

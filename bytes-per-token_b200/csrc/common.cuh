@@ -37,6 +37,10 @@ void* tensor_map_encoder();
     if (!(cond)) return ::bpt::set_error(status, __VA_ARGS__); \
   } while (0)
 
+// The head of a workspace: the merge kernels' ticket counters (65,536 x u32), which every call leaves at zero. Reads that keep
+// no tickets leave it alone, so that one workspace serves all of them in turn.
+constexpr int64_t kTicketBytes = 65536 * 4;
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- device-side error flag ------------------------------------------------------------------------------------

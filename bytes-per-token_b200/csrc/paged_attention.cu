@@ -538,6 +538,7 @@ int paged_dispatch(const PagedArgs& a, int kind, int64_t D, int flags, cudaStrea
 // The split kernels count per sequence, the persistent kernel per (sequence, KV head).
 constexpr int64_t kMaxSeqs = 65536;
 constexpr int64_t kCounterBytes = kMaxSeqs * 4;
+static_assert(kCounterBytes == kTicketBytes, "what the reads without tickets leave alone");
 static_assert(kCounterBytes == kCounterBytesP, "one counter region for every merge kernel");
 static_assert(int64_t(kPersistMaxSeqs) * kMmaMaxHkv <= kMaxSeqs, "persistent tickets fit the counter region");
 

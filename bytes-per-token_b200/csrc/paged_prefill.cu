@@ -376,6 +376,7 @@ Plan plan_prefill(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int 
   return p;
 }
 
+// Of a workspace, behind the tickets of other reads: the tiles' counts of parts, the parts' sums, the parts.
 int64_t count_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * 4 + 255) / 256 * 256; }
 int64_t lse_bytes(const Plan& p, int64_t Hkv) { return (p.tiles * Hkv * p.n_splits * p.rows * 4 + 255) / 256 * 256; }
 
@@ -388,7 +389,7 @@ extern "C" int64_t bpt_paged_prefill_workspace_bytes(int64_t T, int64_t B, int64
                                                      int64_t tokens) {
   if (T < 1 || B < 1 || Hkv < 1 || Hq < Hkv || tokens < 1) return 0;
   const Plan p = plan_prefill(T, B, Hq, Hkv, D, kind, tokens);
-  return p.n_splits > 1 ? count_bytes(p, Hkv) + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
+  return p.n_splits > 1 ? kTicketBytes + count_bytes(p, Hkv) + lse_bytes(p, Hkv) + p.tiles * Hkv * p.n_splits * p.rows * D * 4 : 0;
 }
 
 extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
@@ -482,7 +483,7 @@ extern "C" int bpt_paged_prefill(const bpt_paged_prefill_args* args) {
     BPT_REQUIRE(aligned16(workspace), BPT_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", who);
     BPT_REQUIRE(workspace_bytes >= need, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
                 (long long)workspace_bytes, (long long)need);
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    uint8_t* ws = static_cast<uint8_t*>(workspace) + kTicketBytes;
     a.part_count = reinterpret_cast<int*>(ws);
     a.part_lse = reinterpret_cast<float*>(ws + count_bytes(p, Hkv));
     a.part_out = reinterpret_cast<float*>(ws + count_bytes(p, Hkv) + lse_bytes(p, Hkv));

@@ -533,14 +533,15 @@ int read_dim(const ReadArgs& a, int64_t D, bool merge, int flags, cudaStream_t s
 }
 
 struct ReadWorkspace {
-  int64_t meta, lse, total;  // offsets of the second and third part, the size
+  int64_t meta, lse, out, total;  // offsets of the three parts, behind the tickets of other reads; the size
 };
 ReadWorkspace read_workspace(int64_t Hq, int64_t Hkv, int64_t D, int kind) {
   const int64_t heads = Hkv * ((Hq / Hkv + 7) / 8), warps = read_ranges(heads, D, kind) * heads;
   ReadWorkspace w;
-  w.meta = (warps * 16 + 255) / 256 * 256;
-  w.lse = w.meta + (warps * 2 * 8 * 4 + 255) / 256 * 256;
-  w.total = w.lse + warps * 2 * 8 * D * 4;
+  w.meta = kTicketBytes;
+  w.lse = w.meta + (warps * 16 + 255) / 256 * 256;
+  w.out = w.lse + (warps * 2 * 8 * 4 + 255) / 256 * 256;
+  w.total = w.out + warps * 2 * 8 * D * 4;
   return w;
 }
 
@@ -683,9 +684,9 @@ extern "C" int bpt_paged_read(const bpt_paged_read_args* args) {
       BPT_REQUIRE(workspace_bytes >= w.total, BPT_ERR_WORKSPACE, "%s: workspace of %lld bytes, need %lld", who,
                   (long long)workspace_bytes, (long long)w.total);
       uint8_t* ws = static_cast<uint8_t*>(workspace);
-      a.ws_meta = reinterpret_cast<int4*>(ws);
-      a.ws_lse = reinterpret_cast<float*>(ws + w.meta);
-      a.ws_out = reinterpret_cast<float*>(ws + w.lse);
+      a.ws_meta = reinterpret_cast<int4*>(ws + w.meta);
+      a.ws_lse = reinterpret_cast<float*>(ws + w.lse);
+      a.ws_out = reinterpret_cast<float*>(ws + w.out);
     }
   } else {
     BPT_REQUIRE(lse_partial, BPT_ERR_INVALID, "%s: null output", who);

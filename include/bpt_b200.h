@@ -163,7 +163,7 @@ int bpt_paged_attend(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_s
  * recorded (device error 2), keys of a block out of range are left out and recorded.
  * With out_partial NULL: the merged attention out [B, Hq, D] in out_dtype. `tokens` bounds the longest length (it sizes the
  * launch, not the result); `workspace`: bpt_paged_read_workspace_bytes(...) bytes of any content, not shared by calls that
- * may overlap. Otherwise out_partial f32 [B, Hq, n_splits, D] and lse_partial f32 [B, Hq, n_splits] receive the parts (keys
+ * may overlap. Its first 256 KiB are not touched, so a workspace of bpt_paged_attend that is large enough serves both. Otherwise out_partial f32 [B, Hq, n_splits, D] and lse_partial f32 [B, Hq, n_splits] receive the parts (keys
  * [i split, (i + 1) split), the last part the rest; out 0, lse -inf where none is visible).
  * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024, split a multiple of 16.
  * Replaces: as bpt_paged_attend, for the reference's unquantized pages too (engine/kv_cache.py:98-169). */
