@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import functools
 import math
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -385,18 +386,20 @@ def attend_workspace(batch: int, q_heads: int, head_dim: int, n_splits: int, dev
     return ws
 
 
-_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+_LOCAL = threading.local()
 
 
 def _scratch(need: int, device: torch.device) -> torch.Tensor:
     """`need` bytes that nothing is kept in from one call to the next. While a CUDA graph is captured they are the graph's own,
-    so that two graphs never share them; otherwise the device's and stream's, grown on demand."""
+    so that two graphs never share them; otherwise the host thread's, for this device and stream, grown on demand: a call is
+    two launches that pass parts through them, and another thread's launches on the stream may come between."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(need, dtype=torch.uint8, device=device)
+    held = _LOCAL.__dict__
     key = (device.index, stream_of(device))
-    ws = _SCRATCH.get(key)
+    ws = held.get(key)
     if ws is None or ws.numel() < need:
-        ws = _SCRATCH[key] = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = held[key] = torch.empty(need, dtype=torch.uint8, device=device)
     return ws
 
 
@@ -449,7 +452,7 @@ def attend(
     launch; `kv_ready=True` adds the promise that the lengths, block table and pools are not written by the
     kernel this call follows, so the persistent kernel starts copying pages before it waits on that kernel.
     `workspace` (`attend_workspace`, of the batch's query heads and head dim; paged caches only) is the call's alone while it
-    runs; without one the device's and stream's is used.
+    runs; without one the call finds its own.
 
     Paged caches of any kind take, and 16-bit pages ("bf16", "f16") or pages of other than 16 tokens always run, the any-format
     kernel with: `softcap` c > 0
