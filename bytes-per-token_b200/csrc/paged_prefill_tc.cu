@@ -549,8 +549,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int w = warp - 4;
       const int32_t* table = a.src.block_table + int64_t(b) * a.src.bt_stride;
       const int take_from = max(from, lo);
-      auto block_at = [&](int key) -> int {  // -1: none is visible there, -2: the table names one out of range
-        if (key >= to) return -1;
+      // A step's pages: 64 / page size of them (one where pages are longer).
+      const int page_log2 = min(a.src.bs_log2, 6), per_log2 = 6 - page_log2, window_log2 = 5 - per_log2;
+      auto block_at = [&](int key) -> int {  // -1: no key is visible there, -2: the table names a block out of range
+        if (key >= to || key + (1 << page_log2) <= take_from) return -1;
         const int blk = table[key >> a.src.bs_log2];
         if (blk < 0 || blk >= a.src.num_blocks) {
           record_error(kDevErrBlockIndex);
@@ -558,9 +560,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         return blk;
       };
-      // A step's pages: 64 / page size of them (one where pages are longer). Lane i of a window holds page i mod per_step of
-      // step first + i / per_step; the next window is loaded while this one is in use.
-      const int page_log2 = min(a.src.bs_log2, 6), per_log2 = 6 - page_log2, window_log2 = 5 - per_log2;
+      // Lane i of a window holds page i mod per_step of step first + i / per_step; the next window is loaded while this one is
+      // in use.
       auto window = [&](int first) {
         const int back = steps - 1 - first - (lane >> per_log2);  // steps go from the last keys to the first
         return back < 0 ? -1 : block_at(from + (back << 6) + ((lane & ((1 << per_log2) - 1)) << page_log2));

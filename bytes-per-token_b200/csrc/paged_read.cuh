@@ -236,7 +236,8 @@ __device__ __forceinline__ void values16(uint32_t tile, int lane, const uint32_t
 // One warp's copies of groups of 16 keys from the pages into shared memory: its i-th group is keys first + step * i ..
 // first + step * i + 15 of KV head hk (`first`, `step` multiples of 16). Keys outside [from, to), and those of a block that
 // the table names out of range, are not read: their places hold zeros, and flag bits 0 (keys 0-7) and 1 (keys 8-15) tell
-// of bad blocks. Lane n holds the blocks of the group 32 i + n, so a group's rows need no load of the table.
+// of bad blocks. Entries of pages with no key in [from, to) are not looked at: a page given back behind a window may hold
+// anything there. Lane n holds the blocks of the group 32 i + n, so a group's rows need no load of the table.
 template <int KIND, int D>
 struct GroupLoader {
   static constexpr int RB = D * kElemBytes<KIND>;
@@ -259,8 +260,8 @@ struct GroupLoader {
     from = from_;
     to = to_;
   }
-  __device__ __forceinline__ int block_at(int key) const {
-    if (key >= to) return -1;
+  __device__ __forceinline__ int block_at(int key, int keys) const {  // of keys key .. key + keys - 1
+    if (key >= to || key + keys <= from) return -1;
     const int blk = table[key >> src.bs_log2];
     if (blk < 0 || blk >= src.num_blocks) {
       record_error(kDevErrBlockIndex);
@@ -273,8 +274,8 @@ struct GroupLoader {
     const bool two = src.bs_log2 == 3;  // pages of 8 keys: a group spans two
     if ((i & 31) == 0) {
       const int n = i + lane, key = first + step * n;
-      held = n < count ? block_at(key) : -1;
-      if (two) held2 = n < count ? block_at(key + 8) : -1;
+      held = n < count ? block_at(key, two ? 8 : 16) : -1;
+      if (two) held2 = n < count ? block_at(key + 8, 8) : -1;
     }
     const int key0 = first + step * i;
     const int blk = __shfl_sync(0xffffffffu, held, i & 31);
@@ -283,7 +284,7 @@ struct GroupLoader {
     const int64_t slot = (int64_t(max(blk, 0)) << src.bs_log2) + inside;
     const int64_t slot2 = two ? (int64_t(max(blk2, 0)) << 3) - 8 : slot;  // so that row r of the group is slot2 + r
     const int64_t at = slot * row_bytes + head_bytes, at2 = slot2 * row_bytes + head_bytes;
-    if (lane == 0) *flag = (blk < 0 && key0 < to ? 1u : 0u) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u);
+    if (lane == 0) *flag = (blk < 0 && key0 < to ? 1u : 0u) | (blk2 < 0 && key0 + 8 < to ? 2u : 0u);  // (or unseen)
     constexpr int CPR = RB / 16;
     const int r0 = lane / CPR, c0 = lane % CPR;  // this lane's chunk of the first rows; a pass of the warp takes STEP rows
     constexpr int STEP = CPR >= 32 ? 1 : 32 / CPR;
