@@ -30,8 +30,10 @@ def prefill_attend(q: torch.Tensor, kv: PagedQuantKV, cu_seqlens: torch.Tensor, 
     - `softcap` c > 0: scores become c * tanh(score / c); `alibi_slopes` [Hq]: they fall by slope * |p - j|.
 
     A token that sees no key gets zeros; rows of q that belong to no sequence leave `out` as it is. q is f16 or bf16, of the
-    pages' own dtype where they are 16-bit. A value that is NaN or infinite reaches every token of its sequence that shares a
-    tile of rows with one that sees it; where no token sees it, it reaches none. `tokens` bounds the longest length (no host sync on lengths.max()).
+    pages' own dtype where they are 16-bit. Tokens are taken in tiles of neighbours in their sequence (128 rows, 64 over INT8
+    pages; a token has a row per query head of a KV head). A value that is NaN or infinite reaches every token of a tile if its
+    key lies between the first and the last that the tile's tokens see, whether or not one of them sees it; before the first
+    and behind the last it reaches none. Table entries between those two have to name blocks of the pool. `tokens` bounds the longest length (no host sync on lengths.max()).
     `workspace`: `bpt_paged_prefill_workspace_bytes` bytes of any content (a workspace of `attend`'s that is large enough serves
     too: its first 256 KiB, where `attend` keeps counters, are left alone).
     """

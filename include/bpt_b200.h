@@ -200,7 +200,9 @@ int bpt_paged_read(const bpt_paged_read_args* args);
  * key_starts (int32 [T]: documents packed in one sequence), prefix_lens (int32 [B]: a prefix that all of its tokens see
  * whole) and alibi_slopes (fp32 [Hq]) may be NULL; softcap 0: no cap; window 0: no window. No visible key gives 0. out
  * [T, Hq, D] contiguous, in q's type. `tokens` bounds the longest length (it sizes the launch, not the result).
- * A value that is NaN or infinite spreads to every query whose tile reads its key, visible to it or not.
+ * A value that is NaN or infinite spreads to every query whose tile (128 neighbouring rows of a sequence, a row per token and
+ * query head of a KV head; 64 over int8 pages) reads its key, visible to it or not: all keys between the first and the last
+ * that the tile's rows see.
  * `workspace`: bpt_paged_prefill_workspace_bytes(...) bytes (0: none needed), as for bpt_paged_read.
  * Supported: D in {64, 128, 256}, any Hq / Hkv, block_size a power of two from 8 to 1024; rows of q start on 16 bytes.
  * Replaces: the prefill read of PagedKVCache + Attention.forward (engine/kv_cache.py:158-169, engine/attention.py:12-31). */
