@@ -10,7 +10,8 @@
 //
 // Every format but int8 takes csrc/paged_prefill_tc.cu. The kernel here serves int8 pages, whose scale per key goes on the
 // scores (a factor per column of S) and on the probabilities (a factor per column of P), so that the codes themselves are the
-// operands. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. It is bound by
+// operands. A power of two per row keeps a row's largest product of a probability and a scale in f16's range however small
+// the values are. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. It is bound by
 // the legacy matrix path and the conversion of the codes: the same design over bf16 pages took 467 us for twelve ragged prompts
 // where the tcgen05 kernel takes 120. This file also holds, for both kernels, the plan and the join: where there
 // are few tiles, each takes several CTAs, with a part of its keys each, and a second kernel, launched dependently, joins them.
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   }
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // a row's largest product of a probability and a value scale so far, and the power of two under which o holds them
+  float most[2] = {0.f, 0.f}, fit[2] = {1.f, 1.f};
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
@@ -212,28 +215,39 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
       const float shrink = exp2_approx(m[i2] - off[i2]);
       m[i2] = to_m;
       l[i2] *= shrink;
+      most[i2] *= shrink;
+      // the probabilities, and what they bring to the output: times their values' scales
+      float here = 0.f;
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) {
+        const __half2 vs = *reinterpret_cast<const __half2*>(scales_of(st, n >> 1) + 16 + 8 * (n & 1) + 2 * t);
+        const float x = exp2_approx(s[n][2 * i2] - off[i2]), y = exp2_approx(s[n][2 * i2 + 1] - off[i2]);
+        l[i2] += x + y;
+        s[n][2 * i2] = x * __low2float(vs);
+        s[n][2 * i2 + 1] = y * __high2float(vs);
+        here = fmaxf(here, fmaxf(s[n][2 * i2], s[n][2 * i2 + 1]));
+      }
+      here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 1));
+      here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 2));
+      most[i2] = fmaxf(most[i2], here);
+      const float to_fit = most[i2] > 0.f ? value_range(most[i2]) : fit[i2], change = shrink * (to_fit * inverse_power(fit[i2]));
+      fit[i2] = to_fit;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
-        o[n][2 * i2] *= shrink;
-        o[n][2 * i2 + 1] *= shrink;
+        o[n][2 * i2] *= change;
+        o[n][2 * i2 + 1] *= change;
       }
     }
 #pragma unroll
     for (int n = 0; n < kKeys / 16; ++n) {
-      // The probabilities enter the product rounded to 16 bits (as any operand of these matrix instructions); the sum that
-      // divides them is taken before the rounding, in fp32.
+      // They enter the product rounded to 16 bits (as any operand of these matrix instructions), a row's largest brought to
+      // [0.5, 1) by a power of two; the sum that divides them is taken before the rounding, in fp32.
       uint32_t p[4];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int i2 = 0; i2 < 2; ++i2) {
-          float x = exp2_approx(s[2 * n + k][2 * i2] - off[i2]), y = exp2_approx(s[2 * n + k][2 * i2 + 1] - off[i2]);
-          l[i2] += x + y;
-          const __half* vs = reinterpret_cast<const __half*>(scales_of(st, n)) + 16 + 8 * k + 2 * t;
-          x *= __half2float(vs[0]);
-          y *= __half2float(vs[1]);
-          p[2 * k + i2] = pack2<KIND>(x, y);
-        }
+        for (int i2 = 0; i2 < 2; ++i2)
+          p[2 * k + i2] = pack2<KIND>(s[2 * n + k][2 * i2] * fit[i2], s[2 * n + k][2 * i2 + 1] * fit[i2]);
       values16<KIND, D>(stage(st) + (kKeys + n * 16) * RB, lane, p, o);
     }
   }
@@ -243,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    inv[i] = l[i] == 0.f ? 0.f : a.src.v_scale / l[i];
+    inv[i] = l[i] == 0.f ? 0.f : inverse_power(fit[i]) / l[i];
   }
   if (parts <= 1) {
 #pragma unroll

@@ -14,6 +14,8 @@
 // The eight query heads fill only half of an MMA's 16 rows, so the other half carries what rounding takes off: rows 0-7 hold q
 // (then the probabilities) rounded to the product's 16-bit type, rows 8-15 the rounded-off rest, and both halves' sums
 // are added in fp32. Products are thus good to 16 (bf16) or 22 bits at no cost.
+// INT8 pages have a scale per key: K's goes on the score, V's on the probability, and a power of two per row keeps a row's
+// largest such product in f16's range however small the values are (5% of the time of 8 sequences of 32,768).
 //
 // A sequence inside one range goes straight to out. One that crosses ranges leaves a part per range, and a second kernel,
 // launched dependently, joins them.
@@ -298,6 +300,8 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
   const float mul = cap ? raw * 2.f * kLog2e / a.softcap : raw * kLog2e;
 
   float m = -INFINITY, l = 0.f;
+  // int8: the row's largest product of a probability and a value scale so far, and the power of two under which o holds them
+  float most = 0.f, fit = 1.f;
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
@@ -344,6 +348,7 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
       const float shrink = to_m == -INFINITY ? 1.f : exp2_approx(m - to_m);
       m = to_m;
       l *= shrink;
+      if constexpr (KIND == BPT_KV_INT8) most *= shrink;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -355,6 +360,24 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
       s[e] = exp2_approx(s[e] - off);
       l += s[e];
       s[e] *= vs[e];
+    }
+    if constexpr (KIND == BPT_KV_INT8) {
+      // The products enter the matrix operands between 2^-1 and 2^10 at a row's largest, where f16 and its rest keep 22 bits.
+      float top_p = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      top_p = fmaxf(top_p, __shfl_xor_sync(0xffffffffu, top_p, 1));
+      top_p = fmaxf(top_p, __shfl_xor_sync(0xffffffffu, top_p, 2));
+      most = fmaxf(most, top_p);
+      const float at = most * fit;
+      if (__any_sync(0xffffffffu, at > 1024.f || (at < 0.5f && most > 0.f))) {
+        const float to_fit = most > 0.f ? value_range(most) : fit, change = to_fit * inverse_power(fit);
+        fit = to_fit;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] *= change;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] *= fit;
     }
     uint32_t p[4];
     p[0] = pack2<KIND>(s[0], s[1]);
@@ -368,7 +391,7 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
   }
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
-  const float inv = l == 0.f ? 0.f : a.src.v_scale / l;
+  const float inv = l == 0.f ? 0.f : KIND == BPT_KV_INT8 ? inverse_power(fit) / l : a.src.v_scale / l;
   const float lse = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
   // where the rows go: straight to out, or to a part
   const int64_t row = int64_t(use.b) * a.Hq + h0 + g;

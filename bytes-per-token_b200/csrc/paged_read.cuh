@@ -353,6 +353,16 @@ __device__ __forceinline__ float2 unit_range(float amax) {
   return make_float2(__uint_as_float(uint32_t(127 - e) << 23), __uint_as_float(uint32_t(127 + e) << 23));
 }
 
+// The power of two that brings `most` > 0, a row's largest probability times the scale of its key's int8 values, to [0.5, 1):
+// scales of small values (max / 127 in f16) would otherwise take the products below what f16 holds. Between 2^-17 and 2^60, so
+// that ratios of two such powers, by which sums move from one to the next, stay in fp32's range.
+__device__ __forceinline__ float value_range(float most) {
+  const int e = min(max(int(__float_as_uint(most) >> 23) - 126, -60), 17);
+  return __uint_as_float(uint32_t(127 - e) << 23);
+}
+// 1 / f of a power of two, exactly.
+__device__ __forceinline__ float inverse_power(float f) { return __uint_as_float(0x7F000000u - __float_as_uint(f)); }
+
 // The checks and fields that every reader of a paged cache of any format shares.
 int paged_source(PagedSource& s, const char* who, const void* k_pool, const void* v_pool, int kind, float k_scale,
                  float v_scale, const void* k_scales, const void* v_scales, const int32_t* block_table, int64_t bt_stride,
