@@ -427,8 +427,9 @@ def _any_format(q, kv, softcap, window, alibi_slopes, key_starts) -> bool:
         return True
     if q.dim() != 3 or kv.k_pool.dim() != 4 or not kv.k_pool.shape[2] or q.shape[1] % kv.k_pool.shape[2]:
         return False
-    block_size, heads = kv.k_pool.shape[1:3]
-    return block_size != 16 or heads > 16 or q.shape[1] // heads not in (1, 2, 4, 8)
+    block_size, heads, dim = kv.k_pool.shape[1:]
+    # (two stages of 16 keys and values of more than 12 heads of 256 pass those kernels' shared memory)
+    return block_size != 16 or heads > (12 if dim == 256 else 16) or q.shape[1] // heads not in (1, 2, 4, 8)
 
 
 def attend(
