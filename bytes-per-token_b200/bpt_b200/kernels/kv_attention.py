@@ -432,6 +432,9 @@ def _any_format(q, kv, softcap, window, alibi_slopes, key_starts) -> bool:
     return block_size != 16 or heads > (12 if dim == 256 else 16) or q.shape[1] // heads not in (1, 2, 4, 8)
 
 
+_PAGED_LAUNCH = {"tokens", "split", "num_warps", "pdl", "kv_ready"}
+
+
 def attend(
     q: torch.Tensor,
     kv: QuantKV | PagedQuantKV,
@@ -448,19 +451,21 @@ def attend(
 ) -> torch.Tensor:
     """Decode attention over a cache: [B, Hq, D] (fp32 unless `out` says otherwise).
 
-    Paged caches run one fused launch: the splits of a sequence are merged by the last of its CTAs to finish.
-    KIVI caches run the split kernel, then the merge kernel. `pdl=True` launches with programmatic dependent
-    launch; `kv_ready=True` adds the promise that the lengths, block table and pools are not written by the
-    kernel this call follows, so the persistent kernel starts copying pages before it waits on that kernel.
-    `workspace` (`attend_workspace`, of the batch's query heads and head dim; paged caches only) is the call's alone while it
-    runs; without one the call finds its own.
+    FP8 and INT8 pages run one fused launch: the splits of a sequence are merged by the last of its CTAs to finish.
+    KIVI caches run the split kernel, then the merge kernel. `launch`: `tokens` and `split` as in `decode_attention`
+    (the any-format kernel below cuts its work by itself, whatever `split`). Over paged caches `pdl=True` launches
+    with programmatic dependent launch; `kv_ready=True` adds the promise that the lengths, block table and pools are
+    not written by the kernel this call follows, so the persistent kernel starts copying pages before it waits on
+    that kernel (the others wait). `workspace` (`attend_workspace`, of the batch's query heads and head dim; paged
+    caches only) is the call's alone while it runs; without one the call finds its own.
 
-    Paged caches of any kind take, and 16-bit pages ("bf16", "f16") or pages of other than 16 tokens always run, the any-format
-    kernel with: `softcap` c > 0
-    (scores c * tanh(score / c)), `window` w > 0 (only the last w keys are seen), `alibi_slopes` fp32 [Hq] (a score falls
-    by slope * distance) and `key_starts` int32 [B] (the first key each sequence sees). A sequence that sees no key
-    gives zeros.
+    Paged caches of any kind take, and 16-bit pages ("bf16", "f16") or pages of other than 16 tokens always run, the
+    any-format kernel (two launches) with: `softcap` c > 0 (scores c * tanh(score / c)), `window` w > 0 (only the last
+    w keys are seen), `alibi_slopes` fp32 [Hq] (a score falls by slope * distance) and `key_starts` int32 [B] (the
+    first key each sequence sees). A sequence that sees no key gives zeros.
     """
+    if isinstance(kv, PagedQuantKV) and not launch.keys() <= _PAGED_LAUNCH:
+        raise TypeError(f"attend has no argument {', '.join(sorted(launch.keys() - _PAGED_LAUNCH))}")
     if _any_format(q, kv, softcap, window, alibi_slopes, key_starts):
         return _paged_read(q, kv, lengths, scale, tokens=launch.get("tokens"), split=launch.get("split"), softcap=softcap,
                            window=window, alibi_slopes=alibi_slopes, key_starts=key_starts, out=out, workspace=workspace,
