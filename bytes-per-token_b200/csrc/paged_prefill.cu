@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) paged_prefill_kernel(const PrefillAr
 #pragma unroll
     for (int n = 0; n < kKeys / 16; ++n) {
       // They enter the product rounded to 16 bits (as any operand of these matrix instructions), a row's largest brought to
-      // [0.5, 1) by a power of two; the sum that divides them is taken before the rounding, in fp32.
+      // [2^9, 2^10) by a power of two; the sum that divides them is taken before the rounding, in fp32.
       uint32_t p[4];
 #pragma unroll
       for (int k = 0; k < 2; ++k)

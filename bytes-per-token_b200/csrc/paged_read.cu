@@ -13,7 +13,8 @@
 //
 // The eight query heads fill only half of an MMA's 16 rows, so the other half carries what rounding takes off: rows 0-7 hold q
 // (then the probabilities) rounded to the product's 16-bit type, rows 8-15 the rounded-off rest, and both halves' sums
-// are added in fp32. Products are thus good to 16 (bf16) or 22 bits at no cost.
+// are added in fp32. Products are thus good to 16 (bf16) or 22 bits at no cost; f16 probabilities stand at up to 2^15, so that
+// a long tail far below the largest keeps its bits too.
 // INT8 pages have a scale per key: K's goes on the score, V's on the probability, and a power of two per row keeps a row's
 // largest such product in f16's range however small the values are (5% of the time of 8 sequences of 32,768).
 //
@@ -277,6 +278,9 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
     request(i);
     if (i < NST - 2) place(i);
   }
+  // Powers are taken of s - (m - kLift): the largest P is 2^15, so that of f16 products a P of 2^-29 of it still has 11 bits
+  // (bf16 has the range anyway; int8 pages bring theirs into range below).
+  constexpr float kLift = KIND == BPT_KV_F16 || KIND == BPT_KV_FP8 ? 15.f : 0.f;
   const bool cap = a.softcap > 0.f;
   const float cap_out = a.softcap * kLog2e;
   const float slope = a.slopes && g < heads ? a.slopes[h0 + g] * kLog2e : 0.f;
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
     if (bad & 2u) s[2] = s[3] = -INFINITY;
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - kLift;
     if (__any_sync(0xffffffffu, top > m)) {
       const float to_m = fmaxf(m, top);
       const float shrink = to_m == -INFINITY ? 1.f : exp2_approx(m - to_m);
@@ -362,13 +366,14 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
       s[e] *= vs[e];
     }
     if constexpr (KIND == BPT_KV_INT8) {
-      // The products enter the matrix operands between 2^-1 and 2^10 at a row's largest, where f16 and its rest keep 22 bits.
+      // The products enter the matrix operands between 2^9 and 2^15 at a row's largest, where f16 and its rest keep 22 bits
+      // of it, and 11 of one 2^-23 as large.
       float top_p = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
       top_p = fmaxf(top_p, __shfl_xor_sync(0xffffffffu, top_p, 1));
       top_p = fmaxf(top_p, __shfl_xor_sync(0xffffffffu, top_p, 2));
       most = fmaxf(most, top_p);
       const float at = most * fit;
-      if (__any_sync(0xffffffffu, at > 1024.f || (at < 0.5f && most > 0.f))) {
+      if (__any_sync(0xffffffffu, at > 32768.f || (at < 512.f && most > 0.f))) {
         const float to_fit = most > 0.f ? value_range(most) : fit, change = to_fit * inverse_power(fit);
         fit = to_fit;
 #pragma unroll

@@ -353,12 +353,12 @@ __device__ __forceinline__ float2 unit_range(float amax) {
   return make_float2(__uint_as_float(uint32_t(127 - e) << 23), __uint_as_float(uint32_t(127 + e) << 23));
 }
 
-// The power of two that brings `most` > 0, a row's largest probability times the scale of its key's int8 values, to [0.5, 1):
-// scales of small values (max / 127 in f16) would otherwise take the products below what f16 holds. Between 2^-17 and 2^60, so
-// that ratios of two such powers, by which sums move from one to the next, stay in fp32's range.
+// The power of two that brings `most` > 0, a row's largest probability times the scale of its key's int8 values, to
+// [2^9, 2^10): scales of small values (max / 127 in f16) would otherwise take the products below what f16 holds. Between 2^-7
+// and 2^70, so that ratios of two such powers, by which sums move from one to the next, stay in fp32's range.
 __device__ __forceinline__ float value_range(float most) {
   const int e = min(max(int(__float_as_uint(most) >> 23) - 126, -60), 17);
-  return __uint_as_float(uint32_t(127 - e) << 23);
+  return __uint_as_float(uint32_t(137 - e) << 23);
 }
 // 1 / f of a power of two, exactly.
 __device__ __forceinline__ float inverse_power(float f) { return __uint_as_float(0x7F000000u - __float_as_uint(f)); }

@@ -158,8 +158,8 @@ int bpt_paged_attend(const void* q, int q_dtype, int64_t q_stride_b, int64_t q_s
 /* Decode attention over a paged cache of any format (BPT_KV_*), with the masks and score changes of current models. Query b
  * sits at position p = lengths[b] - 1 and sees the keys j with max(0, key_starts[b], p - window + 1) <= j <= p:
  *   s_j = softcap tanh(sm_scale q.k_j / softcap) - alibi_slopes[head] (p - j)
- * softcap 0: no cap; window 0: no window; key_starts (int32 [B]) and alibi_slopes (fp32 [Hq]) may be NULL. No visible key
- * gives 0. block_table int32 [B, bt_width], row stride bt_stride; a length beyond the table's pages is cut to them and
+ * softcap 0: no cap (a capped score is good to a few 2^-24 of the cap); window 0: no window; key_starts (int32 [B]) and
+ * alibi_slopes (fp32 [Hq]) may be NULL. No visible key gives 0. block_table int32 [B, bt_width], row stride bt_stride; a length beyond the table's pages is cut to them and
  * recorded (device error 2), keys of a block out of range are left out and recorded.
  * With out_partial NULL: the merged attention out [B, Hq, D] in out_dtype. `tokens` bounds the longest length (it sizes the
  * launch, not the result); `workspace`: bpt_paged_read_workspace_bytes(...) bytes of any content, not shared by calls that
@@ -200,6 +200,7 @@ int bpt_paged_read(const bpt_paged_read_args* args);
  * key_starts (int32 [T]: documents packed in one sequence), prefix_lens (int32 [B]: a prefix that all of its tokens see
  * whole) and alibi_slopes (fp32 [Hq]) may be NULL; softcap 0: no cap; window 0: no window. No visible key gives 0. out
  * [T, Hq, D] contiguous, in q's type. `tokens` bounds the longest length (it sizes the launch, not the result).
+ * Probabilities are rounded to 16 bits, over f16 and E4M3 pages to f16 (one below 2^-25 of its row's largest is lost).
  * A value that is NaN or infinite spreads to every query whose tile (128 neighbouring rows of a sequence, a row per token and
  * query head of a KV head; 64 over int8 pages) reads its key, visible to it or not: all keys between the first and the last
  * that the tile's rows see.
