@@ -20,7 +20,9 @@
 // by an m that lags. A step thus takes no maximum: one pass from S to P and its sum, and O in tensor memory is rescaled a few
 // times per row, if at all. Over f16 and E4M3 pages P is f16, whose smallest step is 2^-24: a power below 2^-25 is lost, N
 // keys lose at most N 2^-25 of the largest value. (Powers of s - m + 4 or + 8 would reach that much further down, but leave m as
-// much less room to lag: heads of 256, capped, 198 and 221 us instead of 168.)
+// much less room to lag: heads of 256, capped, 198 and 221 us instead of 168.) Without cap and bias a power's exponent is one
+// fused product less the rounded m, off by m's rounding for all keys of a row alike: that is only a common factor of P and
+// its sum, and stays in f16's range for scores below 2^27.
 //
 // Measured (B200: 1,646 TFLOP/s bf16 by library product, 6,558 GB/s copy): a prompt of 8,192 tokens, 32 + 8 heads of 128,
 // bf16: 486 us back to back, 1,131 TFLOP/s. There the exponentials (16 a clock per SM) and the products ask for about the same

@@ -278,8 +278,9 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
     request(i);
     if (i < NST - 2) place(i);
   }
-  // Powers are taken of s - (m - kLift): the largest P is 2^15, so that of f16 products a P of 2^-29 of it still has 11 bits
-  // (bf16 has the range anyway; int8 pages bring theirs into range below).
+  // Powers are taken of s - m with m the largest score less kLift: the largest P is 2^15, so that of f16 products a P of 2^-29
+  // of it still has 11 bits (bf16 has the range anyway; int8 pages bring theirs into range below). Beyond 2^22, where fp32 would
+  // round that difference, m is the score itself; m never falls, so no P passes 2^15 either way.
   constexpr float kLift = KIND == BPT_KV_F16 || KIND == BPT_KV_FP8 ? 15.f : 0.f;
   const bool cap = a.softcap > 0.f;
   const float cap_out = a.softcap * kLog2e;
@@ -346,7 +347,8 @@ __global__ void __launch_bounds__(32 * kWarps, ReadShape<KIND, D>::kCtas) paged_
     if (bad & 2u) s[2] = s[3] = -INFINITY;
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - kLift;
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (kLift > 0.f && fabsf(top) < 4194304.f) top -= kLift;
     if (__any_sync(0xffffffffu, top > m)) {
       const float to_m = fmaxf(m, top);
       const float shrink = to_m == -INFINITY ? 1.f : exp2_approx(m - to_m);
