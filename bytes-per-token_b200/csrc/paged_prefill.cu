@@ -12,8 +12,8 @@
 // scores (a factor per column of S) and on the probabilities (a factor per column of P), so that the codes themselves are the
 // operands. A power of two per row keeps a row's largest product of a probability and a scale in f16's range however small
 // the values are. It multiplies with mma.sync: 64 rows per CTA (16 per warp), 64 keys per step, two cp.async stages. It is bound by
-// the legacy matrix path and the conversion of the codes: the same design over bf16 pages took 467 us for twelve ragged prompts
-// where the tcgen05 kernel takes 120. This file also holds, for both kernels, the plan and the join: where there
+// the latency of the legacy products and the codes' conversion at 8 warps an SM (no pipe above 19%): twelve ragged prompts, 16 + 8
+// heads of 128, 676 us (B200), where the tcgen05 kernel takes 124 over bf16 pages. This file also holds, for both kernels, the plan and the join: where there
 // are few tiles, each takes several CTAs, with a part of its keys each, and a second kernel, launched dependently, joins them.
 #include "paged_prefill.cuh"
 

@@ -24,13 +24,14 @@
 // fused product less the rounded m, off by m's rounding for all keys of a row alike: that is only a common factor of P and
 // its sum, and stays in f16's range for scores below 2^27.
 //
-// Measured (B200: 1,646 TFLOP/s bf16 by library product, 6,558 GB/s copy): a prompt of 8,192 tokens, 32 + 8 heads of 128,
-// bf16: 486 us back to back, 1,131 TFLOP/s. There the exponentials (16 a clock per SM) and the products ask for about the same
-// time, and each step's chain S -> P -> O has to hide behind the other CTA's. Ragged batches are bound by what is not the loop:
-// about 9 us per CTA for its map, first pages, queries and rows out. 256 rows in one CTA per SM took 713 us for that
-// prompt, pages by cp.async warps 1,128, a box per 64 dims 687, K and V by one warp 565; a polynomial in place of a
-// quarter of the exponentials 576 against 572. E4M3: two chunks of about 1,800 tokens over 4,500, 16 + 4 heads of 128, 236 us
-// (bf16 157): the two converting warps.
+// Measured (B200: 1,647 TFLOP/s bf16 by library product in a burst, 1,405 sustained; 6,558 GB/s copy): a prompt of 8,192 tokens,
+// 32 + 8 heads of 128, bf16: 511 us by itself (1,076 TFLOP/s), 550 to 567 when calls follow each other, at 1,570 MHz under the
+// power limit (980 TFLOP/s). Products and exponentials each fill 57% of their pipe; a step's chain S -> P -> O has to hide
+// behind the other CTA's. Ragged batches (12 prompts of 17 to 2,000: 124 us) are bound by what is not the loop: about 9 us per
+// CTA for its map, first pages, queries and rows out. Heads of 256, capped, 4,096 tokens in a window of 1,024: 166 us, one CTA
+// an SM. E4M3: two chunks of about 1,800 tokens over 2,700, 16 + 4 heads of 128, 200 us (bf16 133): the two converting warps.
+// For that prompt, on the way here: 256 rows in one CTA per SM 713 us; 128 rows with a box per 64 dims 687, a box per page
+// 565, K and V by warps of their own 538; a polynomial in place of a quarter of the exponentials 576 where 572 was without.
 //
 // Every wait is bounded; a thread whose wait runs out records it and leaves its loop, the others follow by their own limits,
 // and the CTA still awaits its copies and products, frees its tensor memory and returns.
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       } else {
         // Warp 6 brings the codes, 8 keys a TMA box, a lane a box, into the second half of the place that their f16 values
         // take; warps 4 and 5 then take four of the eight places each, two at a time: codes into registers, f16 back. (One
-        // warp that both brought and converted left the ring empty while it waited: two chunks of about 1,800 tokens 357 us, not 236.)
+        // warp that both brought and converted left the ring empty while it waited: heads of 128 took half as long again.)
         constexpr int CPR = D / 16, PER = CPR * 8 / 32;  // 16-byte chunks of a key's codes; a lane's of 8 keys
         auto order = [&](int n, int& j, bool& v) {
           v = is_v(n) || n >= 2 * steps - 1;

@@ -21,10 +21,11 @@
 // A sequence inside one range goes straight to out. One that crosses ranges leaves a part per range, and a second kernel,
 // launched dependently, joins them.
 //
-// Measured (B200, 6,558 GB/s copy): f16, 8 sequences of 32,768, 32 query and 8 KV heads of 128, capped: 186 us, 5.8 TB/s;
-// bf16, 32 sequences of 512 to 4,096: 63 us, 4.8 TB/s (start and join); E4M3 in a window of 4,096, 17 sequences: 33 us, bound
-// by the codes' conversion; one sequence of 1,000: 15 us, two launches and a dependent chain of loads. A ring of six stages
-// with one CTA an SM took 73 us for the batch of 32, twelve warps an SM 37 for the E4M3 one.
+// Measured (B200, 6,558 GB/s copy; captured): f16, 8 sequences of 32,768, 32 query and 8 KV heads of 128, capped: 186 us,
+// 5.8 TB/s (INT8 156 us, 3.5 TB/s); bf16, 32 sequences of 512 to 4,096: 62 us, 4.9 TB/s (start and join); E4M3 in a window of
+// 4,096, 17 sequences: 32 us, 1.8 TB/s, bound by the latency of a warp's chain at 8 warps an SM (0.3 instructions a cycle, no
+// pipe above 14%); one sequence of 1,000: 14 us, two launches and a dependent chain of loads. A ring of six stages with one
+// CTA an SM took 73 us for the batch of 32.
 #include <algorithm>
 
 #include "paged_read.cuh"
@@ -524,7 +525,7 @@ int launch(const void* kernel, dim3 grid, int threads, int smem, bool dependent,
 }
 
 // The most ranges of a merged read: as many as give every warp of a full GPU one head of one range (two CTAs per SM, one at
-// 16-bit heads of 256; three CTAs of 8-bit heads of 128 measured 37 us where two take 35).
+// 16-bit heads of 256; three CTAs of 8-bit heads of 128 took 37 us where two took 35).
 int64_t read_ranges(int64_t heads, int64_t D, int kind) {
   const bool wide = D == 256 && (kind == BPT_KV_F16 || kind == BPT_KV_BF16);
   return std::max<int64_t>(int64_t(num_sms()) * (wide ? 1 : 2) * kWarps / heads, 1);

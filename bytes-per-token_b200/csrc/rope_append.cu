@@ -16,9 +16,10 @@
 // 64, 128, 256) and a warp 32 / (D / 16) heads of one token at a time. A warp takes `per_warp` such groups of one
 // token, keeping the token's cos and sin in registers.
 //
-// Measured (B200, 6,558 GB/s copy): 8,192 tokens of 16 + 8 + 8 heads of 128 with norms into bf16 pages 39 us, 3.6 TB/s (the
-// floor is 21 us: loads of a warp's groups follow one another, and registers leave 32 warps an SM; with 40 by
-// __launch_bounds__ 35 us, but 2,001 tokens into E4M3 pages 10.5 us instead of 8); 64 tokens 4.4 us, launch and latency.
+// Measured (B200, 6,558 GB/s copy): 8,192 tokens of 16 + 8 + 8 heads of 128 with norms into bf16 pages 38 us, 3.6 TB/s (the
+// floor is 21 us: a warp's groups load one after another, and 71 registers leave 24 warps an SM; held to 40 warps by
+// __launch_bounds__ 35 us, but 2,001 tokens into E4M3 pages 10.5 us instead of 8); into INT8 pages 62 us (the head's maximum
+// and the quotients on top); 64 tokens 4.2 us, launch and latency.
 #include "common.cuh"
 
 namespace bpt {
