@@ -221,6 +221,9 @@ class PagedQuantizedKVCache:
         rotation and the scores' options are those of `rope_kv_append`, `attend` and `prefill_attend`; 16-bit pages take
         queries of their own dtype where several tokens come at once. Returns [B, Hq, Q, D] in q's dtype.
         """
+        takes = (_SIXTEEN[self.kind],) if self.kind in _SIXTEEN else (torch.float16, torch.bfloat16)
+        if meta.q_len > 1 and q.dtype not in takes:  # (before anything is stored)
+            raise ValueError(f"several tokens over {self.kind!r} pages take queries of {' or '.join(map(str, takes))}, got {q.dtype}")
         kv = self.layer_view(layer, meta)
         tokens = [x.transpose(1, 2).flatten(0, 1) for x in (q, k, v)]  # [B * Q, H, D]
         turned = rope_kv_append(*tokens, kv, meta.positions, cos, sin, meta.write_blocks, meta.write_offsets, q_norm=q_norm,
